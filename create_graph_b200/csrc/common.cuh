@@ -74,4 +74,9 @@ int csr_build_launch(const int32_t* index, int64_t n, int64_t rows, int32_t* row
                      cudaStream_t s);
 }  // namespace seg
 
+namespace dense {
+// the device error word of the half-precision products (dense.cu)
+int device_error(int* out, bool reset);
+}  // namespace dense
+
 }  // namespace cg

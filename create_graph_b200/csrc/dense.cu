@@ -1,0 +1,566 @@
+// Half-precision dense layer: y = f(x W^T + b) + r in one product with a fused
+// epilogue, and the elementwise passes of its first and second derivatives.
+//
+//   z = x W^T + b,  y = f(z) + r,  f one of identity, relu, silu, gelu (erf)
+//   gz = gy f'(z);  dx = gz W;  dW = gz^T x;  db = sum over rows of gz;  dr = gy
+//   second order, given cotangents h of gz and hb of db:
+//     d gy = (h + hb) f'(z),  d z = (h + hb) gy f''(z)
+//
+// Products accumulate in fp32 (half_gemm.cuh); the activation, bias and
+// residual are applied to the fp32 accumulator, which is rounded to the
+// half-precision output once. z is kept in the layer's own type for the
+// backward: its rounding (2^-9 relative in bf16) is of the size of the rounding
+// of y itself.
+#include <math.h>
+
+#include "half_gemm.cuh"
+#include "../../include/cg_b200.h"
+
+namespace cg {
+namespace dense {
+
+// device error word of this translation unit's kernels
+__device__ int g_dense_error = 0;
+
+// ---- half-precision values ---------------------------------------------------
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ float2 unpack2(uint32_t u, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t u, __nv_bfloat16) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(w[i], T());
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+}
+
+// ---- activations ---------------------------------------------------------------
+// The hardware-approximated exp and division (about 1e-6 relative, far below
+// the 2^-9 or 2^-11 of the output's rounding) keep the epilogue warps ahead of
+// the tensor cores; exp overflowing to infinity gives 0, the limit.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float act(float z, int kind) {
+  if (kind == CG_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
+  if (kind == CG_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+  if (kind == CG_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  return z;
+}
+__device__ __forceinline__ float act_grad(float z, int kind) {
+  if (kind == CG_ACT_SILU) {
+    const float s = sigmoid(z);
+    return s * (1.0f + z * (1.0f - s));
+  }
+  if (kind == CG_ACT_GELU)  // Phi(z) + z phi(z)
+    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  return 1.0f;
+}
+__device__ __forceinline__ float act_grad2(float z, int kind) {
+  if (kind == CG_ACT_SILU) {
+    const float s = sigmoid(z);
+    return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
+  }
+  if (kind == CG_ACT_GELU) return 0.39894228f * __expf(-0.5f * z * z) * (2.0f - z * z);
+  return 0.0f;
+}
+
+// ---- epilogue --------------------------------------------------------------------
+struct EpiArgs {
+  void* y;
+  int64_t ld_y;
+  const void* bias;      // (n,) or null
+  const void* residual;  // (m, n) or null
+  int64_t ld_res;
+  void* z;               // (m, n): pre-activation out, or null
+  int64_t ld_z;
+  float* partial;        // split-K: raw fp32 tiles, (splits, m, n)
+  int act;
+  int vec;               // 16-byte groups of 8 columns: n, pitches multiples of 8, pointers aligned
+};
+
+template <class T>
+struct Epi {
+  using Args = EpiArgs;
+  struct Aux {
+    uint4 r[4];
+  };
+  const EpiArgs& a;
+  int m, n, split;
+  __device__ Epi(const EpiArgs& args, int m_, int n_, int /*batch*/, int split_)
+      : a(args), m(m_), n(n_), split(split_) {}
+  static __device__ int* error_word() { return &g_dense_error; }
+
+  // lane -> rows (lane >> 2) + 8 i, columns 8 (lane & 3) .. + 7 of the block
+  __device__ void fetch(Aux& aux, int row0, int col0, int lane) const {
+    if (a.residual == nullptr || !a.vec || a.partial) return;
+    const int col = col0 + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + (lane >> 2) + 8 * i;
+      aux.r[i] = row < m && col < n
+                     ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ld_res + col)
+                     : make_uint4(0, 0, 0, 0);
+    }
+  }
+  // eight columns of one row: bias, pre-activation, activation, residual
+  __device__ __forceinline__ void finish8(float (&v)[8], const float (&bias)[8], const uint4& res, int64_t row,
+                                          int col) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
+    if (a.z) *reinterpret_cast<uint4*>(static_cast<T*>(a.z) + row * a.ld_z + col) = pack8<T>(v);
+    if (a.act == CG_ACT_SILU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act(v[e], CG_ACT_SILU);
+    } else if (a.act == CG_ACT_GELU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act(v[e], CG_ACT_GELU);
+    } else if (a.act == CG_ACT_RELU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act(v[e], CG_ACT_RELU);
+    }
+    if (a.residual) {
+      float r[8];
+      unpack8<T>(res, r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += r[e];
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.ld_y + col) = pack8<T>(v);
+  }
+  __device__ __forceinline__ void load_bias8(float (&b)[8], int col) const {
+    if (a.bias) {
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + col)), b);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void finish1(float v, int64_t row, int col) const {
+    if (a.bias) v += to_float(static_cast<const T*>(a.bias)[col]);
+    if (a.z) static_cast<T*>(a.z)[row * a.ld_z + col] = from_float<T>(v);
+    v = act(v, a.act);
+    if (a.residual) v += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]);
+    static_cast<T*>(a.y)[row * a.ld_y + col] = from_float<T>(v);
+  }
+  __device__ void store(const Aux& aux, const float* stage, int row0, int col0, int lane) const {
+    if (a.vec) {
+      const int c = (lane & 3) * 8, col = col0 + c;
+      if (col >= n) return;
+      float bias[8];
+      if (!a.partial) load_bias8(bias, col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (lane >> 2) + 8 * i;
+        const int64_t row = row0 + r;
+        if (row >= m) break;
+        float v[8];
+        half::stage_read8(stage, r, c, v);
+        if (a.partial) {
+          float4* p = reinterpret_cast<float4*>(a.partial + ((int64_t)split * m + row) * n + col);
+          p[0] = make_float4(v[0], v[1], v[2], v[3]);
+          p[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          finish8(v, bias, aux.r[i], row, col);
+        }
+      }
+    } else {
+      // unaligned or ragged outputs: one column per lane, one row per step
+      const int col = col0 + lane;
+      if (col >= n) return;
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r) {
+        const int64_t row = row0 + r;
+        if (row >= m) break;
+        const float v = stage[half::stage_idx(r, lane)];
+        if (a.partial) a.partial[((int64_t)split * m + row) * n + col] = v;
+        else finish1(v, row, col);
+      }
+    }
+  }
+};
+
+// Joins the k-splits in split order (the same sum every run) and finishes the
+// elements as the epilogue does.
+template <class T>
+__global__ void join_splits_kernel(EpiArgs a, int splits, int m, int n) {
+  const float* partial = a.partial;
+  a.partial = nullptr;
+  const Epi<T> epi(a, m, n, 0, 0);
+  const int64_t mn = (int64_t)m * n, stride = (int64_t)gridDim.x * blockDim.x;
+  const int64_t first = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (a.vec) {
+    const int n8 = n / 8;
+    for (int64_t i = first; i < mn / 8; i += stride) {
+      const int64_t row = i / n8;
+      const int col = (int)(i % n8) * 8;
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (int s = 0; s < splits; ++s) {
+        const float4* p = reinterpret_cast<const float4*>(partial + s * mn + i * 8);
+        const float4 x = __ldg(p), y = __ldg(p + 1);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+      float bias[8];
+      epi.load_bias8(bias, col);
+      const uint4 res = a.residual ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) +
+                                                                      row * a.ld_res + col)
+                                   : make_uint4(0, 0, 0, 0);
+      epi.finish8(v, bias, res, row, col);
+    }
+  } else {
+    for (int64_t i = first; i < mn; i += stride) {
+      float v = 0.0f;
+      for (int s = 0; s < splits; ++s) v += partial[s * mn + i];
+      epi.finish1(v, i / n, (int)(i % n));
+    }
+  }
+}
+
+// ---- elementwise passes of the derivatives -----------------------------------------
+// gz = gy f'(z) and the column sums of gz (the bias gradient) in one pass over
+// gy and z: block (x, y) owns 32 x V columns and the rows of chunk y; its eight
+// warps walk the rows, each lane adding up V columns in fp32, and the warps'
+// sums meet in shared memory in warp order. V = 8 (16-byte groups) or 1.
+template <class T, int V>
+__global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
+                                                       const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
+                                                       int64_t ld_gz, int rows, int cols, int kind, int rows_per,
+                                                       float* __restrict__ partial) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (blockIdx.x * 32 + lane) * V;
+  const int r0 = blockIdx.y * rows_per, r1 = min(rows, r0 + rows_per);
+  float sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum[e] = 0.0f;
+  if (col < cols) {
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      float g[V], x[V];
+      if constexpr (V == 8) {
+        unpack8<T>(*reinterpret_cast<const uint4*>(gy + r * ld_gy + col), g);
+        if (gz) unpack8<T>(*reinterpret_cast<const uint4*>(z + r * ld_z + col), x);
+      } else {
+        g[0] = to_float(gy[r * ld_gy + col]);
+        if (gz) x[0] = to_float(z[r * ld_z + col]);
+      }
+      if (gz) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[e] *= act_grad(x[e], kind);
+        if constexpr (V == 8) *reinterpret_cast<uint4*>(gz + r * ld_gz + col) = pack8<T>(g);
+        else gz[r * ld_gz + col] = from_float<T>(g[0]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[e] += g[e];
+    }
+  }
+  if (partial == nullptr) return;
+  __shared__ float sums[8][32 * V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sums[warp][lane * V + e] = sum[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * V; c += 256) {
+    const int at = blockIdx.x * 32 * V + c;
+    if (at >= cols) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][c];
+    partial[(int64_t)blockIdx.y * cols + at] = s;
+  }
+}
+
+// db[c] = sum of the chunks' sums in chunk order, rounded once.
+template <class T>
+__global__ void join_columns_kernel(const float* __restrict__ partial, int chunks, int cols, T* __restrict__ db) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < chunks; ++i) s += partial[(int64_t)i * cols + c];
+  db[c] = from_float<T>(s);
+}
+
+// Second order: t = h + hb; dgy = t f'(z), dz = t gy f''(z).
+template <class T>
+__global__ void act_grad2_kernel(const T* __restrict__ h, const T* __restrict__ hb, const T* __restrict__ gy,
+                                 const T* __restrict__ z, T* __restrict__ dgy, T* __restrict__ dz, int64_t rows,
+                                 int cols, int kind) {
+  const int64_t n = rows * cols, stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += stride) {
+    const float t = (h ? to_float(h[i]) : 0.0f) + (hb ? to_float(hb[i % cols]) : 0.0f);
+    const float x = to_float(z[i]);
+    dgy[i] = from_float<T>(t * act_grad(x, kind));
+    dz[i] = from_float<T>(t * to_float(gy[i]) * act_grad2(x, kind));
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Plan {
+  int cg, bn, splits, kt_per;
+};
+
+// Tile and k-split of a product.
+static Plan plan_of(const cg_linear_args& g) {
+  const int64_t sms = sm_count();
+  const int64_t kts = ceil_div<int64_t>(g.k, half::kBK);
+  struct Shape {
+    int cg, bn;
+    double clocks, fixed;
+  };
+  static const Shape shapes[] = {{2, 256, 560, 1500}, {2, 128, 320, 1300}, {1, 128, 330, 1200}, {1, 64, 230, 1000}};
+  Plan best = {1, 64, 1, (int)kts};
+  double least = 0.0;
+  for (const Shape& s : shapes) {
+    const int64_t tiles = ceil_div<int64_t>(g.m, s.cg * half::kRows) * ceil_div<int64_t>(g.n, s.bn);
+    const int64_t slots = sms / s.cg;
+    int64_t most = slots / tiles < kts / 4 ? slots / tiles : kts / 4;
+    for (int64_t splits = 1; splits <= (most < 1 ? 1 : most); ++splits) {
+      const int64_t per = ceil_div<int64_t>(kts, splits);
+      const int64_t used = ceil_div<int64_t>(kts, per);
+      if (used != splits) continue;
+      const int64_t waves = ceil_div<int64_t>(tiles * splits, slots);
+      double cost = (double)waves * ((double)per * s.clocks + s.fixed);
+      if (splits > 1) cost += 4000.0 + (double)splits * g.m * g.n * 8.0 / 2500.0;
+      if (least == 0.0 || cost < least) {
+        least = cost;
+        best = {s.cg, s.bn, (int)splits, (int)per};
+      }
+    }
+  }
+  return best;
+}
+
+static int64_t workspace_bytes(const cg_linear_args& g) {
+  const Plan p = plan_of(g);
+  return p.splits > 1 ? (int64_t)p.splits * g.m * g.n * (int64_t)sizeof(float) : 0;
+}
+
+template <int CG, int BN, class T>
+static int launch(const cg_linear_args& g, const Plan& p, const EpiArgs& ea, bool bf16, cudaStream_t s) {
+  half::Launch<EpiArgs> L;
+  memset(&L, 0, sizeof(L));
+  L.groups = 1;
+  L.bf16 = bf16;
+  auto& G = L.g[0];
+  int rc;
+  if ((rc = half::make_half_map(&G.map_a, g.a, bf16, g.a_mn_major ? g.k : g.m, g.a_mn_major ? g.m : g.k, g.lda, 1,
+                                g.lda * (g.a_mn_major ? g.k : g.m), g.a_mn_major != 0, half::kRows)))
+    return rc;
+  if ((rc = half::make_half_map(&G.map_b, g.b, bf16, g.b_mn_major ? g.k : g.n, g.b_mn_major ? g.n : g.k, g.ldb, 1,
+                                g.ldb * (g.b_mn_major ? g.k : g.n), g.b_mn_major != 0, BN / CG)))
+    return rc;
+  G.m = (int)g.m;
+  G.n = (int)g.n;
+  G.k = (int)g.k;
+  G.batch = 1;
+  G.a_mn = g.a_mn_major;
+  G.b_mn = g.b_mn_major;
+  G.splits = p.splits;
+  G.kt_per = p.kt_per;
+  G.epi = ea;
+  const int64_t items = half::plan_group<CG, BN>(G);
+  CG_REQUIRE(items < (1ll << 31), "linear_half: too many tiles");
+  L.items = (int)items;
+  return half::launch_half_gemm<CG, BN, 1, Epi<T>>(L, s);
+}
+
+template <class T>
+static int run_typed(const cg_linear_args& g, bool bf16, cudaStream_t s) {
+  int rc;
+  if ((rc = half::bind_context())) return rc;
+  const Plan p = plan_of(g);
+  EpiArgs ea;
+  ea.y = g.y;
+  ea.ld_y = g.ld_y;
+  ea.bias = g.bias;
+  ea.residual = g.residual;
+  ea.ld_res = g.ld_residual;
+  ea.z = g.z;
+  ea.ld_z = g.ld_z;
+  ea.act = g.act;
+  ea.partial = nullptr;
+  ea.vec = g.n % 8 == 0 && g.ld_y % 8 == 0 && aligned16(g.y) && (g.bias == nullptr || aligned16(g.bias)) &&
+           (g.residual == nullptr || (aligned16(g.residual) && g.ld_residual % 8 == 0)) &&
+           (g.z == nullptr || (aligned16(g.z) && g.ld_z % 8 == 0));
+  if (p.splits > 1) {
+    CG_REQUIRE(g.workspace != nullptr && aligned16(g.workspace) && g.workspace_bytes >= workspace_bytes(g),
+               "linear_half: this shape splits K %d ways and needs %lld workspace bytes on a 16-byte boundary "
+               "(cg_linear_half_workspace_bytes)",
+               p.splits, (long long)workspace_bytes(g));
+    ea.partial = g.workspace;
+  }
+  if (p.cg == 2 && p.bn == 256) rc = launch<2, 256, T>(g, p, ea, bf16, s);
+  else if (p.cg == 2) rc = launch<2, 128, T>(g, p, ea, bf16, s);
+  else if (p.bn == 128) rc = launch<1, 128, T>(g, p, ea, bf16, s);
+  else rc = launch<1, 64, T>(g, p, ea, bf16, s);
+  if (rc || p.splits == 1) return rc;
+  const int64_t work = ceil_div<int64_t>(g.m * g.n, ea.vec ? 8 : 1);
+  const int64_t blocks = ceil_div<int64_t>(work, 256);
+  const int64_t most = (int64_t)sm_count() * 8;
+  join_splits_kernel<T><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(ea, p.splits, (int)g.m, (int)g.n);
+  CG_LAUNCHED("linear_half split join");
+  return kOk;
+}
+
+static int run(const cg_linear_args* args, void* stream) {
+  CG_REQUIRE(args != nullptr, "linear_half: args is NULL");
+  const cg_linear_args& g = *args;
+  CG_REQUIRE(g.dtype == CG_F16 || g.dtype == CG_BF16, "linear_half: dtype %d is neither CG_F16 nor CG_BF16", g.dtype);
+  CG_REQUIRE(g.act == CG_ACT_NONE || g.act == CG_ACT_SILU || g.act == CG_ACT_RELU || g.act == CG_ACT_GELU,
+             "linear_half: bad act %d", g.act);
+  CG_REQUIRE(g.m >= 0 && g.n >= 0 && g.k >= 0, "linear_half: negative size");
+  if (g.m == 0 || g.n == 0) return kOk;
+  CG_REQUIRE(g.k >= 1, "linear_half: k must be >= 1");
+  const int64_t most = (1ll << 31) - 512;  // tile coordinates are 32-bit
+  CG_REQUIRE(g.m < most && g.n < most && g.k < most, "linear_half: size too large");
+  CG_REQUIRE(g.a && g.b && g.y, "linear_half: a, b and y must be non-null");
+  CG_REQUIRE(aligned16(g.a) && aligned16(g.b), "linear_half: a and b must be 16-byte aligned");
+  CG_REQUIRE(g.lda % 8 == 0 && g.ldb % 8 == 0, "linear_half: lda and ldb must be multiples of 8 values");
+  CG_REQUIRE(g.lda >= (g.a_mn_major ? g.m : g.k) && g.ldb >= (g.b_mn_major ? g.n : g.k) && g.ld_y >= g.n &&
+                 (g.residual == nullptr || g.ld_residual >= g.n) && (g.z == nullptr || g.ld_z >= g.n),
+             "linear_half: row pitch smaller than the row");
+  if (g.dtype == CG_F16) return run_typed<__half>(g, false, as_stream(stream));
+  return run_typed<__nv_bfloat16>(g, true, as_stream(stream));
+}
+
+// Row chunks of act_grad: enough blocks to fill the SMs several times, each of
+// at least 32 rows.
+static int chunk_rows(int64_t rows, int64_t cols, int v) {
+  const int64_t strips = ceil_div<int64_t>(cols, 32 * v);
+  int64_t chunks = ceil_div<int64_t>((int64_t)sm_count() * 8, strips);
+  int64_t per = ceil_div<int64_t>(rows, chunks);
+  per = ceil_div<int64_t>(per < 32 ? 32 : per, 8) * 8;
+  const int64_t least = ceil_div<int64_t>(rows, 65535);  // gridDim.y
+  return (int)(per < least ? least : per);
+}
+
+template <class T>
+static int act_grad_typed(const cg_act_grad_args& g, cudaStream_t s) {
+  const bool vec = g.cols % 8 == 0 && aligned16(g.gy) && g.ld_gy % 8 == 0 &&
+                   (g.gz == nullptr || (aligned16(g.z) && aligned16(g.gz) && g.ld_z % 8 == 0 && g.ld_gz % 8 == 0));
+  const int per = chunk_rows(g.rows, g.cols, vec ? 8 : 1);
+  const int chunks = (int)ceil_div<int64_t>(g.rows, per);
+  const dim3 grid((unsigned)ceil_div<int64_t>(g.cols, vec ? 256 : 32), (unsigned)chunks);
+  float* partial = g.db ? g.scratch : nullptr;
+  if (vec)
+    act_grad_kernel<T, 8><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
+                                               (int)g.rows, (int)g.cols, g.act, per, partial);
+  else
+    act_grad_kernel<T, 1><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
+                                               (int)g.rows, (int)g.cols, g.act, per, partial);
+  CG_LAUNCHED("act_grad_half");
+  if (g.db) {
+    join_columns_kernel<T><<<(unsigned)ceil_div<int64_t>(g.cols, 128), 128, 0, s>>>(partial, chunks, (int)g.cols,
+                                                                                    (T*)g.db);
+    CG_LAUNCHED("act_grad_half column join");
+  }
+  return kOk;
+}
+
+static int64_t act_grad_scratch(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  int64_t most = 0;
+  for (int v : {1, 8}) {
+    const int64_t chunks = ceil_div<int64_t>(rows, chunk_rows(rows, cols, v));
+    if (chunks > most) most = chunks;
+  }
+  return most * cols * (int64_t)sizeof(float);
+}
+
+static int act_grad_run(const cg_act_grad_args* args, void* stream) {
+  CG_REQUIRE(args != nullptr, "act_grad_half: args is NULL");
+  const cg_act_grad_args& g = *args;
+  CG_REQUIRE(g.dtype == CG_F16 || g.dtype == CG_BF16, "act_grad_half: dtype %d is neither CG_F16 nor CG_BF16",
+             g.dtype);
+  CG_REQUIRE(g.rows >= 0 && g.cols >= 0 && g.rows < (1ll << 31) - 512 && g.cols < (1ll << 31) - 512,
+             "act_grad_half: bad size");
+  if (g.rows == 0 || g.cols == 0) {
+    // a sum over no rows
+    if (g.db && g.cols > 0) CG_CUDA(cudaMemsetAsync(g.db, 0, (size_t)g.cols * 2, as_stream(stream)));
+    return kOk;
+  }
+  CG_REQUIRE(g.gy != nullptr && (g.gz == nullptr || g.z != nullptr), "act_grad_half: null input");
+  CG_REQUIRE(g.gz != nullptr || g.db != nullptr, "act_grad_half: no output asked for");
+  CG_REQUIRE(g.ld_gy >= g.cols && (g.gz == nullptr || (g.ld_z >= g.cols && g.ld_gz >= g.cols)),
+             "act_grad_half: row pitch smaller than the row");
+  CG_REQUIRE(g.db == nullptr || (g.scratch != nullptr && g.scratch_bytes >= act_grad_scratch(g.rows, g.cols)),
+             "act_grad_half: the column sums need %lld scratch bytes (cg_act_grad_half_scratch_bytes)",
+             (long long)act_grad_scratch(g.rows, g.cols));
+  if (g.dtype == CG_F16) return act_grad_typed<__half>(g, as_stream(stream));
+  return act_grad_typed<__nv_bfloat16>(g, as_stream(stream));
+}
+
+template <class T>
+static int act_grad2_typed(const void* h, const void* hb, const void* gy, const void* z, void* dgy, void* dz,
+                           int64_t rows, int64_t cols, int act, cudaStream_t s) {
+  const int64_t blocks = ceil_div<int64_t>(rows * cols, 256), most = (int64_t)sm_count() * 16;
+  act_grad2_kernel<T><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
+      (const T*)h, (const T*)hb, (const T*)gy, (const T*)z, (T*)dgy, (T*)dz, rows, (int)cols, act);
+  CG_LAUNCHED("act_grad2_half");
+  return kOk;
+}
+
+int device_error(int* out, bool reset) {
+  CG_CUDA(cudaMemcpyFromSymbol(out, g_dense_error, sizeof(int)));
+  const int zero = 0;
+  if (reset) CG_CUDA(cudaMemcpyToSymbol(g_dense_error, &zero, sizeof(int)));
+  return kOk;
+}
+
+}  // namespace dense
+}  // namespace cg
+
+extern "C" {
+
+int cg_linear_half(const cg_linear_args* args, void* stream) { return cg::dense::run(args, stream); }
+
+int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args) {
+  if (args == nullptr || args->m <= 0 || args->n <= 0 || args->k <= 0) return 0;
+  return cg::dense::workspace_bytes(*args);
+}
+
+int cg_act_grad_half(const cg_act_grad_args* args, void* stream) { return cg::dense::act_grad_run(args, stream); }
+
+int64_t cg_act_grad_half_scratch_bytes(int64_t rows, int64_t cols) { return cg::dense::act_grad_scratch(rows, cols); }
+
+int cg_act_grad2_half(const void* h, const void* hb, const void* gy, const void* z, void* dgy, void* dz, int64_t rows,
+                      int64_t cols, int act, int dtype, void* stream) {
+  using namespace cg;
+  CG_REQUIRE(dtype == CG_F16 || dtype == CG_BF16, "act_grad2_half: dtype %d is neither CG_F16 nor CG_BF16", dtype);
+  CG_REQUIRE(rows >= 0 && cols >= 0 && cols < (1ll << 31), "act_grad2_half: bad size");
+  if (rows == 0 || cols == 0) return kOk;
+  CG_REQUIRE((h || hb) && gy && z && dgy && dz, "act_grad2_half: null buffer");
+  if (dtype == CG_F16)
+    return dense::act_grad2_typed<__half>(h, hb, gy, z, dgy, dz, rows, cols, act, as_stream(stream));
+  return dense::act_grad2_typed<__nv_bfloat16>(h, hb, gy, z, dgy, dz, rows, cols, act, as_stream(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,504 @@
+// Half-precision tensor-core products with a fused epilogue: the main loop that
+// the dense layer (dense.cu) and the Newton-Schulz products (muon.cu) share.
+//
+//   D(m, n) = sum_k A(m, k) B(n, k),  fp32 accumulation in TMEM (kind::f16)
+//
+// Persistent: one CTA (CG = 1) or a pair of CTAs on two SMs (CG = 2, one
+// cta_group::2 accumulator tile of 256 rows) per SM or SM pair walks work items
+// (group, batch entry, m-tile, n-tile, k-split):
+//   warp 0      TMA producer: k-slices of 64 values (one 128-byte swizzle row)
+//               of A and B into a ring of shared-memory stages;
+//   warp 1      one thread issues the UMMAs (K = 16) of a stage, commits the
+//               stage back to the producers and each finished accumulator to
+//               the epilogue (two accumulators: an item's epilogue runs beside
+//               the next item's products);
+//   warps 2..9  epilogue: tcgen05.ld (thread = row), a transpose through
+//               shared memory, then 16-byte row segments in and out.
+// Operands are K-major (contiguous along k) or MN-major (contiguous along m or
+// n), so x W^T, g W and g^T x read their operands as they are stored.
+// PLANES = 2: every operand is a pair of fp16 planes hi + lo (22 significant
+// bits) and a k-slice makes the products lo hi + hi lo + hi hi; the dropped
+// lo lo term is 2^-22 relative.
+// A pair of SMs halves the B bytes each SM stages per flop: a 256 x 256 tile
+// takes 32 KB of shared memory per 64-wide slice and SM against 48 KB for the
+// 128 x 256 tile of one SM, which is what lets six stages fit.
+// Every wait is bounded: on timeout the kernel records an error in the
+// translation unit's error word, lets its copies land and unwinds.
+#pragma once
+
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace cg {
+namespace half {
+
+using namespace cg::sm100;
+
+constexpr int kBK = 64;        // half-precision values per k-slice: 128 bytes
+constexpr int kRows = 128;     // accumulator rows per CTA
+constexpr int kEpiWarps = 8;   // two per TMEM lane quarter
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kMaxGroups = 8;  // problems of different shapes in one launch
+
+// Bounded wait: 2^24 polls are about half a second at the least, hundreds of
+// times the longest tile.
+__device__ inline bool wait(uint64_t* bar, uint32_t parity, int* error_word) {
+  return mbar_wait(bar, parity, error_word, 1u << 24);
+}
+
+// ---- PTX of the cta_group::2 forms -----------------------------------------
+__device__ inline uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ inline void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrive on the barrier at this shared-memory offset in CTA `rank` of the cluster.
+__device__ inline void mbar_arrive_remote(uint64_t* bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(rank)
+      : "memory");
+}
+template <int CG>
+__device__ inline void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  if (CG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  } else {
+    // both CTAs of the pair report to the leader's barrier (bit 24 of the
+    // shared-window address is the CTA's place in the pair)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  }
+}
+template <int CG>
+__device__ inline void tmem_alloc_cg(uint32_t* slot, uint32_t cols) {
+  if (CG == 1) {
+    tmem_alloc(slot, cols);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ inline void tmem_dealloc_cg(uint32_t taddr, uint32_t cols) {
+  if (CG == 1) tmem_dealloc(taddr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+template <int CG>
+__device__ inline void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  if (CG == 1) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  }
+}
+// Arrive on `bar` (in both CTAs of a pair) once this thread's UMMAs have completed.
+template <int CG>
+__device__ inline void umma_commit_cg(uint64_t* bar) {
+  if (CG == 1) {
+    umma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+
+// Instruction descriptor of kind::f16 with fp32 accumulation; both operands
+// have the same type (bf16 or fp16).
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4)                         // D format: f32
+         | ((bf16 ? 1u : 0u) << 7)         // A format: f16 / bf16
+         | ((bf16 ? 1u : 0u) << 10)        // B format
+         | ((a_mn_major ? 1u : 0u) << 15)  // A major
+         | ((b_mn_major ? 1u : 0u) << 16)  // B major
+         | ((uint32_t)(n >> 3) << 17)      // N / 8
+         | ((uint32_t)(m >> 4) << 24);     // M / 16
+}
+
+// ---- tiles ------------------------------------------------------------------
+template <int CG, int BN, int PLANES>
+struct Tile {
+  static constexpr int kBRows = BN / CG;                       // B rows this CTA stages
+  static constexpr int kA = kRows * kBK * 2;
+  static constexpr int kB = kBRows * kBK * 2;
+  static constexpr int kStage = PLANES * (kA + kB);
+  static constexpr int kStaging = kEpiWarps * 32 * 32 * 4;     // one 32 x 32 fp32 block per epilogue warp
+  static constexpr int kStagesFit = (227 * 1024 - kStaging - 1024 - 512) / kStage;
+  static constexpr int kStages = kStagesFit < 8 ? kStagesFit : 8;
+  static constexpr int kBytes = kStages * kStage + kStaging + 1024 /*alignment*/ + 512 /*barriers*/;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static_assert(kBRows % 64 == 0, "MN-major boxes are 64 wide");
+  static_assert(kStages >= 3 && kTmemCols <= 512, "tile");
+};
+
+// One problem of a launch: `batch` products of one shape.
+template <class EpiArgs>
+struct Group {
+  CUtensorMap map_a, map_b;  // 3-D: (contiguous, rows, batch entry x plane)
+  int m, n, k;
+  int m_tiles, n_tiles;      // in tiles of CG * 128 x BN
+  int batch;
+  int a_mn, b_mn;            // MN-major operands
+  int splits, kt_per;        // k-slices per split
+  int n_fast;                // consecutive items walk n first
+  int lower;                 // symmetric result: only tiles that reach the lower triangle
+  int tiles;                 // items per batch entry and split
+  int first_item;
+  EpiArgs epi;
+};
+
+template <class EpiArgs>
+struct Launch {
+  Group<EpiArgs> g[kMaxGroups];
+  int groups, items;
+  int bf16;
+};
+
+struct Item {
+  int g, batch, split, m0, n0, kt0, kt1;
+};
+
+// Tiles of a symmetric result that reach its lower triangle: row block i (of
+// `bm` rows) holds those with n0 <= m0 + bm - 1.
+__host__ __device__ inline int lower_tiles_of_row(int i, int bm, int bn, int n_tiles) {
+  const int c = ((i + 1) * bm + bn - 1) / bn;
+  return c < n_tiles ? c : n_tiles;
+}
+
+template <int BM, int BN, class EpiArgs>
+__device__ inline Item item_of(const Launch<EpiArgs>& L, int w) {
+  Item it;
+  it.g = 0;
+  while (it.g + 1 < L.groups && w >= L.g[it.g + 1].first_item) ++it.g;
+  const Group<EpiArgs>& g = L.g[it.g];
+  w -= g.first_item;
+  int t = w % g.tiles;
+  w /= g.tiles;
+  it.batch = w % g.batch;
+  it.split = w / g.batch;
+  int mt, nt;
+  if (g.lower) {
+    mt = 0;
+    int c;
+    while (t >= (c = lower_tiles_of_row(mt, BM, BN, g.n_tiles))) {
+      t -= c;
+      ++mt;
+    }
+    nt = t;
+  } else if (g.n_fast) {
+    nt = t % g.n_tiles;
+    mt = t / g.n_tiles;
+  } else {
+    mt = t % g.m_tiles;
+    nt = t / g.m_tiles;
+  }
+  it.m0 = mt * BM;
+  it.n0 = nt * BN;
+  const int kt_all = (g.k + kBK - 1) / kBK;
+  it.kt0 = it.split * g.kt_per;
+  it.kt1 = it.kt0 + g.kt_per < kt_all ? it.kt0 + g.kt_per : kt_all;
+  return it;
+}
+
+// Place of column c of row r in a warp's staged 32 x 32 block: the row's eight
+// 16-byte chunks are XOR-swizzled by (r & 7), so row-per-lane writes and
+// 8-columns-per-lane reads are free of bank conflicts.
+__device__ __forceinline__ int stage_idx(int r, int c) { return r * 32 + ((((c >> 2) ^ (r & 7)) << 2) | (c & 3)); }
+
+__device__ __forceinline__ void stage_read8(const float* stage, int r, int c, float (&v)[8]) {
+  const float4 x = *reinterpret_cast<const float4*>(stage + stage_idx(r, c));
+  const float4 y = *reinterpret_cast<const float4*>(stage + stage_idx(r, c + 4));
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+}
+
+// Epi: Epi::Args (kernel parameter), Epi::Aux (values prefetched for one 32 x 32
+// block), Epi(args, m, n, batch entry, split), fetch(aux, row0, col0, lane),
+// store(aux, stage, row0, col0, lane) and error_word() (the translation unit's).
+template <int CG, int BN, int PLANES, class Epi>
+__global__ void __launch_bounds__(kThreads, 1)
+    half_gemm_kernel(const __grid_constant__ Launch<typename Epi::Args> L) {
+  using T = Tile<CG, BN, PLANES>;
+  constexpr int BM = CG * kRows;
+  constexpr int STAGES = T::kStages;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  // 128-byte swizzled tiles need 1024-byte alignment
+  unsigned char* tiles = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* staging = reinterpret_cast<float*>(tiles + STAGES * T::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + STAGES * T::kStage + T::kStaging);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], CG * kEpiWarps);  // one arrival per epilogue warp of the pair
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc_cg<CG>(tmem_slot, T::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();  // the peer's barriers exist before anything reports to them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  int* const error_word = Epi::error_word();
+  bool ok = true;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer (each CTA of a pair loads its own rows) ----------------
+    uint32_t it = 0;
+    for (int w = first; w < L.items && ok; w += step) {
+      const Item item = item_of<BM, BN>(L, w);
+      const auto& g = L.g[item.g];
+      const int m0 = item.m0 + (int)rank * kRows, n0 = item.n0 + (int)rank * T::kBRows;
+      for (int kt = item.kt0; kt < item.kt1; ++kt, ++it) {
+        const int s = it % STAGES;
+        const uint32_t round = it / STAGES;
+        if (it >= STAGES && !(ok = wait(&empty[s], (round - 1) & 1, error_word))) break;
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * T::kStage);
+        const int k0 = kt * kBK;
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+          unsigned char* sa = tiles + s * T::kStage + p * (T::kA + T::kB);
+          unsigned char* sb = sa + T::kA;
+          const int z = item.batch * PLANES + p;
+          if (!g.a_mn) {
+            tma_load_3d<CG>(sa, &g.map_a, &full[s], k0, m0, z);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kRows / 64; ++c)
+              tma_load_3d<CG>(sa + c * (kBK * 128), &g.map_a, &full[s], m0 + 64 * c, k0, z);
+          }
+          if (!g.b_mn) {
+            tma_load_3d<CG>(sb, &g.map_b, &full[s], k0, n0, z);
+          } else {
+#pragma unroll
+            for (int c = 0; c < T::kBRows / 64; ++c)
+              tma_load_3d<CG>(sb + c * (kBK * 128), &g.map_b, &full[s], n0 + 64 * c, k0, z);
+          }
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---------------- UMMA issuer (the pair's leader) ----------------
+    uint32_t it = 0;
+    int j = 0;
+    for (int w = first; w < L.items && ok; w += step, ++j) {
+      const Item item = item_of<BM, BN>(L, w);
+      const auto& g = L.g[item.g];
+      const uint32_t idesc = idesc_f16(BM, BN, L.bf16 != 0, g.a_mn != 0, g.b_mn != 0);
+      // K-major: 8-row groups 1024 B apart, 16 values along k = 32 B. MN-major:
+      // 64-wide m (n) blocks kBK * 128 B apart, 8-deep k groups 1024 B apart,
+      // 16 along k = two groups.
+      const uint32_t a_lbo = g.a_mn ? kBK * 128 : 16, a_step = g.a_mn ? 2048 : 32;
+      const uint32_t b_lbo = g.b_mn ? kBK * 128 : 16, b_step = g.b_mn ? 2048 : 32;
+      const int b = j & 1, use = j >> 1;
+      if (use > 0 && !(ok = wait(&acc_empty[b], (use - 1) & 1, error_word))) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + b * BN;
+      for (int kt = item.kt0; kt < item.kt1; ++kt, ++it) {
+        const int s = it % STAGES;
+        if (!(ok = wait(&full[s], (it / STAGES) & 1, error_word))) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(tiles + s * T::kStage), sb = sa + T::kA;
+        auto da = [&](int p, int kk) {
+          return smem_desc(sa + p * (T::kA + T::kB) + kk * a_step, a_lbo, 1024, kSwizzle128B);
+        };
+        auto db = [&](int p, int kk) {
+          return smem_desc(sb + p * (T::kA + T::kB) + kk * b_step, b_lbo, 1024, kSwizzle128B);
+        };
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk) {
+          const bool on = kt > item.kt0 || kk > 0;
+          if (PLANES == 2) {  // the small cross terms first, then the hi product
+            umma_f16<CG>(acc, da(1, kk), db(0, kk), idesc, on);
+            umma_f16<CG>(acc, da(0, kk), db(1, kk), idesc, true);
+            umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, true);
+          } else {
+            umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, on);
+          }
+        }
+        umma_commit_cg<CG>(&empty[s]);
+      }
+      umma_commit_cg<CG>(&acc_full[b]);
+    }
+  } else if (warp >= 2) {
+    // ---------------- epilogue ----------------
+    // Warp e of a TMEM lane quarter (32 rows) takes alternate 32-column blocks.
+    const int quarter = warp & 3, e = warp - 2;
+    float* stage = staging + e * (32 * 32);
+    int j = 0;
+    for (int w = first; w < L.items; w += step, ++j) {
+      const Item item = item_of<BM, BN>(L, w);
+      const auto& g = L.g[item.g];
+      const Epi epi(g.epi, g.m, g.n, item.batch, item.split);
+      const int row0 = item.m0 + (int)rank * kRows + quarter * 32;
+      const int b = j & 1, use = j >> 1;
+      typename Epi::Aux aux;
+      const int c_first = 32 * (e >> 2);
+      epi.fetch(aux, row0, item.n0 + c_first, lane);  // beside the wait for the accumulator
+      if (!(ok = wait(&acc_full[b], use & 1, error_word))) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = c_first; c0 < BN; c0 += 64) {
+        float v[32];
+        tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c0, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<float4*>(stage + stage_idx(lane, 4 * q)) =
+              make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        __syncwarp();
+        typename Epi::Aux next;
+        if (c0 + 64 < BN) epi.fetch(next, row0, item.n0 + c0 + 64, lane);
+        epi.store(aux, stage, row0, item.n0 + c0, lane);
+        __syncwarp();
+        aux = next;
+      }
+      // the accumulator may be overwritten once every epilogue warp has read it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) mbar_arrive_remote(&acc_empty[b], 0);
+        else mbar_arrive(&acc_empty[b]);
+      }
+    }
+  }
+  // after a timeout, the copies and products still in flight get time to land
+  // before the shared memory and TMEM they use are given back
+  if (!ok)
+    for (int i = 0; i < 1000; ++i) __nanosleep(2000);
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync_all();  // neither CTA leaves while its peer may report to it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_cg<CG>(tmem, T::kTmemCols);
+  }
+}
+
+// ---- host side ----------------------------------------------------------------
+inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// The driver's encoder needs a current context; threads such as autograd's
+// backward workers may not have bound the runtime's primary context yet.
+inline int bind_context() {
+  int dev = 0;
+  CG_CUDA(cudaGetDevice(&dev));
+  CG_CUDA(cudaSetDevice(dev));
+  return kOk;
+}
+
+// 3-D tensor map over `planes` matrices of `rows` x `cols` half-precision values
+// (row pitch ld, matrix pitch `stride`, in values). mn: 64-wide boxes of kBK
+// rows (k along the rows), else kBK-wide boxes of `box_rows` rows.
+inline int make_half_map(CUtensorMap* map, const void* ptr, bool bf16, int64_t rows, int64_t cols, int64_t ld,
+                         int64_t planes, int64_t stride, bool mn, int box_rows) {
+  auto fn = encode_fn();
+  CG_REQUIRE(fn != nullptr, "half gemm: cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(stride * 2)};
+  cuuint32_t box[3] = {(cuuint32_t)kBK, (cuuint32_t)(mn ? kBK : box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CG_REQUIRE(r == CUDA_SUCCESS, "half gemm: cuTensorMapEncodeTiled failed (%d): rows %lld cols %lld ld %lld", (int)r,
+             (long long)rows, (long long)cols, (long long)ld);
+  return kOk;
+}
+
+// Fill in a group's tile counts; the caller has set m, n, k, batch, splits,
+// kt_per and lower. Returns its items.
+template <int CG, int BN, class EpiArgs>
+int64_t plan_group(Group<EpiArgs>& g) {
+  constexpr int BM = CG * kRows;
+  g.m_tiles = (g.m + BM - 1) / BM;
+  g.n_tiles = (g.n + BN - 1) / BN;
+  // walk the shorter side first: a wave of tiles then shares whole rows of
+  // tiles of the longer operand, each read once, and the other operand in L2
+  g.n_fast = g.n_tiles <= g.m_tiles;
+  int64_t tiles = (int64_t)g.m_tiles * g.n_tiles;
+  if (g.lower) {
+    tiles = 0;
+    for (int i = 0; i < g.m_tiles; ++i) tiles += lower_tiles_of_row(i, BM, BN, g.n_tiles);
+  }
+  g.tiles = (int)tiles;
+  return tiles * g.batch * g.splits;
+}
+
+template <int CG, int BN, int PLANES, class Epi>
+int launch_half_gemm(const Launch<typename Epi::Args>& L, cudaStream_t stream) {
+  using T = Tile<CG, BN, PLANES>;
+  auto kernel = half_gemm_kernel<CG, BN, PLANES, Epi>;
+  CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));
+  const int slots = sm_count() / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CG * (L.items < slots ? L.items : slots)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = T::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  CG_CUDA(cudaLaunchKernelEx(&cfg, kernel, L));
+  CG_LAUNCHED("half_gemm");
+  return kOk;
+}
+
+}  // namespace half
+}  // namespace cg

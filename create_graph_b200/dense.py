@@ -1,0 +1,281 @@
+"""
+The half-precision dense layer: y = f(x W^T + b) + r in one product.
+
+    y = dense.linear(x, weight, bias, activation="silu", residual=r)
+
+bf16 or fp16 tensors, fp32 accumulation on the tcgen05 tensor cores, bias,
+activation and residual applied to the fp32 accumulator and rounded once
+(``cg_linear_half``). ``activation`` is "none", "relu", "silu" or "gelu" (the
+erf form). x is (..., K), weight (N, K), bias (N,), residual (..., N); all have
+one dtype. Transposed and row-strided views of x and weight are read in place
+when their rows start on 16-byte boundaries; others are copied once.
+
+The op is differentiable twice, as the force pass of ``cg.create_graph`` needs:
+
+    gz = gy f'(z);  dx = gz W;  dW = gz^T x;  db = sum of gz;  dr = gy
+
+with gz and db formed in one pass over gy and the kept pre-activation z, the
+gradients as products of the same kernel, and the second order (f'') as an
+explicit kernel. gz is rounded to the layer's dtype before the two products,
+as every operand of the tensor cores is. Without a gradient to prepare, z is
+not written. The fp32 layers of the energy network are in
+``create_graph_b200.nn``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import Tensor, nn
+
+from create_graph_b200 import native
+from create_graph_b200.compile_config import engine_will_execute
+from create_graph_b200.errors import NativeError
+from create_graph_b200.nn import _edges, _Fused
+
+ACTIVATIONS = {"none": native.ACT_NONE, "relu": native.ACT_RELU, "silu": native.ACT_SILU, "gelu": native.ACT_GELU}
+
+
+def _pitched(rows: int, cols: int, like: Tensor) -> Tensor:
+    """An uninitialised (rows, cols) matrix whose rows start on 16-byte boundaries."""
+    pitch = -(-cols // 8) * 8
+    out = torch.empty(rows, pitch, dtype=like.dtype, device=like.device)
+    return out if pitch == cols else out[:, :cols]
+
+
+def _fits_tma(t: Tensor, row: int, col: int) -> bool:
+    """Whether t, contiguous along dimension ``col``, can be read in place by
+    TMA: 16-byte aligned base and row pitch, rows that do not overlap."""
+    pitch = t.stride(row) if t.shape[row] > 1 else -(-t.shape[col] // 8) * 8
+    return (t.stride(col) == 1 or t.shape[col] == 1) and pitch % 8 == 0 and pitch >= t.shape[col] \
+        and t.data_ptr() % 16 == 0
+
+
+def _operand(t: Tensor) -> tuple[Tensor, int, bool]:
+    """(tensor, row pitch, MN-major) of a logical (rows, K) operand."""
+    if _fits_tma(t, 0, 1):
+        return t, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8, False
+    if _fits_tma(t, 1, 0):
+        return t, t.stride(1) if t.shape[1] > 1 else -(-t.shape[0] // 8) * 8, True
+    if t.stride(0) == 1 and t.shape[0] > 1:  # transposed with an odd pitch: keep its layout
+        copy = _pitched(t.shape[1], t.shape[0], t)
+        copy.copy_(t.t())
+        return copy, copy.stride(0), True
+    copy = _pitched(t.shape[0], t.shape[1], t)
+    copy.copy_(t)
+    return copy, copy.stride(0), False
+
+
+def _rows(t: Tensor) -> Tensor:
+    """t with unit column stride (a copy when it has none)."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = native.ACT_NONE,
+            residual: Tensor | None = None, keep_z: bool = False):
+    """(y, z) with z = a @ b.T + bias and y = f(z) + residual; z is None unless
+    ``keep_z``. a (M, K), b (N, K), either of them possibly a transposed view."""
+    m, k = a.shape
+    n = b.shape[0]
+    y = torch.empty(m, n, dtype=a.dtype, device=a.device)
+    z = torch.empty_like(y) if keep_z else None
+    if m == 0 or n == 0:
+        return y, z
+    if k == 0:  # an empty sum: one zero column gives it
+        a, b = a.new_zeros(m, 8), b.new_zeros(n, 8)
+        k = 8
+    args = native.LinearArgs()
+    args.m, args.n, args.k = m, n, k
+    a, args.lda, args.a_mn_major = _operand(a)
+    b, args.ldb, args.b_mn_major = _operand(b)
+    args.a, args.b = a.data_ptr(), b.data_ptr()
+    if bias is not None:
+        bias = bias.contiguous()
+        args.bias = bias.data_ptr()
+    if residual is not None:
+        residual = _rows(residual)
+        args.residual, args.ld_residual = residual.data_ptr(), max(residual.stride(0), n)
+    if z is not None:
+        args.z, args.ld_z = z.data_ptr(), n
+    args.y, args.ld_y = y.data_ptr(), n
+    args.act, args.dtype = activation, native.HALF_DTYPES[a.dtype]
+    nbytes = native.lib().cg_linear_half_workspace_bytes(ctypes.byref(args))
+    workspace = None
+    if nbytes > 0:
+        workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=a.device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
+    native.invoke("cg_linear_half", ctypes.byref(args), native.stream_ptr(a.device), info=(m, n, k))
+    return y, z
+
+
+def _act_grad(gy: Tensor, z: Tensor | None, activation: int, want_db: bool):
+    """(gz, db): gz = gy f'(z) (gy itself without an activation), db its column
+    sums or None."""
+    gy = _rows(gy)
+    rows, cols = gy.shape
+    args = native.ActGradArgs()
+    args.rows, args.cols, args.act, args.dtype = rows, cols, activation, native.HALF_DTYPES[gy.dtype]
+    args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), cols)
+    gz, db, scratch = gy, None, None
+    if activation != native.ACT_NONE:
+        gz = _pitched(rows, cols, gy)
+        args.z, args.ld_z = z.data_ptr(), max(z.stride(0), cols)
+        args.gz, args.ld_gz = gz.data_ptr(), max(gz.stride(0), cols)
+    if want_db:
+        db = torch.empty(cols, dtype=gy.dtype, device=gy.device)
+        nbytes = native.lib().cg_act_grad_half_scratch_bytes(rows, cols)
+        scratch = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=gy.device)
+        args.db, args.scratch, args.scratch_bytes = db.data_ptr(), scratch.data_ptr(), nbytes
+    if args.gz or args.db:
+        native.invoke("cg_act_grad_half", ctypes.byref(args), native.stream_ptr(gy.device))
+    return gz, db
+
+
+class _Product(_Fused):
+    """C = a @ b.T; backward: g @ b and g.T @ a."""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        ctx.save_for_backward(a, b)
+        ctx.edges = _edges(a, b)
+        return product(a, b)[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        a, b = ctx.saved_tensors
+        ga = _Product.apply(g, b.t()) if ctx.needs_input_grad[0] and engine_will_execute(ctx.edges[0]) else None
+        gb = _Product.apply(g.t(), a.t()) if ctx.needs_input_grad[1] and engine_will_execute(ctx.edges[1]) else None
+        return ga, gb
+
+
+class _ActGrad(_Fused):
+    """(gz, db) of _act_grad; backward: the second-order kernel."""
+
+    @staticmethod
+    def forward(ctx, gy, z, activation, want_db):
+        ctx.save_for_backward(gy, z)
+        ctx.activation = activation
+        ctx.set_materialize_grads(False)
+        gz, db = _act_grad(gy, z, activation, want_db)
+        return (gz.view_as(gz) if gz is gy else gz), db
+
+    @staticmethod
+    def backward(ctx, h, hb):
+        gy, z = ctx.saved_tensors
+        if h is None and hb is None:
+            return None, None, None, None
+        if z is None:  # no activation: gz is gy
+            t = hb.expand(gy.shape) if h is None else h if hb is None else h + hb
+            return t, None, None, None
+        return *_ActGrad2.apply(h, hb, gy, z, ctx.activation), None, None
+
+
+class _ActGrad2(_Fused):
+    """(dgy, dz) = ((h + hb) f'(z), (h + hb) gy f''(z)): the last derivative the
+    force training needs."""
+
+    @staticmethod
+    def forward(ctx, h, hb, gy, z, activation):
+        h = None if h is None else h.contiguous()
+        hb = None if hb is None else hb.contiguous()
+        gy, z = gy.contiguous(), z.contiguous()
+        dgy, dz = torch.empty_like(gy), torch.empty_like(z)
+        native.invoke("cg_act_grad2_half", native.ptr(h), native.ptr(hb), gy.data_ptr(), z.data_ptr(),
+                      dgy.data_ptr(), dz.data_ptr(), gy.shape[0], gy.shape[1], activation,
+                      native.HALF_DTYPES[gy.dtype], native.stream_ptr(gy.device))
+        return dgy, dz
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NativeError("dense.linear: third derivatives are not supported")
+
+
+class _Linear(_Fused):
+    """(y, z) from one product; z is None without an activation."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, activation):
+        y, z = product(x, w, b, activation, r, keep_z=activation != native.ACT_NONE)
+        ctx.save_for_backward(x, w, z)
+        ctx.edges = _edges(x, w, b)
+        ctx.activation = activation
+        # z is seldom used: its gradient arrives as None, not as zeros
+        ctx.set_materialize_grads(False)
+        return y, z
+
+    @staticmethod
+    def backward(ctx, gy, gz_direct):
+        x, w, z = ctx.saved_tensors
+        want = [ctx.needs_input_grad[i] and engine_will_execute(ctx.edges[i]) for i in range(3)]
+        gz, db = gz_direct, None
+        if gy is not None and any(want):
+            alone = gz_direct is None
+            gz, db = _ActGrad.apply(gy, z, ctx.activation, want[2] and alone)
+            if not alone:
+                gz = gz + gz_direct
+        if gz is None:
+            return None, None, None, gy, None
+        if want[2] and db is None:
+            db = _ActGrad.apply(gz, None, native.ACT_NONE, True)[1]
+        dx = _Product.apply(gz, w.t()) if want[0] else None
+        dw = _Product.apply(gz.t(), x.t()) if want[1] else None
+        return dx, dw, db, (gy if ctx.needs_input_grad[3] else None), None
+
+
+def _checked(x, weight, bias, residual, activation) -> int:
+    native.require_cuda(x, weight, bias, residual)
+    if activation not in ACTIVATIONS:
+        raise NativeError(f"dense.linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if x.dtype not in native.HALF_DTYPES:
+        raise NativeError(f"dense.linear: float16 or bfloat16 expected, got {x.dtype} (the fp32 layers are in "
+                          "create_graph_b200.nn)")
+    named = {"weight": weight, "bias": bias, "residual": residual}
+    for name, t in named.items():
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise NativeError(f"dense.linear: {name} is {t.dtype} on {t.device}, x {x.dtype} on {x.device}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise NativeError(f"dense.linear: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
+    n = weight.shape[0]
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise NativeError(f"dense.linear: bias must be ({n},), got {tuple(bias.shape)}")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
+        raise NativeError(f"dense.linear: residual must be {(*x.shape[:-1], n)}, got {tuple(residual.shape)}")
+    return ACTIVATIONS[activation]
+
+
+def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation: str = "none",
+           residual: Tensor | None = None) -> Tensor:
+    """f(x @ weight.T + bias) + residual (see the module's description)."""
+    act = _checked(x, weight, bias, residual, activation)
+    n, shape = weight.shape[0], x.shape
+    if x.dim() != 2:
+        x = x.reshape(math.prod(shape[:-1]), shape[-1])
+    if residual is not None and residual.dim() != 2:
+        residual = residual.reshape(x.shape[0], n)
+    with torch.cuda.device(x.device):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+            y = _Linear.apply(x, weight, bias, residual, act)[0]
+        else:
+            y = product(x, weight, bias, act, residual)[0]
+    return y if len(shape) == 2 else y.view(*shape[:-1], n)
+
+
+class Linear(nn.Module):
+    """A half-precision layer y = f(x W^T + b) + r, initialised as torch.nn.Linear."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "none",
+                 dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        if dtype not in native.HALF_DTYPES:
+            raise NativeError(f"dense.Linear: float16 or bfloat16 expected, got {dtype}")
+        if activation not in ACTIVATIONS:
+            raise NativeError(f"dense.Linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+        self.activation = activation
+        like = nn.Linear(in_features, out_features, bias=bias, device=device)
+        self.weight = nn.Parameter(like.weight.detach().to(dtype))
+        self.bias = nn.Parameter(like.bias.detach().to(dtype)) if bias else None
+
+    def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
+        return linear(x, self.weight, self.bias, activation=self.activation, residual=residual)

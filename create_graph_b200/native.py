@@ -20,7 +20,7 @@ from create_graph_b200.errors import NativeError
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "libcg_b200.so"
 ABI_VERSION = 1
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
 ATTN_PRECISIONS = {"fp32": 0, "tf32": 1}  # CG_ATTN_FP32, CG_ATTN_TF32
 
 
@@ -31,6 +31,7 @@ def attn_precision(name: str) -> int:
         raise ValueError(f"attention precision must be one of {sorted(ATTN_PRECISIONS)}, got {name!r}") from None
 
 _DTYPES = {torch.float32: F32, torch.float64: F64}
+HALF_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 
 i64 = ctypes.c_int64
 i32 = ctypes.c_int32
@@ -102,6 +103,49 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", i64),
+        ("n", i64),
+        ("k", i64),
+        ("a", vp),
+        ("lda", i64),
+        ("b", vp),
+        ("ldb", i64),
+        ("bias", vp),
+        ("residual", vp),
+        ("ld_residual", i64),
+        ("z", vp),
+        ("ld_z", i64),
+        ("y", vp),
+        ("ld_y", i64),
+        ("a_mn_major", i32),
+        ("b_mn_major", i32),
+        ("act", i32),
+        ("dtype", i32),
+        ("workspace", vp),
+        ("workspace_bytes", i64),
+    ]
+
+
+class ActGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", i64),
+        ("cols", i64),
+        ("gy", vp),
+        ("ld_gy", i64),
+        ("z", vp),
+        ("ld_z", i64),
+        ("gz", vp),
+        ("ld_gz", i64),
+        ("db", vp),
+        ("scratch", vp),
+        ("scratch_bytes", i64),
+        ("act", i32),
+        ("dtype", i32),
+    ]
+
+
 class PooledAttnArgs(ctypes.Structure):
     _fields_ = [
         ("n", i64),
@@ -148,7 +192,7 @@ class GeomArgs(ctypes.Structure):
     ]
 
 
-ACT_NONE, ACT_SILU, ACT_SILU_GRAD, ACT_ADD = 0, 1, 2, 3
+ACT_NONE, ACT_SILU, ACT_SILU_GRAD, ACT_ADD, ACT_RELU, ACT_GELU = 0, 1, 2, 3, 4, 5
 GEMM_TF32, GEMM_FP32 = 0, 1
 f32 = ctypes.c_float
 _I = ctypes.c_int
@@ -165,6 +209,11 @@ _SIGNATURES = {
     "cg_gemm_tf32": (ctypes.c_int, [ctypes.POINTER(GemmArgs), vp]),
     "cg_gemm_workspace_bytes": (i64, [ctypes.POINTER(GemmArgs)]),
     "cg_gemm_tf32_noalloc": (ctypes.c_int, [ctypes.POINTER(GemmArgs), vp]),
+    "cg_linear_half": (_I, [ctypes.POINTER(LinearArgs), vp]),
+    "cg_linear_half_workspace_bytes": (i64, [ctypes.POINTER(LinearArgs)]),
+    "cg_act_grad_half": (_I, [ctypes.POINTER(ActGradArgs), vp]),
+    "cg_act_grad_half_scratch_bytes": (i64, [i64, i64]),
+    "cg_act_grad2_half": (_I, [vp, vp, vp, vp, vp, vp, i64, i64, _I, _I, vp]),
     "cg_device_error": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
     "cg_gather_rows": (_I, [vp, i64, vp, i64, i64, vp, i64, vp]),
     "cg_segment_sum": (_I, [vp, i64, vp, vp, i64, i64, vp, i64, _I, vp]),

@@ -28,6 +28,8 @@ extern "C" {
 /* dtype codes */
 #define CG_F32 0
 #define CG_F64 1
+#define CG_F16 2
+#define CG_BF16 3
 
 /* Text of the last error raised on the calling thread ("" if none). */
 const char* cg_last_error(void);
@@ -193,6 +195,8 @@ int cg_pooled_attn_out(const cg_pooled_attn_args* a, void* stream);
 #define CG_ACT_SILU 1
 #define CG_ACT_SILU_GRAD 2
 #define CG_ACT_ADD 3
+#define CG_ACT_RELU 4 /* cg_linear_half only */
+#define CG_ACT_GELU 5 /* cg_linear_half only: z Phi(z), the erf form */
 /* product precision (cg_gemm_args.precision) */
 #define CG_GEMM_TF32 0 /* one product of tf32-rounded operands, fp32 accumulation */
 #define CG_GEMM_FP32 1 /* three-term tf32 split x = hi + lo: A_lo B_hi + A_hi B_lo + A_hi B_hi,
@@ -240,6 +244,66 @@ int64_t cg_gemm_workspace_bytes(const cg_gemm_args* args);
  * threads) race; each call writes every scratch element it later reads, so
  * nothing needs clearing between calls. No counterpart in the reference. */
 int cg_gemm_tf32_noalloc(const cg_gemm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Half-precision dense layer (bf16 or fp16 values, fp32 accumulation on the
+ * tcgen05 tensor cores, one rounding at the end):
+ *   z = A B^T + bias,  y = f(z) + residual
+ * A(m, k), B(n, k) are K-major or MN-major as in cg_gemm_args; bias (n,) and
+ * residual (m, n) may be NULL; act is CG_ACT_NONE, CG_ACT_SILU, CG_ACT_RELU or
+ * CG_ACT_GELU; z, when set, receives the pre-activation (what the backward
+ * needs). Every tensor has the type `dtype` (CG_F16 or CG_BF16). a and b are
+ * 16-byte aligned with pitches that are multiples of 8 values; the others may
+ * have any alignment and pitch. No counterpart in the reference (its layers
+ * are torch's, compiled by Inductor: src/create_graph/region.py:191-198).
+ * ---------------------------------------------------------------------- */
+typedef struct cg_linear_args {
+  int64_t m, n, k;
+  const void* a;
+  int64_t lda;
+  const void* b;
+  int64_t ldb;
+  const void* bias;
+  const void* residual;
+  int64_t ld_residual;
+  void* z;
+  int64_t ld_z;
+  void* y;
+  int64_t ld_y;
+  int32_t a_mn_major, b_mn_major;
+  int32_t act;
+  int32_t dtype;
+  float* workspace; /* split-K partial tiles; cg_linear_half_workspace_bytes() bytes */
+  int64_t workspace_bytes;
+} cg_linear_args;
+
+int cg_linear_half(const cg_linear_args* args, void* stream);
+/* Workspace bytes cg_linear_half needs for these args (0: no split). */
+int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args);
+
+/* gz = gy f'(z) and db[c] = sum over rows of gz, in one pass. gz NULL: gz is
+ * gy itself (no activation) and only db is formed; db NULL: only gz. */
+typedef struct cg_act_grad_args {
+  int64_t rows, cols;
+  const void* gy;
+  int64_t ld_gy;
+  const void* z;
+  int64_t ld_z;
+  void* gz;
+  int64_t ld_gz;
+  void* db;       /* (cols,) */
+  float* scratch; /* with db: cg_act_grad_half_scratch_bytes() bytes */
+  int64_t scratch_bytes;
+  int32_t act;
+  int32_t dtype;
+} cg_act_grad_args;
+
+int cg_act_grad_half(const cg_act_grad_args* args, void* stream);
+int64_t cg_act_grad_half_scratch_bytes(int64_t rows, int64_t cols);
+/* Second order: for cotangents h of gz and hb of db (either may be NULL),
+ * dgy = (h + hb) f'(z) and dz = (h + hb) gy f''(z); contiguous (rows, cols). */
+int cg_act_grad2_half(const void* h, const void* hb, const void* gy, const void* z, void* dgy, void* dz, int64_t rows,
+                      int64_t cols, int act, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Segment sums over a sorted CSR, their transpose, column reductions.
