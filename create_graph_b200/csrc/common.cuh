@@ -79,4 +79,9 @@ namespace dense {
 int device_error(int* out, bool reset);
 }  // namespace dense
 
+namespace muon {
+// the same of the Newton-Schulz products (muon.cu)
+int device_error(int* out, bool reset);
+}  // namespace muon
+
 }  // namespace cg

@@ -109,6 +109,7 @@ struct EpiArgs {
 template <class T>
 struct Epi {
   using Args = EpiArgs;
+  static constexpr int kGroups = 1;
   struct Aux {
     uint4 r[4];
   };
@@ -169,7 +170,7 @@ struct Epi {
     if (a.residual) v += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]);
     static_cast<T*>(a.y)[row * a.ld_y + col] = from_float<T>(v);
   }
-  __device__ void store(const Aux& aux, const float* stage, int row0, int col0, int lane) const {
+  __device__ void store(const Aux& aux, float* stage, int row0, int col0, int lane) const {
     if (a.vec) {
       const int c = (lane & 3) * 8, col = col0 + c;
       if (col >= n) return;
@@ -365,7 +366,7 @@ static int64_t workspace_bytes(const cg_linear_args& g) {
 
 template <int CG, int BN, class T>
 static int launch(const cg_linear_args& g, const Plan& p, const EpiArgs& ea, bool bf16, cudaStream_t s) {
-  half::Launch<EpiArgs> L;
+  half::LaunchOf<Epi<T>> L;
   memset(&L, 0, sizeof(L));
   L.groups = 1;
   L.bf16 = bf16;

@@ -783,10 +783,11 @@ int64_t cg_gemm_workspace_bytes(const cg_gemm_args* args) {
 }
 
 int cg_device_error(int* out, int reset) {
-  int v = 0, dense = 0;
+  int v = 0, dense = 0, muon = 0;
   CG_CUDA(cudaMemcpyFromSymbol(&v, cg::gemm::g_gemm_error, sizeof(int)));
   if (int rc = cg::dense::device_error(&dense, reset != 0)) return rc;
-  if (v == 0) v = dense;
+  if (int rc = cg::muon::device_error(&muon, reset != 0)) return rc;
+  if (v == 0) v = dense != 0 ? dense : muon;
   if (reset) {
     const int zero = 0;
     CG_CUDA(cudaMemcpyToSymbol(cg::gemm::g_gemm_error, &zero, sizeof(int)));

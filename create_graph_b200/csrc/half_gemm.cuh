@@ -18,7 +18,10 @@
 // n), so x W^T, g W and g^T x read their operands as they are stored.
 // PLANES = 2: every operand is a pair of fp16 planes hi + lo (22 significant
 // bits) and a k-slice makes the products lo hi + hi lo + hi hi; the dropped
-// lo lo term is 2^-22 relative.
+// lo lo term is 2^-22 relative. The tensor core truncates as it adds to an
+// accumulator (a sum of positive terms over k = 3072, 576 additions, came out
+// 2e-5 low), so accumulators then hold kSumSlices k-slices at a time and the
+// epilogue warps add them up in registers, rounded to nearest.
 // A pair of SMs halves the B bytes each SM stages per flop: a 256 x 256 tile
 // takes 32 KB of shared memory per 64-wide slice and SM against 48 KB for the
 // 128 x 256 tile of one SM, which is what lets six stages fit.
@@ -42,7 +45,8 @@ constexpr int kBK = 64;        // half-precision values per k-slice: 128 bytes
 constexpr int kRows = 128;     // accumulator rows per CTA
 constexpr int kEpiWarps = 8;   // two per TMEM lane quarter
 constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr int kMaxGroups = 8;  // problems of different shapes in one launch
+constexpr int kSumSlices = 2;  // k-slices summed in one accumulator when PLANES = 2
+constexpr int kBand = 8;       // m-tiles of one band of the tile walk
 
 // Bounded wait: 2^24 polls are about half a second at the least, hundreds of
 // times the longest tile.
@@ -170,19 +174,21 @@ struct Group {
   int batch;
   int a_mn, b_mn;            // MN-major operands
   int splits, kt_per;        // k-slices per split
-  int n_fast;                // consecutive items walk n first
   int lower;                 // symmetric result: only tiles that reach the lower triangle
   int tiles;                 // items per batch entry and split
   int first_item;
   EpiArgs epi;
 };
 
-template <class EpiArgs>
+// A launch: up to GROUPS problems of different shapes, walked in order.
+template <class EpiArgs, int GROUPS>
 struct Launch {
-  Group<EpiArgs> g[kMaxGroups];
+  Group<EpiArgs> g[GROUPS];
   int groups, items;
   int bf16;
 };
+template <class Epi>
+using LaunchOf = Launch<typename Epi::Args, Epi::kGroups>;
 
 struct Item {
   int g, batch, split, m0, n0, kt0, kt1;
@@ -195,11 +201,12 @@ __host__ __device__ inline int lower_tiles_of_row(int i, int bm, int bn, int n_t
   return c < n_tiles ? c : n_tiles;
 }
 
-template <int BM, int BN, class EpiArgs>
-__device__ inline Item item_of(const Launch<EpiArgs>& L, int w) {
+template <int BM, int BN, class EpiArgs, int GROUPS>
+__device__ inline Item item_of(const Launch<EpiArgs, GROUPS>& L, int w) {
   Item it;
   it.g = 0;
-  while (it.g + 1 < L.groups && w >= L.g[it.g + 1].first_item) ++it.g;
+  if (GROUPS > 1)
+    while (it.g + 1 < L.groups && w >= L.g[it.g + 1].first_item) ++it.g;
   const Group<EpiArgs>& g = L.g[it.g];
   w -= g.first_item;
   int t = w % g.tiles;
@@ -215,12 +222,14 @@ __device__ inline Item item_of(const Launch<EpiArgs>& L, int w) {
       ++mt;
     }
     nt = t;
-  } else if (g.n_fast) {
-    nt = t % g.n_tiles;
-    mt = t / g.n_tiles;
   } else {
-    mt = t % g.m_tiles;
-    nt = t / g.m_tiles;
+    // bands of kBand m-tiles, each walked m first: a wave of tiles then covers
+    // a near-square block and reads few rows of either operand
+    const int band = t / (kBand * g.n_tiles);
+    t -= band * kBand * g.n_tiles;
+    const int high = g.m_tiles - band * kBand < kBand ? g.m_tiles - band * kBand : kBand;
+    mt = band * kBand + t % high;
+    nt = t / high;
   }
   it.m0 = mt * BM;
   it.n0 = nt * BN;
@@ -242,12 +251,12 @@ __device__ __forceinline__ void stage_read8(const float* stage, int r, int c, fl
   v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
 
-// Epi: Epi::Args (kernel parameter), Epi::Aux (values prefetched for one 32 x 32
+// Epi: Epi::Args (kernel parameter), Epi::kGroups (problems per launch), Epi::Aux (values prefetched for one 32 x 32
 // block), Epi(args, m, n, batch entry, split), fetch(aux, row0, col0, lane),
 // store(aux, stage, row0, col0, lane) and error_word() (the translation unit's).
 template <int CG, int BN, int PLANES, class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
-    half_gemm_kernel(const __grid_constant__ Launch<typename Epi::Args> L) {
+    half_gemm_kernel(const __grid_constant__ LaunchOf<Epi> L) {
   using T = Tile<CG, BN, PLANES>;
   constexpr int BM = CG * kRows;
   constexpr int STAGES = T::kStages;
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- UMMA issuer (the pair's leader) ----------------
     uint32_t it = 0;
     int j = 0;
-    for (int w = first; w < L.items && ok; w += step, ++j) {
+    for (int w = first; w < L.items && ok; w += step) {
       const Item item = item_of<BM, BN>(L, w);
       const auto& g = L.g[item.g];
       const uint32_t idesc = idesc_f16(BM, BN, L.bf16 != 0, g.a_mn != 0, g.b_mn != 0);
@@ -334,74 +343,116 @@ __global__ void __launch_bounds__(kThreads, 1)
       // 16 along k = two groups.
       const uint32_t a_lbo = g.a_mn ? kBK * 128 : 16, a_step = g.a_mn ? 2048 : 32;
       const uint32_t b_lbo = g.b_mn ? kBK * 128 : 16, b_step = g.b_mn ? 2048 : 32;
-      const int b = j & 1, use = j >> 1;
-      if (use > 0 && !(ok = wait(&acc_empty[b], (use - 1) & 1, error_word))) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + b * BN;
-      for (int kt = item.kt0; kt < item.kt1; ++kt, ++it) {
-        const int s = it % STAGES;
-        if (!(ok = wait(&full[s], (it / STAGES) & 1, error_word))) break;
+      // one accumulator per item, or per kSumSlices of it
+      const int per = PLANES == 2 ? kSumSlices : item.kt1 - item.kt0;
+      for (int kt0 = item.kt0; kt0 < item.kt1 && ok; kt0 += per, ++j) {
+        const int b = j & 1, use = j >> 1;
+        const int kt1 = kt0 + per < item.kt1 ? kt0 + per : item.kt1;
+        if (use > 0 && !(ok = wait(&acc_empty[b], (use - 1) & 1, error_word))) break;
         tc_fence_after();
-        const uint32_t sa = smem_u32(tiles + s * T::kStage), sb = sa + T::kA;
-        auto da = [&](int p, int kk) {
-          return smem_desc(sa + p * (T::kA + T::kB) + kk * a_step, a_lbo, 1024, kSwizzle128B);
-        };
-        auto db = [&](int p, int kk) {
-          return smem_desc(sb + p * (T::kA + T::kB) + kk * b_step, b_lbo, 1024, kSwizzle128B);
-        };
+        const uint32_t acc = tmem + b * BN;
+        for (int kt = kt0; kt < kt1; ++kt, ++it) {
+          const int s = it % STAGES;
+          if (!(ok = wait(&full[s], (it / STAGES) & 1, error_word))) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(tiles + s * T::kStage), sb = sa + T::kA;
+          auto da = [&](int p, int kk) {
+            return smem_desc(sa + p * (T::kA + T::kB) + kk * a_step, a_lbo, 1024, kSwizzle128B);
+          };
+          auto db = [&](int p, int kk) {
+            return smem_desc(sb + p * (T::kA + T::kB) + kk * b_step, b_lbo, 1024, kSwizzle128B);
+          };
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk) {
-          const bool on = kt > item.kt0 || kk > 0;
-          if (PLANES == 2) {  // the small cross terms first, then the hi product
-            umma_f16<CG>(acc, da(1, kk), db(0, kk), idesc, on);
-            umma_f16<CG>(acc, da(0, kk), db(1, kk), idesc, true);
-            umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, true);
-          } else {
-            umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, on);
+          for (int kk = 0; kk < kBK / 16; ++kk) {
+            const bool on = kt > kt0 || kk > 0;
+            if (PLANES == 2) {  // the small cross terms first, then the hi product
+              umma_f16<CG>(acc, da(1, kk), db(0, kk), idesc, on);
+              umma_f16<CG>(acc, da(0, kk), db(1, kk), idesc, true);
+              umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, true);
+            } else {
+              umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, on);
+            }
           }
+          umma_commit_cg<CG>(&empty[s]);
         }
-        umma_commit_cg<CG>(&empty[s]);
+        umma_commit_cg<CG>(&acc_full[b]);
       }
-      umma_commit_cg<CG>(&acc_full[b]);
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
     // Warp e of a TMEM lane quarter (32 rows) takes alternate 32-column blocks.
     const int quarter = warp & 3, e = warp - 2;
     float* stage = staging + e * (32 * 32);
-    int j = 0;
-    for (int w = first; w < L.items; w += step, ++j) {
-      const Item item = item_of<BM, BN>(L, w);
-      const auto& g = L.g[item.g];
-      const Epi epi(g.epi, g.m, g.n, item.batch, item.split);
-      const int row0 = item.m0 + (int)rank * kRows + quarter * 32;
-      const int b = j & 1, use = j >> 1;
-      typename Epi::Aux aux;
-      const int c_first = 32 * (e >> 2);
-      epi.fetch(aux, row0, item.n0 + c_first, lane);  // beside the wait for the accumulator
-      if (!(ok = wait(&acc_full[b], use & 1, error_word))) break;
-      tc_fence_after();
-#pragma unroll 1
-      for (int c0 = c_first; c0 < BN; c0 += 64) {
-        float v[32];
-        tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c0, v);
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<float4*>(stage + stage_idx(lane, 4 * q)) =
-              make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        __syncwarp();
-        typename Epi::Aux next;
-        if (c0 + 64 < BN) epi.fetch(next, row0, item.n0 + c0 + 64, lane);
-        epi.store(aux, stage, row0, item.n0 + c0, lane);
-        __syncwarp();
-        aux = next;
-      }
-      // the accumulator may be overwritten once every epilogue warp has read it
+    const int c_first = 32 * (e >> 2);
+    // the accumulator may be overwritten once every epilogue warp has read it
+    auto release = [&](int b) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if (CG == 2) mbar_arrive_remote(&acc_empty[b], 0);
         else mbar_arrive(&acc_empty[b]);
+      }
+    };
+    auto put = [&](const float (&v)[32]) {  // row `lane` of the warp's block
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<float4*>(stage + stage_idx(lane, 4 * q)) =
+            make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      __syncwarp();
+    };
+    int j = 0;
+    for (int w = first; w < L.items && ok; w += step) {
+      const Item item = item_of<BM, BN>(L, w);
+      const auto& g = L.g[item.g];
+      const Epi epi(g.epi, g.m, g.n, item.batch, item.split);
+      const int row0 = item.m0 + (int)rank * kRows + quarter * 32;
+      typename Epi::Aux aux;
+      epi.fetch(aux, row0, item.n0 + c_first, lane);  // beside the wait for the accumulator
+      if constexpr (PLANES == 2) {
+        constexpr int NB = BN / 64;
+        float sum[NB][32];
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) sum[q][x] = 0.0f;
+        for (int kt = item.kt0; kt < item.kt1; kt += kSumSlices, ++j) {
+          const int b = j & 1;
+          if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int q = 0; q < NB; ++q) {
+            float v[32];
+            tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + 64 * q, v);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum[q][x] += v[x];
+          }
+          release(b);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+          put(sum[q]);
+          epi.store(aux, stage, row0, item.n0 + c_first + 64 * q, lane);
+          __syncwarp();
+          if (q + 1 < NB) epi.fetch(aux, row0, item.n0 + c_first + 64 * (q + 1), lane);
+        }
+      } else {
+        const int b = j & 1;
+        if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = c_first; c0 < BN; c0 += 64) {
+          float v[32];
+          tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c0, v);
+          put(v);
+          typename Epi::Aux next;
+          if (c0 + 64 < BN) epi.fetch(next, row0, item.n0 + c0 + 64, lane);
+          epi.store(aux, stage, row0, item.n0 + c0, lane);
+          __syncwarp();
+          aux = next;
+        }
+        release(b);
+        ++j;
       }
     }
   }
@@ -466,9 +517,6 @@ int64_t plan_group(Group<EpiArgs>& g) {
   constexpr int BM = CG * kRows;
   g.m_tiles = (g.m + BM - 1) / BM;
   g.n_tiles = (g.n + BN - 1) / BN;
-  // walk the shorter side first: a wave of tiles then shares whole rows of
-  // tiles of the longer operand, each read once, and the other operand in L2
-  g.n_fast = g.n_tiles <= g.m_tiles;
   int64_t tiles = (int64_t)g.m_tiles * g.n_tiles;
   if (g.lower) {
     tiles = 0;
@@ -479,7 +527,7 @@ int64_t plan_group(Group<EpiArgs>& g) {
 }
 
 template <int CG, int BN, int PLANES, class Epi>
-int launch_half_gemm(const Launch<typename Epi::Args>& L, cudaStream_t stream) {
+int launch_half_gemm(const LaunchOf<Epi>& L, cudaStream_t stream) {
   using T = Tile<CG, BN, PLANES>;
   auto kernel = half_gemm_kernel<CG, BN, PLANES, Epi>;
   CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));

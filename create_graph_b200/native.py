@@ -146,6 +146,41 @@ class ActGradArgs(ctypes.Structure):
     ]
 
 
+class NsEntry(ctypes.Structure):
+    _fields_ = [
+        ("x", vp),
+        ("ld_x", i64),
+        ("stride_x", i64),
+        ("out", vp),
+        ("ld_out", i64),
+        ("stride_out", i64),
+        ("momentum", vp),
+        ("ld_momentum", i64),
+        ("rows", i64),
+        ("cols", i64),
+        ("count", i64),
+    ]
+
+
+class NsArgs(ctypes.Structure):
+    _fields_ = [
+        ("entries", ctypes.POINTER(NsEntry)),
+        ("n", i32),
+        ("dtype", i32),
+        ("steps", i32),
+        ("nesterov", i32),
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("momentum", ctypes.c_float),
+        ("lr", ctypes.c_float),
+        ("weight_decay", ctypes.c_float),
+        ("workspace", vp),
+        ("workspace_bytes", i64),
+    ]
+
+
 class PooledAttnArgs(ctypes.Structure):
     _fields_ = [
         ("n", i64),
@@ -214,6 +249,9 @@ _SIGNATURES = {
     "cg_act_grad_half": (_I, [ctypes.POINTER(ActGradArgs), vp]),
     "cg_act_grad_half_scratch_bytes": (i64, [i64, i64]),
     "cg_act_grad2_half": (_I, [vp, vp, vp, vp, vp, vp, i64, i64, _I, _I, vp]),
+    "cg_newton_schulz": (_I, [ctypes.POINTER(NsArgs), vp]),
+    "cg_muon_step": (_I, [ctypes.POINTER(NsArgs), vp]),
+    "cg_newton_schulz_workspace_bytes": (i64, [ctypes.POINTER(NsArgs)]),
     "cg_device_error": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
     "cg_gather_rows": (_I, [vp, i64, vp, i64, i64, vp, i64, vp]),
     "cg_segment_sum": (_I, [vp, i64, vp, vp, i64, i64, vp, i64, _I, vp]),

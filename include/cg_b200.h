@@ -454,6 +454,46 @@ int cg_neighbor_list(const float* pos, const int32_t* sys_ptr, int64_t n_systems
                      int64_t max_atoms_per_system, float cutoff, int32_t k, int32_t* nbr, int32_t* counts,
                      int32_t* rev_ptr, int32_t* rev_idx, int32_t* workspace, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Newton-Schulz orthogonalisation of matrices, and the optimizer step on it:
+ *   X = G / max(|G|_F, eps); `steps` times
+ *   A = X X^T, B = b A + c A A, X = a X + B X   (X^T X and X B when rows > cols)
+ * at fp32-level accuracy (pairs of fp16 planes, three products each).
+ * cg_newton_schulz: out = X for every matrix; x and out have the type `dtype`
+ * (CG_F32, CG_F16 or CG_BF16) and may be the same memory.
+ * cg_muon_step (fp32): with g = x and m = momentum,
+ *   m = m + (1 - mu) (g - m);  u = nesterov ? g + mu (m - g) : m;
+ *   out = (1 - lr weight_decay) out - lr sqrt(max(1, rows / cols)) X(u).
+ * Matrices are given as runs of `count` of one shape at regular strides (in
+ * elements; cg_muon_step takes runs of one). No counterpart in the reference,
+ * which ships no optimizer.
+ * ---------------------------------------------------------------------- */
+typedef struct cg_ns_entry {
+  const void* x;
+  int64_t ld_x, stride_x;
+  void* out;
+  int64_t ld_out, stride_out;
+  float* momentum;
+  int64_t ld_momentum;
+  int64_t rows, cols, count;
+} cg_ns_entry;
+
+typedef struct cg_ns_args {
+  const cg_ns_entry* entries; /* host memory, read during the call only */
+  int32_t n;
+  int32_t dtype;
+  int32_t steps;
+  int32_t nesterov;
+  float a, b, c, eps;
+  float momentum, lr, weight_decay; /* cg_muon_step: mu, lr, wd */
+  void* workspace;                  /* 256-byte aligned; cg_newton_schulz_workspace_bytes() bytes */
+  int64_t workspace_bytes;
+} cg_ns_args;
+
+int cg_newton_schulz(const cg_ns_args* args, void* stream);
+int cg_muon_step(const cg_ns_args* args, void* stream);
+int64_t cg_newton_schulz_workspace_bytes(const cg_ns_args* args);
+
 /* The device error word kernels set when a bounded wait gave up (0: none);
  * reset != 0 clears it. Synchronises with the device. No reference
  * counterpart: the reference's kernels are generated by Inductor and have no
