@@ -12,8 +12,8 @@
 //               stage back to the producers and each finished accumulator to
 //               the epilogue (two accumulators: an item's epilogue runs beside
 //               the next item's products);
-//   warps 2..9  epilogue: tcgen05.ld (thread = row), a transpose through
-//               shared memory, then 16-byte row segments in and out.
+//   warps 2..9  epilogue: tcgen05.ld (thread = row), the layer's own arithmetic,
+//               and the result through shared memory to global memory.
 // Operands are K-major (contiguous along k) or MN-major (contiguous along m or
 // n), so x W^T, g W and g^T x read their operands as they are stored.
 // PLANES = 2: every operand is a pair of fp16 planes hi + lo (22 significant
@@ -90,6 +90,19 @@ __device__ inline void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* 
         : "memory");
   }
 }
+// A block between this CTA's shared memory and global memory; out-of-range
+// parts are read as zero and not written. Stores are one bulk group each.
+__device__ inline void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until all this thread's stores have read their shared memory / are complete.
+__device__ inline void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ inline void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 template <int CG>
 __device__ inline void tmem_alloc_cg(uint32_t* slot, uint32_t cols) {
   if (CG == 1) {
@@ -150,13 +163,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a
 }
 
 // ---- tiles ------------------------------------------------------------------
-template <int CG, int BN, int PLANES>
+template <int CG, int BN, int PLANES, int STAGING>
 struct Tile {
   static constexpr int kBRows = BN / CG;                       // B rows this CTA stages
   static constexpr int kA = kRows * kBK * 2;
   static constexpr int kB = kBRows * kBK * 2;
   static constexpr int kStage = PLANES * (kA + kB);
-  static constexpr int kStaging = kEpiWarps * 32 * 32 * 4;     // one 32 x 32 fp32 block per epilogue warp
+  static constexpr int kStaging = kEpiWarps * STAGING;         // the epilogue warps' own blocks
   static constexpr int kStagesFit = (227 * 1024 - kStaging - 1024 - 512) / kStage;
   static constexpr int kStages = kStagesFit < 8 ? kStagesFit : 8;
   static constexpr int kBytes = kStages * kStage + kStaging + 1024 /*alignment*/ + 512 /*barriers*/;
@@ -251,25 +264,29 @@ __device__ __forceinline__ void stage_read8(const float* stage, int r, int c, fl
   v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
 
-// Epi: Epi::Args (kernel parameter), Epi::kGroups (problems per launch), Epi::Aux (values prefetched for one 32 x 32
-// block), Epi(args, m, n, batch entry, split), fetch(aux, row0, col0, lane),
-// store(aux, stage, row0, col0, lane) and error_word() (the translation unit's).
+// Epi: Epi::Args (kernel parameter, per group), Epi::kGroups (problems per
+// launch), kStagingBytes (shared memory per epilogue warp, a multiple of 1024),
+// Epi(launch, staging, barrier, lane), begin(group, item, row0), fetch(col0)
+// (starts what the next block reads), store(accumulator, col0) (a block of 32
+// rows: 64 columns from TMEM, or 32 summed ones with PLANES = 2), finish(), and
+// error_word() (the translation unit's).
 template <int CG, int BN, int PLANES, class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
     half_gemm_kernel(const __grid_constant__ LaunchOf<Epi> L) {
-  using T = Tile<CG, BN, PLANES>;
+  using T = Tile<CG, BN, PLANES, Epi::kStagingBytes>;
   constexpr int BM = CG * kRows;
   constexpr int STAGES = T::kStages;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // 128-byte swizzled tiles need 1024-byte alignment
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* staging = reinterpret_cast<float*>(tiles + STAGES * T::kStage);
+  unsigned char* staging = tiles + STAGES * T::kStage;
   uint64_t* full = reinterpret_cast<uint64_t*>(tiles + STAGES * T::kStage + T::kStaging);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* epi_bars = acc_empty + 2;  // one per epilogue warp, for the blocks it loads
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bars + kEpiWarps);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
@@ -284,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], CG * kEpiWarps);  // one arrival per epilogue warp of the pair
     }
+    for (int e = 0; e < kEpiWarps; ++e) mbar_init(&epi_bars[e], 1);
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc_cg<CG>(tmem_slot, T::kTmemCols);
@@ -380,10 +398,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
-    // Warp e of a TMEM lane quarter (32 rows) takes alternate 32-column blocks.
-    const int quarter = warp & 3, e = warp - 2;
-    float* stage = staging + e * (32 * 32);
-    const int c_first = 32 * (e >> 2);
+    // Two warps share a TMEM lane quarter (32 rows) and take alternate column blocks.
+    const int quarter = warp & 3, e = warp - 2, half_of = e >> 2;
     // the accumulator may be overwritten once every epilogue warp has read it
     auto release = [&](int b) {
       tc_fence_before();
@@ -393,28 +409,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         else mbar_arrive(&acc_empty[b]);
       }
     };
-    auto put = [&](const float (&v)[32]) {  // row `lane` of the warp's block
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        *reinterpret_cast<float4*>(stage + stage_idx(lane, 4 * q)) =
-            make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-      __syncwarp();
-    };
+    Epi epi(L, staging + e * Epi::kStagingBytes, &epi_bars[e], lane);
     int j = 0;
     for (int w = first; w < L.items && ok; w += step) {
       const Item item = item_of<BM, BN>(L, w);
       const auto& g = L.g[item.g];
-      const Epi epi(g.epi, g.m, g.n, item.batch, item.split);
       const int row0 = item.m0 + (int)rank * kRows + quarter * 32;
-      typename Epi::Aux aux;
-      epi.fetch(aux, row0, item.n0 + c_first, lane);  // beside the wait for the accumulator
+      epi.begin(g, item, row0);
       if constexpr (PLANES == 2) {
+        // 32-column blocks half_of, half_of + 2, ..
         constexpr int NB = BN / 64;
+        const int c_first = 32 * half_of;
         float sum[NB][32];
 #pragma unroll
         for (int q = 0; q < NB; ++q)
 #pragma unroll
           for (int x = 0; x < 32; ++x) sum[q][x] = 0.0f;
+        epi.fetch(item.n0 + c_first);  // beside the wait for the accumulator
         for (int kt = item.kt0; kt < item.kt1; kt += kSumSlices, ++j) {
           const int b = j & 1;
           if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
@@ -431,30 +442,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
-          put(sum[q]);
-          epi.store(aux, stage, row0, item.n0 + c_first + 64 * q, lane);
-          __syncwarp();
-          if (q + 1 < NB) epi.fetch(aux, row0, item.n0 + c_first + 64 * (q + 1), lane);
+          epi.store(sum[q], item.n0 + c_first + 64 * q);
+          if (q + 1 < NB) epi.fetch(item.n0 + c_first + 64 * (q + 1));
         }
       } else {
+        // 64-column blocks half_of, half_of + 2, ..
         const int b = j & 1;
+        const uint32_t acc = tmem + b * BN + ((uint32_t)(quarter * 32) << 16);
+        if (64 * half_of < BN) epi.fetch(item.n0 + 64 * half_of);  // beside the wait for the accumulator
         if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = c_first; c0 < BN; c0 += 64) {
-          float v[32];
-          tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c0, v);
-          put(v);
-          typename Epi::Aux next;
-          if (c0 + 64 < BN) epi.fetch(next, row0, item.n0 + c0 + 64, lane);
-          epi.store(aux, stage, row0, item.n0 + c0, lane);
-          __syncwarp();
-          aux = next;
+        for (int c0 = 64 * half_of; c0 < BN; c0 += 128) {
+          if (c0 >= 128) epi.fetch(item.n0 + c0);
+          if (!(ok = epi.store(acc + c0, item.n0 + c0, error_word))) break;
         }
         release(b);
         ++j;
       }
     }
+    epi.finish();
   }
   // after a timeout, the copies and products still in flight get time to land
   // before the shared memory and TMEM they use are given back
@@ -510,6 +517,22 @@ inline int make_half_map(CUtensorMap* map, const void* ptr, bool bf16, int64_t r
   return kOk;
 }
 
+// 3-D map of a result or residual: blocks of 128 bytes x 32 rows, swizzled.
+inline int make_block_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* ptr, int64_t rows,
+                          int64_t cols, int64_t ld, int64_t planes, int64_t stride) {
+  auto fn = encode_fn();
+  CG_REQUIRE(fn != nullptr, "half gemm: cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(stride * size)};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CG_REQUIRE(r == CUDA_SUCCESS, "half gemm: cuTensorMapEncodeTiled failed (%d): rows %lld cols %lld ld %lld", (int)r,
+             (long long)rows, (long long)cols, (long long)ld);
+  return kOk;
+}
+
 // Fill in a group's tile counts; the caller has set m, n, k, batch, splits,
 // kt_per and lower. Returns its items.
 template <int CG, int BN, class EpiArgs>
@@ -528,7 +551,7 @@ int64_t plan_group(Group<EpiArgs>& g) {
 
 template <int CG, int BN, int PLANES, class Epi>
 int launch_half_gemm(const LaunchOf<Epi>& L, cudaStream_t stream) {
-  using T = Tile<CG, BN, PLANES>;
+  using T = Tile<CG, BN, PLANES, Epi::kStagingBytes>;
   auto kernel = half_gemm_kernel<CG, BN, PLANES, Epi>;
   CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));
   const int slots = sm_count() / CG;

@@ -241,60 +241,80 @@ struct EpiArgs {
 
 struct EpiBase {
   using Args = EpiArgs;
+  using L = half::Launch<EpiArgs, muon::kGroups>;
   static constexpr int kGroups = muon::kGroups;
-  struct Aux {
-    Planes8 p[4];
-  };
-  const EpiArgs& a;
-  int m, n, batch;
-  __device__ EpiBase(const EpiArgs& args, int m_, int n_, int batch_) : a(args), m(m_), n(n_), batch(batch_) {}
+  static constexpr int kStagingBytes = 32 * 32 * 4;
+  float* stage;
+  const EpiArgs* a;
+  Planes8 aux[4];
+  int lane, m, n, batch, row0;
+  __device__ EpiBase(const L&, unsigned char* staging, uint64_t*, int lane_)
+      : stage(reinterpret_cast<float*>(staging)), lane(lane_) {}
   static __device__ int* error_word() { return &g_muon_error; }
-
+  __device__ void begin(const half::Group<EpiArgs>& g, const half::Item& item, int row) {
+    a = &g.epi;
+    m = g.m;
+    n = g.n;
+    batch = item.batch;
+    row0 = row;
+  }
   // lane -> rows (lane >> 2) + 8 i, columns 8 (lane & 3) .. + 7 of the block;
   // planes have pitches of whole groups of eight
-  __device__ void fetch(Aux& aux, int row0, int col0, int lane) const {
-    if (a.aux == nullptr) return;
+  __device__ void fetch(int col0) {
+    if (a->aux == nullptr) return;
     const int col = col0 + (lane & 3) * 8;
-    const __half* base = a.aux + batch * 2 * a.aux_plane + col;
+    const __half* base = a->aux + batch * 2 * a->aux_plane + col;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = row0 + (lane >> 2) + 8 * i;
       if (row < m && col < n) {
-        const __half* at = base + (int64_t)row * a.aux_pitch;
-        aux.p[i].hi = *reinterpret_cast<const uint4*>(at);
-        aux.p[i].lo = *reinterpret_cast<const uint4*>(at + a.aux_plane);
+        const __half* at = base + (int64_t)row * a->aux_pitch;
+        aux[i].hi = *reinterpret_cast<const uint4*>(at);
+        aux[i].lo = *reinterpret_cast<const uint4*>(at + a->aux_plane);
       } else {
-        aux.p[i].hi = aux.p[i].lo = make_uint4(0, 0, 0, 0);
+        aux[i].hi = aux[i].lo = make_uint4(0, 0, 0, 0);
       }
     }
   }
+  __device__ __forceinline__ void put_rows(const float (&v)[32]) {  // row `lane` of the block
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4*>(stage + half::stage_idx(lane, 4 * q)) =
+          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    __syncwarp();
+  }
+  __device__ __forceinline__ void put_back8(int r, int c, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(stage + half::stage_idx(r, c)) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(stage + half::stage_idx(r, c + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+  }
   __device__ __forceinline__ void value8(const Planes8& p, float (&v)[8]) const {
-    if (a.aux) {
+    if (a->aux) {
       float x[8];
       join8(p, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = a.alpha * x[e] + a.beta * v[e];
+      for (int e = 0; e < 8; ++e) v[e] = a->alpha * x[e] + a->beta * v[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= a.beta;
+      for (int e = 0; e < 8; ++e) v[e] *= a->beta;
     }
   }
+  __device__ void finish() {}
 };
 
 // The result as planes, for the next product.
 struct SplitEpi : EpiBase {
-  __device__ SplitEpi(const EpiArgs& args, int m_, int n_, int batch_, int /*split*/) : EpiBase(args, m_, n_, batch_) {}
-
+  using EpiBase::EpiBase;
   __device__ __forceinline__ void put8(const float (&v)[8], int64_t row, int col) const {
-    __half* at = a.out + batch * 2 * a.out_plane + row * a.out_pitch + col;
+    __half* at = a->out + batch * 2 * a->out_plane + row * a->out_pitch + col;
     Planes8 p;
     split8(v, p);
     *reinterpret_cast<uint4*>(at) = p.hi;
-    *reinterpret_cast<uint4*>(at + a.out_plane) = p.lo;
+    *reinterpret_cast<uint4*>(at + a->out_plane) = p.lo;
   }
-  __device__ void store(const Aux& aux, float* stage, int row0, int col0, int lane) const {
-    if (a.lower && row0 + 31 < col0) return;  // above the diagonal: its mirror block writes it
-    const bool diagonal = a.lower && row0 == col0, mirror = a.lower && !diagonal;
+  __device__ void store(const float (&acc)[32], int col0) {
+    if (a->lower && row0 + 31 < col0) return;  // above the diagonal: its mirror block writes it
+    put_rows(acc);
+    const bool diagonal = a->lower && row0 == col0, mirror = a->lower && !diagonal;
     const int c = (lane & 3) * 8, col = col0 + c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -306,11 +326,8 @@ struct SplitEpi : EpiBase {
       } else {
         half::stage_read8(stage, r, c, v);
       }
-      value8(aux.p[i], v);
-      if (mirror) {
-        *reinterpret_cast<float4*>(stage + half::stage_idx(r, c)) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(stage + half::stage_idx(r, c + 4)) = make_float4(v[4], v[5], v[6], v[7]);
-      }
+      value8(aux[i], v);
+      if (mirror) put_back8(r, c, v);
       if (row < m && col < n) put8(v, row, col);
     }
     if (mirror) {
@@ -324,6 +341,7 @@ struct SplitEpi : EpiBase {
         if (col0 + t < n && row0 + c < m) put8(v, col0 + t, row0 + c);
       }
     }
+    __syncwarp();
   }
 };
 
@@ -337,8 +355,10 @@ struct FinalEpi : EpiBase {
   T* out;
   int64_t ld;
   bool vec;
-  __device__ FinalEpi(const EpiArgs& args, int m_, int n_, int batch_, int /*split*/) : EpiBase(args, m_, n_, batch_) {
-    const OutRef ref = args.table[batch_];
+  using EpiBase::EpiBase;
+  __device__ void begin(const half::Group<EpiArgs>& g, const half::Item& item, int row) {
+    EpiBase::begin(g, item, row);
+    const OutRef ref = a->table[batch];
     out = static_cast<T*>(ref.ptr);
     ld = ref.ld;
     constexpr int kGroup = 16 / sizeof(T);
@@ -346,53 +366,54 @@ struct FinalEpi : EpiBase {
   }
   __device__ __forceinline__ void put8(const float (&v)[8], float* p) const {
     float4* q = reinterpret_cast<float4*>(p);
-    if (a.keep != 0.0f) {
+    const float rate = a->rate, keep = a->keep;
+    if (keep != 0.0f) {
       const float4 x = q[0], y = q[1];
-      q[0] = make_float4(a.keep * x.x + a.rate * v[0], a.keep * x.y + a.rate * v[1], a.keep * x.z + a.rate * v[2],
-                         a.keep * x.w + a.rate * v[3]);
-      q[1] = make_float4(a.keep * y.x + a.rate * v[4], a.keep * y.y + a.rate * v[5], a.keep * y.z + a.rate * v[6],
-                         a.keep * y.w + a.rate * v[7]);
+      q[0] = make_float4(keep * x.x + rate * v[0], keep * x.y + rate * v[1], keep * x.z + rate * v[2],
+                         keep * x.w + rate * v[3]);
+      q[1] = make_float4(keep * y.x + rate * v[4], keep * y.y + rate * v[5], keep * y.z + rate * v[6],
+                         keep * y.w + rate * v[7]);
     } else {
-      q[0] = make_float4(a.rate * v[0], a.rate * v[1], a.rate * v[2], a.rate * v[3]);
-      q[1] = make_float4(a.rate * v[4], a.rate * v[5], a.rate * v[6], a.rate * v[7]);
+      q[0] = make_float4(rate * v[0], rate * v[1], rate * v[2], rate * v[3]);
+      q[1] = make_float4(rate * v[4], rate * v[5], rate * v[6], rate * v[7]);
     }
   }
   template <class H>
   __device__ __forceinline__ void put8(const float (&v)[8], H* p) const {
     H h[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) put_value(h + e, a.rate * v[e]);
+    for (int e = 0; e < 8; ++e) put_value(h + e, a->rate * v[e]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
   }
-  __device__ void store(const Aux& aux, float* stage, int row0, int col0, int lane) const {
+  __device__ void store(const float (&acc)[32], int col0) {
+    put_rows(acc);
     const int c = (lane & 3) * 8, col = col0 + c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = (lane >> 2) + 8 * i, row = row0 + r;
       float v[8];
       half::stage_read8(stage, r, c, v);
-      value8(aux.p[i], v);
+      value8(aux[i], v);
       if (vec) {
         if (row < m && col < n) put8(v, out + row * ld + col);
       } else {
-        *reinterpret_cast<float4*>(stage + half::stage_idx(r, c)) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(stage + half::stage_idx(r, c + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+        put_back8(r, c, v);
       }
     }
-    if (!vec) {  // odd pitches: one column per lane
-      __syncwarp();
-      const int cs = col0 + lane;
-      if (cs >= n) return;
+    __syncwarp();
+    const int cs = col0 + lane;
+    if (!vec && cs < n) {  // odd pitches: one column per lane
 #pragma unroll 8
       for (int r = 0; r < 32; ++r) {
         const int row = row0 + r;
         if (row >= m) break;
-        float v = a.rate * stage[half::stage_idx(r, lane)];
+        float v = a->rate * stage[half::stage_idx(r, lane)];
         T* p = out + row * ld + cs;
-        if (sizeof(T) == 4 && a.keep != 0.0f) v += a.keep * *reinterpret_cast<const float*>(p);
+        if (sizeof(T) == 4 && a->keep != 0.0f) v += a->keep * *reinterpret_cast<const float*>(p);
         put_value(p, v);
       }
     }
+    __syncwarp();
   }
 };
 
