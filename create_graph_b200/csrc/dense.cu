@@ -66,30 +66,45 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 }
 
 // ---- activations ---------------------------------------------------------------
-// The hardware-approximated exp and division (about 1e-6 relative, far below
-// the 2^-9 or 2^-11 of the output's rounding) keep the epilogue warps ahead of
-// the tensor cores; exp overflowing to infinity gives 0, the limit. The normal
-// distribution function Phi is Abramowitz and Stegun's formula 7.1.26 for erfc
-// (absolute error below 1.5e-7), taken on the side where it is small: with
-// CUDA's erff the gelu epilogue alone outlasted the products (65536 x 3072 x
-// 768: 509 us against 298 us without an activation).
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// The hardware's approximate 2^x and reciprocal (about 1e-6 relative together,
+// far below the 2^-9 or 2^-11 of the output's rounding; results below 2^-126
+// are flushed to zero) keep the epilogue warps ahead of the tensor cores; 2^x
+// overflowing to infinity gives 0, the limit. The normal distribution function
+// Phi is Abramowitz and Stegun's formula 7.1.26 for erfc (absolute error below
+// 1.5e-7), taken on the side where it is small: with CUDA's erff the gelu
+// epilogue alone outlasted the products (65536 x 3072 x 768: 509 us against
+// 298 us without an activation).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f;
+constexpr float kInvSqrt2Pi = 0.39894228f;
 
-// Phi(z), and e = exp(-z^2 / 2)
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678f;
-  const float t = __fdividef(1.0f, 1.0f + 0.3275911f * x);
-  e = __expf(-x * x);
+__device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.0f + exp2_approx(-kLog2e * z)); }
+
+// 1 - Phi(|z|), and e = exp(-z^2 / 2)
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+  const float t = rcp_approx(1.0f + (0.3275911f * 0.70710678f) * fabsf(z));
+  e = exp2_approx(z * z * (-0.5f * kLog2e));
   const float poly =
-      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * poly * e;
-  return z < 0.0f ? tail : 1.0f - tail;
+      t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  return poly * e;
 }
 
 __device__ __forceinline__ float act(float z, int kind) {
-  float e;
-  if (kind == CG_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
-  if (kind == CG_ACT_GELU) return z * normal_cdf(z, e);
+  if (kind == CG_ACT_SILU) return z * sigmoid(z);
+  if (kind == CG_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|))
+    float e;
+    const float tail = normal_tail(z, e);
+    return fmaxf(z, 0.0f) - fminf(fabsf(z), 64.0f) * tail;  // the tail is 0 long before 64
+  }
   if (kind == CG_ACT_RELU) return z < 0.0f ? 0.0f : z;
   return z;
 }
@@ -100,8 +115,8 @@ __device__ __forceinline__ float act_grad(float z, int kind) {
   }
   if (kind == CG_ACT_GELU) {  // Phi(z) + z phi(z)
     float e;
-    const float p = normal_cdf(z, e);
-    return p + z * 0.39894228f * e;
+    const float tail = normal_tail(z, e);
+    return (z < 0.0f ? tail : 1.0f - tail) + kInvSqrt2Pi * z * e;
   }
   if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
@@ -111,7 +126,7 @@ __device__ __forceinline__ float act_grad2(float z, int kind) {
     const float s = sigmoid(z);
     return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
   }
-  if (kind == CG_ACT_GELU) return 0.39894228f * __expf(-0.5f * z * z) * (2.0f - z * z);
+  if (kind == CG_ACT_GELU) return kInvSqrt2Pi * exp2_approx(z * z * (-0.5f * kLog2e)) * (2.0f - z * z);
   return 0.0f;
 }
 

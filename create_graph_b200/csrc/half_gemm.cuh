@@ -46,7 +46,7 @@ constexpr int kRows = 128;     // accumulator rows per CTA
 constexpr int kEpiWarps = 8;   // two per TMEM lane quarter
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kSumSlices = 2;  // k-slices summed in one accumulator when PLANES = 2
-constexpr int kBand = 8;       // m-tiles of one band of the tile walk
+constexpr int kBand = 8;       // m-tiles of one band of the tile walk (a power of two)
 
 // Bounded wait: 2^24 polls are about half a second at the least, hundreds of
 // times the longest tile.
@@ -178,6 +178,23 @@ struct Tile {
   static_assert(kStages >= 3 && kTmemCols <= 512, "tile");
 };
 
+// Division of 0 <= n < 2^31 by a fixed d >= 1, without the dozens of
+// instructions of an integer division: floor(n m / 2^(32 + s)) with m = the
+// ceiling of 2^(32 + s) / d, s = ceil(log2 d) - 1 (Granlund and Montgomery,
+// Division by invariant integers using multiplication).
+struct Divisor {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s); }
+};
+inline Divisor divisor(int64_t d) {
+  Divisor r = {(uint32_t)d, 0, 0};
+  if (d > 1) {
+    while ((2ll << r.s) < d) ++r.s;
+    r.m = (uint32_t)(((1ull << (32 + r.s)) + (uint64_t)d - 1) / (uint64_t)d);
+  }
+  return r;
+}
+
 // One problem of a launch: `batch` products of one shape.
 template <class EpiArgs>
 struct Group {
@@ -189,6 +206,7 @@ struct Group {
   int splits, kt_per;        // k-slices per split
   int lower;                 // symmetric result: only tiles that reach the lower triangle
   int tiles;                 // items per batch entry and split
+  Divisor by_tiles, by_batch, by_band, by_last;  // by tiles, batch, a band's tiles, the last band's height
   int first_item;
   EpiArgs epi;
 };
@@ -222,10 +240,10 @@ __device__ inline Item item_of(const Launch<EpiArgs, GROUPS>& L, int w) {
     while (it.g + 1 < L.groups && w >= L.g[it.g + 1].first_item) ++it.g;
   const Group<EpiArgs>& g = L.g[it.g];
   w -= g.first_item;
-  int t = w % g.tiles;
-  w /= g.tiles;
-  it.batch = w % g.batch;
-  it.split = w / g.batch;
+  const int which = g.by_tiles.div(w);
+  int t = w - which * g.tiles;
+  it.split = g.by_batch.div(which);
+  it.batch = which - it.split * g.batch;
   int mt, nt;
   if (g.lower) {
     mt = 0;
@@ -238,11 +256,11 @@ __device__ inline Item item_of(const Launch<EpiArgs, GROUPS>& L, int w) {
   } else {
     // bands of kBand m-tiles, each walked m first: a wave of tiles then covers
     // a near-square block and reads few rows of either operand
-    const int band = t / (kBand * g.n_tiles);
+    const int band = g.by_band.div(t);
     t -= band * kBand * g.n_tiles;
-    const int high = g.m_tiles - band * kBand < kBand ? g.m_tiles - band * kBand : kBand;
-    mt = band * kBand + t % high;
-    nt = t / high;
+    const int high = g.m_tiles - band * kBand;
+    nt = high >= kBand ? t / kBand : g.by_last.div(t);
+    mt = band * kBand + t - nt * (high >= kBand ? kBand : high);
   }
   it.m0 = mt * BM;
   it.n0 = nt * BN;
@@ -546,6 +564,10 @@ int64_t plan_group(Group<EpiArgs>& g) {
     for (int i = 0; i < g.m_tiles; ++i) tiles += lower_tiles_of_row(i, BM, BN, g.n_tiles);
   }
   g.tiles = (int)tiles;
+  g.by_tiles = divisor(tiles);
+  g.by_batch = divisor(g.batch);
+  g.by_band = divisor((int64_t)kBand * g.n_tiles);
+  g.by_last = divisor(g.m_tiles % kBand ? g.m_tiles % kBand : kBand);
   return tiles * g.batch * g.splits;
 }
 
