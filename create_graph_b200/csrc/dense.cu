@@ -146,15 +146,72 @@ struct EpiArgs {
   int act;
 };
 
+// Two fp32 values per instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.ftz.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.ftz.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 1 / d for two values of at most 2^60 with one reciprocal: the special
+// function unit (16 results per clock and SM) bounds these epilogues, two
+// per element of a 128 x 256 tile are 4096 clocks.
+__device__ __forceinline__ float2 rcp2(float2 d) {
+  const float r = rcp_approx(d.x * d.y);
+  return make_float2(r * d.y, r * d.x);
+}
+
+// silu of two values. 2^-x is held to 2^60, so below z = -41 the sigmoid stays
+// at 2^-60 (times z: 4e-17, where the exact value is smaller still).
+__device__ __forceinline__ float2 silu2(float2 z) {
+  const float2 x = mul2(z, both(-kLog2e));
+  const float2 e = make_float2(exp2_approx(fminf(x.x, 60.0f)), exp2_approx(fminf(x.y, 60.0f)));
+  return mul2(z, rcp2(make_float2(1.0f + e.x, 1.0f + e.y)));
+}
+// gelu of two values: max(z, 0) - |z| (1 - Phi(|z|)), the tail (0 long before
+// 64) as in normal_tail
+__device__ __forceinline__ float2 gelu2(float2 z) {
+  const float2 a = make_float2(fminf(fabsf(z.x), 64.0f), fminf(fabsf(z.y), 64.0f));
+  const float2 t = rcp2(fma2(a, both(0.3275911f * 0.70710678f), both(1.0f)));
+  const float2 u = mul2(mul2(a, a), both(-0.5f * kLog2e));
+  const float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
+  float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+  p = fma2(t, p, both(0.7107068705f));
+  p = fma2(t, p, both(-0.142248368f));
+  p = fma2(t, p, both(0.127414796f));
+  const float2 w = mul2(mul2(mul2(p, t), e), a);
+  return fma2(make_float2(z.x + fabsf(z.x), z.y + fabsf(z.y)), both(0.5f), make_float2(-w.x, -w.y));
+}
+
 // f applied to a thread's values; the branch on the kind is outside the loop.
 template <int N>
 __device__ __forceinline__ void act_all(float (&v)[N], int kind) {
   if (kind == CG_ACT_SILU) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = act(v[e], CG_ACT_SILU);
+    for (int e = 0; e < N; e += 2) {
+      const float2 y = silu2(make_float2(v[e], v[e + 1]));
+      v[e] = y.x;
+      v[e + 1] = y.y;
+    }
   } else if (kind == CG_ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = act(v[e], CG_ACT_GELU);
+    for (int e = 0; e < N; e += 2) {
+      const float2 y = gelu2(make_float2(v[e], v[e + 1]));
+      v[e] = y.x;
+      v[e + 1] = y.y;
+    }
   } else if (kind == CG_ACT_RELU) {
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = act(v[e], CG_ACT_RELU);
@@ -183,23 +240,26 @@ struct EpiBase {
 // residual are applied in registers, the rounded row goes to a 128-byte
 // swizzled block in shared memory and TMA writes the block. The residual comes
 // by TMA into the same block beforehand (each thread reads and overwrites its
-// own row), the pre-activation leaves through a second block.
+// own row); the pre-activation follows through the same block, read from TMEM
+// once more. Sixteen warps, one block each of a 256-wide tile, hide one
+// another's latencies (65536 x 3072 x 768 with gelu: 287 us, eight warps 323 us).
 // Against staging fp32 blocks and storing 64-byte row segments from the
 // threads this halves the shared-memory traffic that competes with the
 // operands: 65536 x 3072 x 768 with no activation took 298 us before, 209 us
 // without any stores.
 template <class T>
 struct BlockEpi : EpiBase {
-  static constexpr int kStagingBytes = 2 * 4096;
+  static constexpr int kWarps = 16;
+  static constexpr int kStagingBytes = 4096;
   using EpiBase::EpiBase;
   uint32_t loads = 0;
 
   __device__ __forceinline__ bool outside(int col0) const { return row0 >= m || col0 >= n; }
-  // 16-byte group c of this thread's row of block b
-  __device__ __forceinline__ uint4* group(int b, int c) const {
-    return reinterpret_cast<uint4*>(staging + b * 4096 + lane * 128 + ((c ^ (lane & 7)) << 4));
+  // 16-byte group c of this thread's row of the block
+  __device__ __forceinline__ uint4* group(int c) const {
+    return reinterpret_cast<uint4*>(staging + lane * 128 + ((c ^ (lane & 7)) << 4));
   }
-  // the blocks are free once the last stores have read them
+  // the block is free once the last store has read it
   __device__ __forceinline__ void fetch(int col0) {
     if (outside(col0)) return;
     if (lane == 0) {
@@ -211,23 +271,43 @@ struct BlockEpi : EpiBase {
     }
     __syncwarp();
   }
+  __device__ __forceinline__ void put(const CUtensorMap* map, int col, int z) {
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) half::tma_store_3d(map, staging, col, row0, z);
+  }
+  __device__ __forceinline__ void reuse() {
+    if (lane == 0) tma_store_wait_read();
+    __syncwarp();
+  }
+  // 32 pre-activations of this thread's row
+  __device__ __forceinline__ void load(uint32_t acc, int col0, float (&v)[32]) const {
+    tmem_load_32(acc, v);
+    if (a.bias == nullptr) return;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = col0 + 8 * c;
+      if (col < n) {
+        float b[8];
+        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + col)), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * c + e] += b[e];
+      }
+    }
+  }
   __device__ __forceinline__ bool store(uint32_t acc, int col0, int* error) {
     if (outside(col0)) return true;
     if (a.partial != nullptr) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+      for (int h = 0; h < 2 && col0 + 32 * h < n; ++h) {
         float v[32];
         tmem_load_32(acc + 32 * h, v);
+        if (h == 1) reuse();
 #pragma unroll
         for (int c = 0; c < 8; ++c)
-          *group(h, c) = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
-                                    __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
-      }
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) {
-        half::tma_store_3d(&a.map_partial, staging, col0, row0, split);
-        if (col0 + 32 < n) half::tma_store_3d(&a.map_partial, staging + 4096, col0 + 32, row0, split);
+          *group(c) = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
+                                 __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
+        put(&a.map_partial, col0 + 32 * h, split);
       }
       return true;
     }
@@ -235,27 +315,7 @@ struct BlockEpi : EpiBase {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[32];
-      tmem_load_32(acc + 32 * h, v);
-      if (a.bias) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = col0 + 32 * h + 8 * c;
-          if (col < n) {
-            float b[8];
-            unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + col)), b);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[8 * c + e] += b[e];
-          }
-        }
-      }
-      if (a.z) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float o[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
-                              v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
-          *group(1, 4 * h + c) = pack8<T>(o);
-        }
-      }
+      load(acc + 32 * h, col0 + 32 * h, v);
       act_all(v, a.act);
       if (a.residual && h == 0) {
         ok = half::wait(bar, loads & 1, error);
@@ -265,7 +325,7 @@ struct BlockEpi : EpiBase {
       for (int c = 0; c < 4; ++c) {
         float o[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
                       v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
-        uint4* at = group(0, 4 * h + c);
+        uint4* at = group(4 * h + c);
         if (a.residual) {
           float r[8];
           unpack8<T>(*at, r);
@@ -275,11 +335,21 @@ struct BlockEpi : EpiBase {
         *at = pack8<T>(o);
       }
     }
-    fence_proxy_async_shared();
-    __syncwarp();
-    if (lane == 0) {
-      if (a.z) half::tma_store_3d(&a.map_z, staging + 4096, col0, row0, 0);
-      half::tma_store_3d(&a.map_y, staging, col0, row0, 0);
+    put(&a.map_y, col0, 0);
+    if (a.z) {
+      reuse();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        load(acc + 32 * h, col0 + 32 * h, v);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float o[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
+                              v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
+          *group(4 * h + c) = pack8<T>(o);
+        }
+      }
+      put(&a.map_z, col0, 0);
     }
     return ok;
   }
@@ -292,6 +362,7 @@ struct BlockEpi : EpiBase {
 // stored one column per lane.
 template <class T>
 struct PlainEpi : EpiBase {
+  static constexpr int kWarps = 8;
   static constexpr int kStagingBytes = 32 * 32 * 4;
   using EpiBase::EpiBase;
   __device__ void fetch(int) {}

@@ -12,8 +12,8 @@
 //               stage back to the producers and each finished accumulator to
 //               the epilogue (two accumulators: an item's epilogue runs beside
 //               the next item's products);
-//   warps 2..9  epilogue: tcgen05.ld (thread = row), the layer's own arithmetic,
-//               and the result through shared memory to global memory.
+//   warps 2..   epilogue: tcgen05.ld (thread = row), the layer's own arithmetic,
+//              and the result through shared memory to global memory.
 // Operands are K-major (contiguous along k) or MN-major (contiguous along m or
 // n), so x W^T, g W and g^T x read their operands as they are stored.
 // PLANES = 2: every operand is a pair of fp16 planes hi + lo (22 significant
@@ -43,8 +43,9 @@ using namespace cg::sm100;
 
 constexpr int kBK = 64;        // half-precision values per k-slice: 128 bytes
 constexpr int kRows = 128;     // accumulator rows per CTA
-constexpr int kEpiWarps = 8;   // two per TMEM lane quarter
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+// warps of a block: producer, issuer and `epi` epilogue warps (a multiple of
+// four, epi / 4 per TMEM lane quarter)
+__host__ __device__ constexpr int threads_of(int epi) { return 32 * (2 + epi); }
 constexpr int kSumSlices = 2;  // k-slices summed in one accumulator when PLANES = 2
 constexpr int kBand = 8;       // m-tiles of one band of the tile walk (a power of two)
 
@@ -163,13 +164,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a
 }
 
 // ---- tiles ------------------------------------------------------------------
-template <int CG, int BN, int PLANES, int STAGING>
+template <int CG, int BN, int PLANES, class Epi>
 struct Tile {
   static constexpr int kBRows = BN / CG;                       // B rows this CTA stages
   static constexpr int kA = kRows * kBK * 2;
   static constexpr int kB = kBRows * kBK * 2;
   static constexpr int kStage = PLANES * (kA + kB);
-  static constexpr int kStaging = kEpiWarps * STAGING;         // the epilogue warps' own blocks
+  static constexpr int kStaging = Epi::kWarps * Epi::kStagingBytes;  // the epilogue warps' own blocks
   static constexpr int kStagesFit = (227 * 1024 - kStaging - 1024 - 512) / kStage;
   static constexpr int kStages = kStagesFit < 8 ? kStagesFit : 8;
   static constexpr int kBytes = kStages * kStage + kStaging + 1024 /*alignment*/ + 512 /*barriers*/;
@@ -283,17 +284,18 @@ __device__ __forceinline__ void stage_read8(const float* stage, int r, int c, fl
 }
 
 // Epi: Epi::Args (kernel parameter, per group), Epi::kGroups (problems per
-// launch), kStagingBytes (shared memory per epilogue warp, a multiple of 1024),
+// launch), kWarps, kStagingBytes (shared memory per epilogue warp, a multiple of 1024),
 // Epi(launch, staging, barrier, lane), begin(group, item, row0), fetch(col0)
 // (starts what the next block reads), store(accumulator, col0) (a block of 32
 // rows: 64 columns from TMEM, or 32 summed ones with PLANES = 2), finish(), and
 // error_word() (the translation unit's).
 template <int CG, int BN, int PLANES, class Epi>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
     half_gemm_kernel(const __grid_constant__ LaunchOf<Epi> L) {
-  using T = Tile<CG, BN, PLANES, Epi::kStagingBytes>;
+  using T = Tile<CG, BN, PLANES, Epi>;
   constexpr int BM = CG * kRows;
   constexpr int STAGES = T::kStages;
+  constexpr int WARPS = Epi::kWarps;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // 128-byte swizzled tiles need 1024-byte alignment
   unsigned char* tiles = reinterpret_cast<unsigned char*>(
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* epi_bars = acc_empty + 2;  // one per epilogue warp, for the blocks it loads
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bars + kEpiWarps);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bars + WARPS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
@@ -317,9 +319,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], CG * kEpiWarps);  // one arrival per epilogue warp of the pair
+      mbar_init(&acc_empty[b], CG * WARPS);  // one arrival per epilogue warp of the pair
     }
-    for (int e = 0; e < kEpiWarps; ++e) mbar_init(&epi_bars[e], 1);
+    for (int e = 0; e < WARPS; ++e) mbar_init(&epi_bars[e], 1);
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc_cg<CG>(tmem_slot, T::kTmemCols);
@@ -416,8 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 2) {
     // ---------------- epilogue ----------------
-    // Two warps share a TMEM lane quarter (32 rows) and take alternate column blocks.
-    const int quarter = warp & 3, e = warp - 2, half_of = e >> 2;
+    // WARPS / 4 warps share a TMEM lane quarter (32 rows) and take turns with its column blocks.
+    const int quarter = warp & 3, e = warp - 2, turn = e >> 2;
     // the accumulator may be overwritten once every epilogue warp has read it
     auto release = [&](int b) {
       tc_fence_before();
@@ -435,9 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row0 = item.m0 + (int)rank * kRows + quarter * 32;
       epi.begin(g, item, row0);
       if constexpr (PLANES == 2) {
-        // 32-column blocks half_of, half_of + 2, ..
-        constexpr int NB = BN / 64;
-        const int c_first = 32 * half_of;
+        // 32-column blocks turn, turn + WARPS / 4, ..
+        constexpr int STEP = 8 * WARPS, NB = BN / STEP;
+        const int c_first = 32 * turn;
         float sum[NB][32];
 #pragma unroll
         for (int q = 0; q < NB; ++q)
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int q = 0; q < NB; ++q) {
             float v[32];
-            tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + 64 * q, v);
+            tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + STEP * q, v);
 #pragma unroll
             for (int x = 0; x < 32; ++x) sum[q][x] += v[x];
           }
@@ -460,19 +462,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
-          epi.store(sum[q], item.n0 + c_first + 64 * q);
-          if (q + 1 < NB) epi.fetch(item.n0 + c_first + 64 * (q + 1));
+          epi.store(sum[q], item.n0 + c_first + STEP * q);
+          if (q + 1 < NB) epi.fetch(item.n0 + c_first + STEP * (q + 1));
         }
       } else {
-        // 64-column blocks half_of, half_of + 2, ..
+        // 64-column blocks turn, turn + WARPS / 4, ..
+        constexpr int STEP = 16 * WARPS;
         const int b = j & 1;
         const uint32_t acc = tmem + b * BN + ((uint32_t)(quarter * 32) << 16);
-        if (64 * half_of < BN) epi.fetch(item.n0 + 64 * half_of);  // beside the wait for the accumulator
+        if (64 * turn < BN) epi.fetch(item.n0 + 64 * turn);  // beside the wait for the accumulator
         if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = 64 * half_of; c0 < BN; c0 += 128) {
-          if (c0 >= 128) epi.fetch(item.n0 + c0);
+        for (int c0 = 64 * turn; c0 < BN; c0 += STEP) {
+          if (c0 >= STEP) epi.fetch(item.n0 + c0);
           if (!(ok = epi.store(acc + c0, item.n0 + c0, error_word))) break;
         }
         release(b);
@@ -573,13 +576,13 @@ int64_t plan_group(Group<EpiArgs>& g) {
 
 template <int CG, int BN, int PLANES, class Epi>
 int launch_half_gemm(const LaunchOf<Epi>& L, cudaStream_t stream) {
-  using T = Tile<CG, BN, PLANES, Epi::kStagingBytes>;
+  using T = Tile<CG, BN, PLANES, Epi>;
   auto kernel = half_gemm_kernel<CG, BN, PLANES, Epi>;
   CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));
   const int slots = sm_count() / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * (L.items < slots ? L.items : slots)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads_of(Epi::kWarps));
   cfg.dynamicSmemBytes = T::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

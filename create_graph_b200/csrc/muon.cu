@@ -243,6 +243,7 @@ struct EpiBase {
   using Args = EpiArgs;
   using L = half::Launch<EpiArgs, muon::kGroups>;
   static constexpr int kGroups = muon::kGroups;
+  static constexpr int kWarps = 8;
   static constexpr int kStagingBytes = 32 * 32 * 4;
   float* stage;
   const EpiArgs* a;
