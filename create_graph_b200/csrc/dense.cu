@@ -747,6 +747,91 @@ static int act_grad_run(const cg_act_grad_args* args, void* stream) {
   return act_grad_typed<__nv_bfloat16>(g, as_stream(stream));
 }
 
+// The products of a backward: dx = gz W (W read along n) and dW = gz^T x.
+static cg_linear_args dx_product(const cg_linear_backward_args& g) {
+  cg_linear_args p;
+  memset(&p, 0, sizeof(p));
+  p.m = g.m;
+  p.n = g.k;
+  p.k = g.n;
+  p.a = g.act == CG_ACT_NONE ? g.gy : g.gz;
+  p.lda = g.act == CG_ACT_NONE ? g.ld_gy : g.ld_gz;
+  p.b = g.w;
+  p.ldb = g.ld_w;
+  p.b_mn_major = !g.w_mn_major;
+  p.y = g.dx;
+  p.ld_y = g.k;
+  p.dtype = g.dtype;
+  return p;
+}
+static cg_linear_args dw_product(const cg_linear_backward_args& g) {
+  cg_linear_args p = dx_product(g);
+  p.m = g.n;
+  p.k = g.m;
+  p.a_mn_major = 1;
+  p.b = g.x;
+  p.ldb = g.ld_x;
+  p.b_mn_major = !g.x_mn_major;
+  p.y = g.dw;
+  return p;
+}
+
+// One region serves the column sums and then each product in turn.
+static int64_t backward_workspace(const cg_linear_backward_args& g) {
+  if (g.m <= 0 || g.n <= 0 || g.k <= 0) return 0;
+  int64_t most = g.db ? act_grad_scratch(g.m, g.n) : 0;
+  const int64_t x = g.dx ? workspace_bytes(dx_product(g)) : 0, w = g.dw ? workspace_bytes(dw_product(g)) : 0;
+  if (x > most) most = x;
+  return w > most ? w : most;
+}
+
+static int backward_run(const cg_linear_backward_args* args, void* stream) {
+  CG_REQUIRE(args != nullptr, "linear_half_backward: args is NULL");
+  const cg_linear_backward_args& g = *args;
+  CG_REQUIRE(g.m >= 1 && g.n >= 1 && g.k >= 1, "linear_half_backward: sizes must be at least 1");
+  CG_REQUIRE(g.workspace_bytes >= backward_workspace(g) &&
+                 (backward_workspace(g) == 0 || (g.workspace != nullptr && aligned16(g.workspace))),
+             "linear_half_backward: needs %lld workspace bytes on a 16-byte boundary "
+             "(cg_linear_half_backward_workspace_bytes)",
+             (long long)backward_workspace(g));
+  int rc;
+  const bool plain = g.act == CG_ACT_NONE;
+  if (!plain || g.db) {
+    cg_act_grad_args a;
+    memset(&a, 0, sizeof(a));
+    a.rows = g.m;
+    a.cols = g.n;
+    a.gy = g.gy;
+    a.ld_gy = g.ld_gy;
+    a.act = g.act;
+    a.dtype = g.dtype;
+    if (!plain) {
+      CG_REQUIRE(g.z != nullptr && g.gz != nullptr, "linear_half_backward: an activation needs z and gz");
+      a.z = g.z;
+      a.ld_z = g.ld_z;
+      a.gz = g.gz;
+      a.ld_gz = g.ld_gz;
+    }
+    a.db = g.db;
+    a.scratch = static_cast<float*>(g.workspace);
+    a.scratch_bytes = g.workspace_bytes;
+    if ((rc = act_grad_run(&a, stream))) return rc;
+  }
+  if (g.dx) {
+    cg_linear_args p = dx_product(g);
+    p.workspace = static_cast<float*>(g.workspace);
+    p.workspace_bytes = g.workspace_bytes;
+    if ((rc = run(&p, stream))) return rc;
+  }
+  if (g.dw) {
+    cg_linear_args p = dw_product(g);
+    p.workspace = static_cast<float*>(g.workspace);
+    p.workspace_bytes = g.workspace_bytes;
+    if ((rc = run(&p, stream))) return rc;
+  }
+  return kOk;
+}
+
 template <class T>
 static int act_grad2_typed(const void* h, const void* hb, const void* gy, const void* z, void* dgy, void* dz,
                            int64_t rows, int64_t cols, int act, cudaStream_t s) {
@@ -774,6 +859,14 @@ int cg_linear_half(const cg_linear_args* args, void* stream) { return cg::dense:
 int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args) {
   if (args == nullptr || args->m <= 0 || args->n <= 0 || args->k <= 0) return 0;
   return cg::dense::workspace_bytes(*args);
+}
+
+int cg_linear_half_backward(const cg_linear_backward_args* args, void* stream) {
+  return cg::dense::backward_run(args, stream);
+}
+
+int64_t cg_linear_half_backward_workspace_bytes(const cg_linear_backward_args* args) {
+  return args == nullptr ? 0 : cg::dense::backward_workspace(*args);
 }
 
 int cg_act_grad_half(const cg_act_grad_args* args, void* stream) { return cg::dense::act_grad_run(args, stream); }

@@ -25,6 +25,7 @@ not written. The fp32 layers of the energy network are in
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -73,23 +74,34 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
-def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = native.ACT_NONE,
-            residual: Tensor | None = None, keep_z: bool = False):
-    """(y, z) with z = a @ b.T + bias and y = f(z) + residual; z is None unless
-    ``keep_z``. a (M, K), b (N, K), either of them possibly a transposed view."""
-    m, k = a.shape
-    n = b.shape[0]
-    y = torch.empty(m, n, dtype=a.dtype, device=a.device)
-    z = torch.empty_like(y) if keep_z else None
-    if m == 0 or n == 0:
-        return y, z
-    if k == 0:  # an empty sum: one zero column gives it
-        a, b = a.new_zeros(m, 8), b.new_zeros(n, 8)
-        k = 8
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(m: int, n: int, k: int) -> int:
     args = native.LinearArgs()
     args.m, args.n, args.k = m, n, k
-    a, args.lda, args.a_mn_major = _operand(a)
-    b, args.ldb, args.b_mn_major = _operand(b)
+    return native.lib().cg_linear_half_workspace_bytes(ctypes.byref(args))
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_workspace_bytes(m: int, n: int, k: int, act: int, dx: bool, dw: bool, db: bool) -> int:
+    args = native.LinearBackwardArgs()
+    args.m, args.n, args.k, args.act = m, n, k, act
+    args.dx, args.dw, args.db = 16 * dx or None, 16 * dw or None, 16 * db or None  # only whether they are wanted
+    return native.lib().cg_linear_half_backward_workspace_bytes(ctypes.byref(args))
+
+
+def _stream(t: Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _forward(a_op, b_op, shape, bias, activation, residual, keep_z, like):
+    """(y, z) of one product of operands as _operand gives them."""
+    m, n, k = shape
+    y = torch.empty((m, n), dtype=like.dtype, device=like.device)
+    z = torch.empty_like(y) if keep_z else None
+    args = native.LinearArgs()
+    args.m, args.n, args.k = m, n, k
+    a, args.lda, args.a_mn_major = a_op
+    b, args.ldb, args.b_mn_major = b_op
     args.a, args.b = a.data_ptr(), b.data_ptr()
     if bias is not None:
         bias = bias.contiguous()
@@ -100,14 +112,62 @@ def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = 
     if z is not None:
         args.z, args.ld_z = z.data_ptr(), n
     args.y, args.ld_y = y.data_ptr(), n
-    args.act, args.dtype = activation, native.HALF_DTYPES[a.dtype]
-    nbytes = native.lib().cg_linear_half_workspace_bytes(ctypes.byref(args))
+    args.act, args.dtype = activation, native.HALF_DTYPES[like.dtype]
+    nbytes = _workspace_bytes(m, n, k)
     workspace = None
     if nbytes > 0:
-        workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=a.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
-    native.invoke("cg_linear_half", ctypes.byref(args), native.stream_ptr(a.device), info=(m, n, k))
+    native.invoke("cg_linear_half", ctypes.byref(args), _stream(like), info=(m, n, k))
     return y, z
+
+
+def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = native.ACT_NONE,
+            residual: Tensor | None = None, keep_z: bool = False):
+    """(y, z) with z = a @ b.T + bias and y = f(z) + residual; z is None unless
+    ``keep_z``. a (M, K), b (N, K), either of them possibly a transposed view."""
+    m, k = a.shape
+    n = b.shape[0]
+    if m == 0 or n == 0:
+        y = torch.empty(m, n, dtype=a.dtype, device=a.device)
+        return y, torch.empty_like(y) if keep_z else None
+    if k == 0:  # an empty sum: zero columns give it
+        a, b, k = a.new_zeros(m, 8), b.new_zeros(n, 8), 8
+    return _forward(_operand(a), _operand(b), (m, n, k), bias, activation, residual, keep_z, a)
+
+
+def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
+    """(dx, dw, db) in one call; None for what is not wanted."""
+    m, n, k = shape
+    args = native.LinearBackwardArgs()
+    args.m, args.n, args.k, args.act, args.dtype = m, n, k, activation, native.HALF_DTYPES[gy.dtype]
+    gz = None
+    if activation == native.ACT_NONE:
+        if not _fits_tma(gy, 0, 1):
+            copy = _pitched(m, n, gy)
+            copy.copy_(gy)
+            gy = copy
+        args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
+    else:
+        gy = _rows(gy)
+        gz = _pitched(m, n, gy)
+        args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), n)
+        args.z, args.ld_z = z.data_ptr(), n
+        args.gz, args.ld_gz = gz.data_ptr(), -(-n // 8) * 8
+    x, args.ld_x, args.x_mn_major = x_op
+    w, args.ld_w, args.w_mn_major = w_op
+    args.x, args.w = x.data_ptr(), w.data_ptr()
+    dx = torch.empty((m, k), dtype=gy.dtype, device=gy.device) if want_dx else None
+    dw = torch.empty((n, k), dtype=gy.dtype, device=gy.device) if want_dw else None
+    db = torch.empty(n, dtype=gy.dtype, device=gy.device) if want_db else None
+    args.dx, args.dw, args.db = native.ptr(dx), native.ptr(dw), native.ptr(db)
+    nbytes = _backward_workspace_bytes(m, n, k, activation, want_dx, want_dw, want_db)
+    workspace = None
+    if nbytes > 0:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=gy.device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
+    native.invoke("cg_linear_half_backward", ctypes.byref(args), _stream(gy), info=(m, n, k))
+    return dx, dw, db
 
 
 def _act_grad(gy: Tensor, z: Tensor | None, activation: int, want_db: bool):
@@ -129,7 +189,7 @@ def _act_grad(gy: Tensor, z: Tensor | None, activation: int, want_db: bool):
         scratch = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=gy.device)
         args.db, args.scratch, args.scratch_bytes = db.data_ptr(), scratch.data_ptr(), nbytes
     if args.gz or args.db:
-        native.invoke("cg_act_grad_half", ctypes.byref(args), native.stream_ptr(gy.device))
+        native.invoke("cg_act_grad_half", ctypes.byref(args), _stream(gy))
     return gz, db
 
 
@@ -184,7 +244,7 @@ class _ActGrad2(_Fused):
         dgy, dz = torch.empty_like(gy), torch.empty_like(z)
         native.invoke("cg_act_grad2_half", native.ptr(h), native.ptr(hb), gy.data_ptr(), z.data_ptr(),
                       dgy.data_ptr(), dz.data_ptr(), gy.shape[0], gy.shape[1], activation,
-                      native.HALF_DTYPES[gy.dtype], native.stream_ptr(gy.device))
+                      native.HALF_DTYPES[gy.dtype], _stream(gy))
         return dgy, dz
 
     @staticmethod
@@ -192,23 +252,54 @@ class _ActGrad2(_Fused):
         raise NativeError("dense.linear: third derivatives are not supported")
 
 
+# below this many flops a product takes less time than finding out whether its
+# result was asked for (a few microseconds per input, on the host)
+_SMALL_FLOPS = 4e9
+
+
 class _Linear(_Fused):
     """(y, z) from one product; z is None without an activation."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, activation):
-        y, z = product(x, w, b, activation, r, keep_z=activation != native.ACT_NONE)
-        ctx.save_for_backward(x, w, z)
-        ctx.edges = _edges(x, w, b)
         ctx.activation = activation
+        ctx.save = m, n, k = x.shape[0], w.shape[0], x.shape[1]
         # z is seldom used: its gradient arrives as None, not as zeros
         ctx.set_materialize_grads(False)
+        keep_z = activation != native.ACT_NONE
+        ctx.operands = None
+        if min(m, n, k) == 0:
+            y, z = product(x, w, b, activation, r, keep_z)
+        else:
+            # the operands as the products read them: x and w themselves, or
+            # copies whose rows start on 16-byte boundaries
+            ctx.operands = x_op, w_op = _operand(x), _operand(w)
+            y, z = _forward(x_op, w_op, ctx.save, b, activation, r, keep_z, x)
+        ctx.save_for_backward(x, w, z)
+        ctx.inputs = (True, True, b is not None)
         return y, z
+
+    @staticmethod
+    def _wanted(ctx):
+        """Which of x, w, b the backward pass running now needs."""
+        need = ctx.needs_input_grad[:3]
+        m, n, k = ctx.save
+        if 2.0 * m * n * k < _SMALL_FLOPS and not torch.is_grad_enabled():
+            return need
+        nodes = iter(ctx.next_functions)
+        nodes = [next(nodes)[0] if given else None for given in ctx.inputs]
+        return [n and engine_will_execute(node) for n, node in zip(need, nodes)]
 
     @staticmethod
     def backward(ctx, gy, gz_direct):
         x, w, z = ctx.saved_tensors
-        want = [ctx.needs_input_grad[i] and engine_will_execute(ctx.edges[i]) for i in range(3)]
+        want = _Linear._wanted(ctx)
+        dr = gy if ctx.needs_input_grad[3] else None
+        if not torch.is_grad_enabled() and gz_direct is None and gy is not None and ctx.operands is not None:
+            if not any(want):
+                return None, None, None, dr, None
+            return *_backward(gy, z, *ctx.operands, ctx.save, ctx.activation, *want), dr, None
+        # the differentiable path: products and passes that record their own backward
         gz, db = gz_direct, None
         if gy is not None and any(want):
             alone = gz_direct is None
@@ -216,25 +307,26 @@ class _Linear(_Fused):
             if not alone:
                 gz = gz + gz_direct
         if gz is None:
-            return None, None, None, gy, None
+            return None, None, None, dr, None
         if want[2] and db is None:
             db = _ActGrad.apply(gz, None, native.ACT_NONE, True)[1]
         dx = _Product.apply(gz, w.t()) if want[0] else None
         dw = _Product.apply(gz.t(), x.t()) if want[1] else None
-        return dx, dw, db, (gy if ctx.needs_input_grad[3] else None), None
+        return dx, dw, db, dr, None
 
 
 def _checked(x, weight, bias, residual, activation) -> int:
-    native.require_cuda(x, weight, bias, residual)
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise NativeError(f"dense.linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    if x.dtype not in native.HALF_DTYPES:
-        raise NativeError(f"dense.linear: float16 or bfloat16 expected, got {x.dtype} (the fp32 layers are in "
+    dtype, device = x.dtype, x.device
+    if dtype not in native.HALF_DTYPES:
+        raise NativeError(f"dense.linear: float16 or bfloat16 expected, got {dtype} (the fp32 layers are in "
                           "create_graph_b200.nn)")
-    named = {"weight": weight, "bias": bias, "residual": residual}
-    for name, t in named.items():
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise NativeError(f"dense.linear: {name} is {t.dtype} on {t.device}, x {x.dtype} on {x.device}")
+    native.require_cuda(x)
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise NativeError(f"dense.linear: {name} is {t.dtype} on {t.device}, x {dtype} on {device}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise NativeError(f"dense.linear: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
     n = weight.shape[0]
@@ -242,24 +334,27 @@ def _checked(x, weight, bias, residual, activation) -> int:
         raise NativeError(f"dense.linear: bias must be ({n},), got {tuple(bias.shape)}")
     if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
         raise NativeError(f"dense.linear: residual must be {(*x.shape[:-1], n)}, got {tuple(residual.shape)}")
-    return ACTIVATIONS[activation]
+    return act
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation: str = "none",
            residual: Tensor | None = None) -> Tensor:
     """f(x @ weight.T + bias) + residual (see the module's description)."""
     act = _checked(x, weight, bias, residual, activation)
-    n, shape = weight.shape[0], x.shape
+    if x.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return linear(x, weight, bias, activation=activation, residual=residual)
+    shape = x.shape
     if x.dim() != 2:
         x = x.reshape(math.prod(shape[:-1]), shape[-1])
-    if residual is not None and residual.dim() != 2:
-        residual = residual.reshape(x.shape[0], n)
-    with torch.cuda.device(x.device):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-            y = _Linear.apply(x, weight, bias, residual, act)[0]
-        else:
-            y = product(x, weight, bias, act, residual)[0]
-    return y if len(shape) == 2 else y.view(*shape[:-1], n)
+        residual = None if residual is None else residual.reshape(x.shape[0], weight.shape[0])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        y = _Linear.apply(x, weight, bias, residual, act)[0]
+    else:
+        y = product(x, weight, bias, act, residual)[0]
+    return y if len(shape) == 2 else y.view(*shape[:-1], weight.shape[0])
 
 
 class Linear(nn.Module):

@@ -128,6 +128,33 @@ class LinearArgs(ctypes.Structure):
     ]
 
 
+class LinearBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("m", i64),
+        ("n", i64),
+        ("k", i64),
+        ("gy", vp),
+        ("ld_gy", i64),
+        ("z", vp),
+        ("ld_z", i64),
+        ("gz", vp),
+        ("ld_gz", i64),
+        ("x", vp),
+        ("ld_x", i64),
+        ("w", vp),
+        ("ld_w", i64),
+        ("dx", vp),
+        ("dw", vp),
+        ("db", vp),
+        ("x_mn_major", i32),
+        ("w_mn_major", i32),
+        ("act", i32),
+        ("dtype", i32),
+        ("workspace", vp),
+        ("workspace_bytes", i64),
+    ]
+
+
 class ActGradArgs(ctypes.Structure):
     _fields_ = [
         ("rows", i64),
@@ -246,6 +273,8 @@ _SIGNATURES = {
     "cg_gemm_tf32_noalloc": (ctypes.c_int, [ctypes.POINTER(GemmArgs), vp]),
     "cg_linear_half": (_I, [ctypes.POINTER(LinearArgs), vp]),
     "cg_linear_half_workspace_bytes": (i64, [ctypes.POINTER(LinearArgs)]),
+    "cg_linear_half_backward": (_I, [ctypes.POINTER(LinearBackwardArgs), vp]),
+    "cg_linear_half_backward_workspace_bytes": (i64, [ctypes.POINTER(LinearBackwardArgs)]),
     "cg_act_grad_half": (_I, [ctypes.POINTER(ActGradArgs), vp]),
     "cg_act_grad_half_scratch_bytes": (i64, [i64, i64]),
     "cg_act_grad2_half": (_I, [vp, vp, vp, vp, vp, vp, i64, i64, _I, _I, vp]),
@@ -318,6 +347,12 @@ def lib() -> ctypes.CDLL:
     return load_library()
 
 
+@functools.cache
+def entry(name: str):
+    """The entry point ``name`` of lib(), looked up once per process."""
+    return getattr(lib(), name)
+
+
 def check(status: int) -> None:
     if status != 0:
         message = load_library().cg_last_error().decode(errors="replace")
@@ -372,7 +407,7 @@ def time_entry_points(names, enable: bool = True) -> None:
 
 def invoke(name: str, *args, info=None) -> None:
     """Call a status-returning entry point (the last argument is the stream)."""
-    fn = getattr(lib(), name)
+    fn = entry(name)
     slot = TIMED.get(name)
     if slot is None:
         check(fn(*args))

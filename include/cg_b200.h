@@ -300,6 +300,35 @@ typedef struct cg_act_grad_args {
 
 int cg_act_grad_half(const cg_act_grad_args* args, void* stream);
 int64_t cg_act_grad_half_scratch_bytes(int64_t rows, int64_t cols);
+/* The whole first-order backward of cg_linear_half for y = f(x W^T + b) + r,
+ * x (m, k), W (n, k): gz = gy f'(z), dx = gz W, dW = gz^T x, db. dx, dw and db
+ * are contiguous; each may be NULL (not formed). With CG_ACT_NONE gz is gy
+ * itself (z and gz unused); else gz is a buffer of pitch ld_gz. What the
+ * products read (x, w and gz, or gy) follows cg_linear_half's alignment rules. */
+typedef struct cg_linear_backward_args {
+  int64_t m, n, k;
+  const void* gy;
+  int64_t ld_gy;
+  const void* z;
+  int64_t ld_z;
+  void* gz;
+  int64_t ld_gz;
+  const void* x;
+  int64_t ld_x;
+  const void* w;
+  int64_t ld_w;
+  void* dx;
+  void* dw;
+  void* db;
+  int32_t x_mn_major, w_mn_major;
+  int32_t act;
+  int32_t dtype;
+  void* workspace; /* 16-byte aligned; cg_linear_half_backward_workspace_bytes() bytes */
+  int64_t workspace_bytes;
+} cg_linear_backward_args;
+
+int cg_linear_half_backward(const cg_linear_backward_args* args, void* stream);
+int64_t cg_linear_half_backward_workspace_bytes(const cg_linear_backward_args* args);
 /* Second order: for cotangents h of gz and hb of db (either may be NULL),
  * dgy = (h + hb) f'(z) and dz = (h + hb) gy f''(z); contiguous (rows, cols). */
 int cg_act_grad2_half(const void* h, const void* hb, const void* gy, const void* z, void* dgy, void* dz, int64_t rows,
