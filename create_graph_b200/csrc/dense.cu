@@ -220,16 +220,19 @@ __device__ __forceinline__ void act_all(float (&v)[N], int kind) {
 
 struct EpiBase {
   using Args = EpiArgs;
-  using L = half::Launch<EpiArgs, 1>;
-  static constexpr int kGroups = 1;
-  const EpiArgs& a;
+  static constexpr int kGroups = 2;  // dx and dW of a backward share a launch
+  using L = half::Launch<EpiArgs, kGroups>;
+  const EpiArgs* p;
   unsigned char* staging;
   uint64_t* bar;
   int lane, m, n, split, row0;
-  __device__ EpiBase(const L& l, unsigned char* staging_, uint64_t* bar_, int lane_)
-      : a(l.g[0].epi), staging(staging_), bar(bar_), lane(lane_), m(l.g[0].m), n(l.g[0].n) {}
+  __device__ EpiBase(const L&, unsigned char* staging_, uint64_t* bar_, int lane_)
+      : staging(staging_), bar(bar_), lane(lane_) {}
   static __device__ int* error_word() { return &g_dense_error; }
-  __device__ void begin(const half::Group<EpiArgs>&, const half::Item& item, int row) {
+  __device__ void begin(const half::Group<EpiArgs>& g, const half::Item& item, int row) {
+    p = &g.epi;
+    m = g.m;
+    n = g.n;
     split = item.split;
     row0 = row;
   }
@@ -264,9 +267,9 @@ struct BlockEpi : EpiBase {
     if (outside(col0)) return;
     if (lane == 0) {
       tma_store_wait_read();
-      if (a.residual != nullptr && a.partial == nullptr) {
+      if (p->residual != nullptr && p->partial == nullptr) {
         mbar_arrive_expect_tx(bar, 4096);
-        half::tma_load_3d<1>(staging, &a.map_res, bar, col0, row0, 0);
+        half::tma_load_3d<1>(staging, &p->map_res, bar, col0, row0, 0);
       }
     }
     __syncwarp();
@@ -283,13 +286,13 @@ struct BlockEpi : EpiBase {
   // 32 pre-activations of this thread's row
   __device__ __forceinline__ void load(uint32_t acc, int col0, float (&v)[32]) const {
     tmem_load_32(acc, v);
-    if (a.bias == nullptr) return;
+    if (p->bias == nullptr) return;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int col = col0 + 8 * c;
       if (col < n) {
         float b[8];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + col)), b);
+        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p->bias) + col)), b);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[8 * c + e] += b[e];
       }
@@ -297,7 +300,7 @@ struct BlockEpi : EpiBase {
   }
   __device__ __forceinline__ bool store(uint32_t acc, int col0, int* error) {
     if (outside(col0)) return true;
-    if (a.partial != nullptr) {
+    if (p->partial != nullptr) {
 #pragma unroll 1
       for (int h = 0; h < 2 && col0 + 32 * h < n; ++h) {
         float v[32];
@@ -307,7 +310,7 @@ struct BlockEpi : EpiBase {
         for (int c = 0; c < 8; ++c)
           *group(c) = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
                                  __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
-        put(&a.map_partial, col0 + 32 * h, split);
+        put(&p->map_partial, col0 + 32 * h, split);
       }
       return true;
     }
@@ -316,8 +319,8 @@ struct BlockEpi : EpiBase {
     for (int h = 0; h < 2; ++h) {
       float v[32];
       load(acc + 32 * h, col0 + 32 * h, v);
-      act_all(v, a.act);
-      if (a.residual && h == 0) {
+      act_all(v, p->act);
+      if (p->residual && h == 0) {
         ok = half::wait(bar, loads & 1, error);
         ++loads;
       }
@@ -326,7 +329,7 @@ struct BlockEpi : EpiBase {
         float o[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
                       v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
         uint4* at = group(4 * h + c);
-        if (a.residual) {
+        if (p->residual) {
           float r[8];
           unpack8<T>(*at, r);
 #pragma unroll
@@ -335,8 +338,8 @@ struct BlockEpi : EpiBase {
         *at = pack8<T>(o);
       }
     }
-    put(&a.map_y, col0, 0);
-    if (a.z) {
+    put(&p->map_y, col0, 0);
+    if (p->z) {
       reuse();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -349,7 +352,7 @@ struct BlockEpi : EpiBase {
           *group(4 * h + c) = pack8<T>(o);
         }
       }
-      put(&a.map_z, col0, 0);
+      put(&p->map_z, col0, 0);
     }
     return ok;
   }
@@ -391,8 +394,8 @@ struct PlainEpi : EpiBase {
           const int64_t row = row0 + r;
           if (row >= m) break;
           const float x = stage[half::stage_idx(r, lane)];
-          if (a.partial) a.partial[((int64_t)split * m + row) * n + col] = x;
-          else finish1(a, x, row, col);
+          if (p->partial) p->partial[((int64_t)split * m + row) * n + col] = x;
+          else finish1(*p, x, row, col);
         }
       }
       __syncwarp();
@@ -453,7 +456,7 @@ template <class T, int V>
 __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
                                                        const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
                                                        int64_t ld_gz, int rows, int cols, int kind, int rows_per,
-                                                       float* __restrict__ partial) {
+                                                       float* __restrict__ partial, T* __restrict__ db) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.x * 32 + lane) * V;
   const int r0 = blockIdx.y * rows_per, r1 = min(rows, r0 + rows_per);
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
       for (int e = 0; e < V; ++e) sum[e] += g[e];
     }
   }
-  if (partial == nullptr) return;
+  if (partial == nullptr && db == nullptr) return;
   __shared__ float sums[8][32 * V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sums[warp][lane * V + e] = sum[e];
@@ -492,7 +495,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += sums[w][c];
-    partial[(int64_t)blockIdx.y * cols + at] = s;
+    if (db) db[at] = from_float<T>(s);  // the only chunk
+    else partial[(int64_t)blockIdx.y * cols + at] = s;
   }
 }
 
@@ -525,80 +529,85 @@ __global__ void act_grad2_kernel(const T* __restrict__ h, const T* __restrict__ 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Plan {
-  int cg, bn, splits, kt_per;
+  int cg, bn;
+  int splits[2], kt_per[2];
 };
 
-// Tile and k-split of a product.
-static Plan plan_of(const cg_linear_args& g) {
+// Tile of a launch and k-splits of its one or two products, by the time of the
+// slot (SM or SM pair) that gets most: a tile takes `fixed` (its epilogue's
+// tail and pipeline start) and `slice` per 64-wide k-slice, in nanoseconds
+// measured on full waves (PLANFIG).
+static Plan plan_of(const cg_linear_args* g, int count) {
   const int64_t sms = sm_count();
-  const int64_t kts = ceil_div<int64_t>(g.k, half::kBK);
   struct Shape {
     int cg, bn;
-    double clocks, fixed;
+    double slice, fixed;
   };
-  static const Shape shapes[] = {{2, 256, 560, 1500}, {2, 128, 320, 1300}, {1, 128, 330, 1200}, {1, 64, 230, 1000}};
-  Plan best = {1, 64, 1, (int)kts};
+  static const Shape shapes[] = {{2, 256, 390, 1300}, {2, 128, 290, 1300}, {1, 128, 330, 1200}, {1, 64, 230, 1000}};
+  const int kMost = 24;
+  int64_t kts[2] = {1, 1};
+  for (int i = 0; i < count; ++i) kts[i] = ceil_div<int64_t>(g[i].k, half::kBK);
+  Plan best = {};
   double least = 0.0;
   for (const Shape& s : shapes) {
-    const int64_t tiles = ceil_div<int64_t>(g.m, s.cg * half::kRows) * ceil_div<int64_t>(g.n, s.bn);
     const int64_t slots = sms / s.cg;
-    int64_t most = slots / tiles < kts / 4 ? slots / tiles : kts / 4;
-    for (int64_t splits = 1; splits <= (most < 1 ? 1 : most); ++splits) {
-      const int64_t per = ceil_div<int64_t>(kts, splits);
-      const int64_t used = ceil_div<int64_t>(kts, per);
-      if (used != splits) continue;
-      const int64_t waves = ceil_div<int64_t>(tiles * splits, slots);
-      double cost = (double)waves * ((double)per * s.clocks + s.fixed);
-      if (splits > 1) cost += 4000.0 + (double)splits * g.m * g.n * 8.0 / 2500.0;
-      if (least == 0.0 || cost < least) {
-        least = cost;
-        best = {s.cg, s.bn, (int)splits, (int)per};
-      }
+    int64_t tiles[2] = {0, 0};
+    int most[2] = {1, 1};
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = ceil_div<int64_t>(g[i].m, s.cg * half::kRows) * ceil_div<int64_t>(g[i].n, s.bn);
+      // more parts than fill the slots twice only add to the join
+      int64_t n = 2 * slots / tiles[i];
+      if (n > kts[i] / 4) n = kts[i] / 4;
+      most[i] = n < 1 ? 1 : n > kMost ? kMost : (int)n;
     }
+    for (int s0 = 1; s0 <= most[0]; ++s0)
+      for (int s1 = 1; s1 <= most[1]; ++s1) {
+        const int split[2] = {s0, s1};
+        int64_t per[2] = {1, 1}, items[2] = {0, 0};
+        double time[2] = {0.0, 0.0}, join = 0.0;
+        bool same = true;
+        for (int i = 0; i < count; ++i) {
+          per[i] = ceil_div<int64_t>(kts[i], split[i]);
+          same = same && ceil_div<int64_t>(kts[i], per[i]) == split[i];
+          items[i] = tiles[i] * split[i];
+          time[i] = (double)per[i] * s.slice + s.fixed;
+          // a launch, and the partial tiles written and read at about 4 TB/s
+          if (split[i] > 1) join += 2500.0 + (double)split[i] * g[i].m * g[i].n * 8.0 / 4000.0;
+        }
+        if (!same) continue;
+        // slot k gets items k, k + slots, ..: at most three different loads
+        const int64_t total = items[0] + items[1], edges[3] = {0, items[0] % slots, total % slots};
+        double cost = 0.0;
+        for (int64_t k : edges) {
+          const int64_t first = items[0] / slots + (k < items[0] % slots), all = total / slots + (k < total % slots);
+          const double load = (double)first * time[0] + (double)(all - first) * time[1];
+          if (load > cost) cost = load;
+        }
+        cost += join;
+        if (least == 0.0 || cost < least) {
+          least = cost;
+          best.cg = s.cg;
+          best.bn = s.bn;
+          for (int i = 0; i < 2; ++i) {
+            best.splits[i] = split[i];
+            best.kt_per[i] = (int)per[i];
+          }
+        }
+      }
   }
   return best;
 }
 
-static int64_t workspace_bytes(const cg_linear_args& g) {
-  const Plan p = plan_of(g);
-  return p.splits > 1 ? (int64_t)p.splits * g.m * g.n * (int64_t)sizeof(float) : 0;
+static int64_t partial_bytes(const cg_linear_args& g, int splits) {
+  return splits > 1 ? ceil_div<int64_t>((int64_t)splits * g.m * g.n * (int64_t)sizeof(float), 256) * 256 : 0;
 }
 
-template <int CG, int BN, class E>
-static int launch(const cg_linear_args& g, const Plan& p, const EpiArgs& ea, bool bf16, cudaStream_t s) {
-  half::LaunchOf<E> L;
-  memset(&L, 0, sizeof(L));
-  L.groups = 1;
-  L.bf16 = bf16;
-  auto& G = L.g[0];
-  int rc;
-  if ((rc = half::make_half_map(&G.map_a, g.a, bf16, g.a_mn_major ? g.k : g.m, g.a_mn_major ? g.m : g.k, g.lda, 1,
-                                g.lda * (g.a_mn_major ? g.k : g.m), g.a_mn_major != 0, half::kRows)))
-    return rc;
-  if ((rc = half::make_half_map(&G.map_b, g.b, bf16, g.b_mn_major ? g.k : g.n, g.b_mn_major ? g.n : g.k, g.ldb, 1,
-                                g.ldb * (g.b_mn_major ? g.k : g.n), g.b_mn_major != 0, BN / CG)))
-    return rc;
-  G.m = (int)g.m;
-  G.n = (int)g.n;
-  G.k = (int)g.k;
-  G.batch = 1;
-  G.a_mn = g.a_mn_major;
-  G.b_mn = g.b_mn_major;
-  G.splits = p.splits;
-  G.kt_per = p.kt_per;
-  G.epi = ea;
-  const int64_t items = half::plan_group<CG, BN>(G);
-  CG_REQUIRE(items < (1ll << 31), "linear_half: too many tiles");
-  L.items = (int)items;
-  return half::launch_half_gemm<CG, BN, 1, E>(L, s);
-}
-
-template <class E>
-static int launch_plan(const cg_linear_args& g, const Plan& p, const EpiArgs& ea, bool bf16, cudaStream_t s) {
-  if (p.cg == 2 && p.bn == 256) return launch<2, 256, E>(g, p, ea, bf16, s);
-  if (p.cg == 2) return launch<2, 128, E>(g, p, ea, bf16, s);
-  if (p.bn == 128) return launch<1, 128, E>(g, p, ea, bf16, s);
-  return launch<1, 64, E>(g, p, ea, bf16, s);
+// Partial tiles of a launch's products, one after the other.
+static int64_t workspace_bytes(const cg_linear_args* g, int count) {
+  const Plan p = plan_of(g, count);
+  int64_t n = 0;
+  for (int i = 0; i < count; ++i) n += partial_bytes(g[i], p.splits[i]);
+  return n;
 }
 
 // 16-byte groups of eight columns everywhere.
@@ -608,66 +617,114 @@ static bool aligned_problem(const cg_linear_args& g) {
          (g.z == nullptr || (aligned16(g.z) && g.ld_z % 8 == 0));
 }
 
+template <int CG, int BN, class E>
+static int launch(const cg_linear_args* g, int count, const Plan& p, const EpiArgs* ea, bool bf16, cudaStream_t s) {
+  half::LaunchOf<E> L;
+  memset(&L, 0, sizeof(L));
+  L.groups = count;
+  L.bf16 = bf16;
+  int64_t items = 0;
+  for (int i = 0; i < count; ++i) {
+    const cg_linear_args& q = g[i];
+    auto& G = L.g[i];
+    int rc;
+    if ((rc = half::make_half_map(&G.map_a, q.a, bf16, q.a_mn_major ? q.k : q.m, q.a_mn_major ? q.m : q.k, q.lda, 1,
+                                  q.lda * (q.a_mn_major ? q.k : q.m), q.a_mn_major != 0, half::kRows)))
+      return rc;
+    if ((rc = half::make_half_map(&G.map_b, q.b, bf16, q.b_mn_major ? q.k : q.n, q.b_mn_major ? q.n : q.k, q.ldb, 1,
+                                  q.ldb * (q.b_mn_major ? q.k : q.n), q.b_mn_major != 0, BN / CG)))
+      return rc;
+    G.m = (int)q.m;
+    G.n = (int)q.n;
+    G.k = (int)q.k;
+    G.batch = 1;
+    G.a_mn = q.a_mn_major;
+    G.b_mn = q.b_mn_major;
+    G.splits = p.splits[i];
+    G.kt_per = p.kt_per[i];
+    G.epi = ea[i];
+    G.first_item = (int)items;
+    items += half::plan_group<CG, BN>(G);
+    CG_REQUIRE(items < (1ll << 31), "linear_half: too many tiles");
+  }
+  L.items = (int)items;
+  return half::launch_half_gemm<CG, BN, 1, E>(L, s);
+}
+
+template <class E>
+static int launch_plan(const cg_linear_args* g, int count, const Plan& p, const EpiArgs* ea, bool bf16,
+                       cudaStream_t s) {
+  if (p.cg == 2 && p.bn == 256) return launch<2, 256, E>(g, count, p, ea, bf16, s);
+  if (p.cg == 2) return launch<2, 128, E>(g, count, p, ea, bf16, s);
+  if (p.bn == 128) return launch<1, 128, E>(g, count, p, ea, bf16, s);
+  return launch<1, 64, E>(g, count, p, ea, bf16, s);
+}
+
+// One or two products (all checked) in one launch, and the joins of those that
+// split k.
 template <class T>
-static int run_typed(const cg_linear_args& g, bool bf16, cudaStream_t s) {
+static int run_typed(const cg_linear_args* g, int count, void* workspace, int64_t bytes, bool bf16, cudaStream_t s) {
   int rc;
   if ((rc = half::bind_context())) return rc;
-  const Plan p = plan_of(g);
-  EpiArgs ea;
-  memset(&ea, 0, sizeof(ea));
-  ea.y = g.y;
-  ea.ld_y = g.ld_y;
-  ea.bias = g.bias;
-  ea.residual = g.residual;
-  ea.ld_res = g.ld_residual;
-  ea.z = g.z;
-  ea.ld_z = g.ld_z;
-  ea.act = g.act;
-  if (p.splits > 1) {
-    CG_REQUIRE(g.workspace != nullptr && aligned16(g.workspace) && g.workspace_bytes >= workspace_bytes(g),
-               "linear_half: this shape splits K %d ways and needs %lld workspace bytes on a 16-byte boundary "
-               "(cg_linear_half_workspace_bytes)",
-               p.splits, (long long)workspace_bytes(g));
-    ea.partial = g.workspace;
+  const Plan p = plan_of(g, count);
+  EpiArgs ea[2];
+  memset(ea, 0, sizeof(ea));
+  bool vec = true;
+  int64_t used = 0;
+  for (int i = 0; i < count; ++i) {
+    const cg_linear_args& q = g[i];
+    ea[i].y = q.y;
+    ea[i].ld_y = q.ld_y;
+    ea[i].bias = q.bias;
+    ea[i].residual = q.residual;
+    ea[i].ld_res = q.ld_residual;
+    ea[i].z = q.z;
+    ea[i].ld_z = q.ld_z;
+    ea[i].act = q.act;
+    vec = vec && aligned_problem(q);
+    if (p.splits[i] > 1) ea[i].partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + used);
+    used += partial_bytes(q, p.splits[i]);
   }
-  const bool vec = aligned_problem(g);
+  CG_REQUIRE(used == 0 || (workspace != nullptr && aligned16(workspace) && bytes >= used),
+             "linear_half: this shape splits K and needs %lld workspace bytes on a 16-byte boundary "
+             "(cg_linear_half_workspace_bytes)",
+             (long long)used);
   if (vec) {
     const auto type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (ea.partial) {
-      if ((rc = half::make_block_map(&ea.map_partial, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ea.partial, g.m, g.n, g.n,
-                                     p.splits, g.m * g.n)))
-        return rc;
-    } else {
+    for (int i = 0; i < count; ++i) {
+      const cg_linear_args& q = g[i];
       auto block_map = [&](CUtensorMap* map, const void* ptr, int64_t ld) {
-        return ptr ? half::make_block_map(map, type, 2, ptr, g.m, g.n, ld, 1, g.m * ld) : kOk;
+        return ptr ? half::make_block_map(map, type, 2, ptr, q.m, q.n, ld, 1, q.m * ld) : kOk;
       };
-      if ((rc = block_map(&ea.map_y, g.y, g.ld_y)) || (rc = block_map(&ea.map_z, g.z, g.ld_z)) ||
-          (rc = block_map(&ea.map_res, g.residual, g.ld_residual)))
-        return rc;
+      if (ea[i].partial)
+        rc = half::make_block_map(&ea[i].map_partial, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ea[i].partial, q.m, q.n,
+                                  q.n, p.splits[i], q.m * q.n);
+      else if ((rc = block_map(&ea[i].map_y, q.y, q.ld_y)) == kOk && (rc = block_map(&ea[i].map_z, q.z, q.ld_z)) == kOk)
+        rc = block_map(&ea[i].map_res, q.residual, q.ld_residual);
+      if (rc) return rc;
     }
-    rc = launch_plan<BlockEpi<T>>(g, p, ea, bf16, s);
+    rc = launch_plan<BlockEpi<T>>(g, count, p, ea, bf16, s);
   } else {
-    rc = launch_plan<PlainEpi<T>>(g, p, ea, bf16, s);
+    rc = launch_plan<PlainEpi<T>>(g, count, p, ea, bf16, s);
   }
-  if (rc || p.splits == 1) return rc;
-  const int64_t blocks = ceil_div<int64_t>(ceil_div<int64_t>(g.m * g.n, vec ? 8 : 1), 256);
-  const int64_t most = (int64_t)sm_count() * 8;
-  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  if (vec) join_splits_kernel<T, true><<<grid, 256, 0, s>>>(ea, p.splits, (int)g.m, (int)g.n);
-  else join_splits_kernel<T, false><<<grid, 256, 0, s>>>(ea, p.splits, (int)g.m, (int)g.n);
-  CG_LAUNCHED("linear_half split join");
+  if (rc) return rc;
+  for (int i = 0; i < count; ++i) {
+    if (p.splits[i] == 1) continue;
+    const int64_t blocks = ceil_div<int64_t>(ceil_div<int64_t>(g[i].m * g[i].n, vec ? 8 : 1), 256);
+    const int64_t most = (int64_t)sm_count() * 8;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    if (vec) join_splits_kernel<T, true><<<grid, 256, 0, s>>>(ea[i], p.splits[i], (int)g[i].m, (int)g[i].n);
+    else join_splits_kernel<T, false><<<grid, 256, 0, s>>>(ea[i], p.splits[i], (int)g[i].m, (int)g[i].n);
+    CG_LAUNCHED("linear_half split join");
+  }
   return kOk;
 }
 
-static int run(const cg_linear_args* args, void* stream) {
-  CG_REQUIRE(args != nullptr, "linear_half: args is NULL");
-  const cg_linear_args& g = *args;
+static int checked(const cg_linear_args& g) {
   CG_REQUIRE(g.dtype == CG_F16 || g.dtype == CG_BF16, "linear_half: dtype %d is neither CG_F16 nor CG_BF16", g.dtype);
   CG_REQUIRE(g.act == CG_ACT_NONE || g.act == CG_ACT_SILU || g.act == CG_ACT_RELU || g.act == CG_ACT_GELU,
              "linear_half: bad act %d", g.act);
-  CG_REQUIRE(g.m >= 0 && g.n >= 0 && g.k >= 0, "linear_half: negative size");
-  if (g.m == 0 || g.n == 0) return kOk;
-  CG_REQUIRE(g.k >= 1, "linear_half: k must be >= 1");
+  CG_REQUIRE(g.m >= 1 && g.n >= 1 && g.k >= 1, "linear_half: sizes must be at least 1");
   const int64_t most = (1ll << 31) - 512;  // tile coordinates are 32-bit
   CG_REQUIRE(g.m < most && g.n < most && g.k < most, "linear_half: size too large");
   CG_REQUIRE(g.a && g.b && g.y, "linear_half: a, b and y must be non-null");
@@ -676,8 +733,20 @@ static int run(const cg_linear_args* args, void* stream) {
   CG_REQUIRE(g.lda >= (g.a_mn_major ? g.m : g.k) && g.ldb >= (g.b_mn_major ? g.n : g.k) && g.ld_y >= g.n &&
                  (g.residual == nullptr || g.ld_residual >= g.n) && (g.z == nullptr || g.ld_z >= g.n),
              "linear_half: row pitch smaller than the row");
-  if (g.dtype == CG_F16) return run_typed<__half>(g, false, as_stream(stream));
-  return run_typed<__nv_bfloat16>(g, true, as_stream(stream));
+  return kOk;
+}
+
+static int run_products(const cg_linear_args* g, int count, void* workspace, int64_t bytes, void* stream) {
+  for (int i = 0; i < count; ++i)
+    if (int rc = checked(g[i])) return rc;
+  if (g->dtype == CG_F16) return run_typed<__half>(g, count, workspace, bytes, false, as_stream(stream));
+  return run_typed<__nv_bfloat16>(g, count, workspace, bytes, true, as_stream(stream));
+}
+
+static int run(const cg_linear_args* args, void* stream) {
+  CG_REQUIRE(args != nullptr, "linear_half: args is NULL");
+  if (args->m == 0 || args->n == 0) return kOk;
+  return run_products(args, 1, args->workspace, args->workspace_bytes, stream);
 }
 
 // Row chunks of act_grad: enough blocks to fill the SMs several times, each of
@@ -698,15 +767,17 @@ static int act_grad_typed(const cg_act_grad_args& g, cudaStream_t s) {
   const int per = chunk_rows(g.rows, g.cols, vec ? 8 : 1);
   const int chunks = (int)ceil_div<int64_t>(g.rows, per);
   const dim3 grid((unsigned)ceil_div<int64_t>(g.cols, vec ? 256 : 32), (unsigned)chunks);
-  float* partial = g.db ? g.scratch : nullptr;
+  const bool direct = chunks == 1;
+  float* partial = g.db && !direct ? g.scratch : nullptr;
+  T* db = g.db && direct ? (T*)g.db : nullptr;
   if (vec)
     act_grad_kernel<T, 8><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
-                                               (int)g.rows, (int)g.cols, g.act, per, partial);
+                                               (int)g.rows, (int)g.cols, g.act, per, partial, db);
   else
     act_grad_kernel<T, 1><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
-                                               (int)g.rows, (int)g.cols, g.act, per, partial);
+                                               (int)g.rows, (int)g.cols, g.act, per, partial, db);
   CG_LAUNCHED("act_grad_half");
-  if (g.db) {
+  if (partial) {
     join_columns_kernel<T><<<(unsigned)ceil_div<int64_t>(g.cols, 128), 128, 0, s>>>(partial, chunks, (int)g.cols,
                                                                                     (T*)g.db);
     CG_LAUNCHED("act_grad_half column join");
@@ -776,13 +847,21 @@ static cg_linear_args dw_product(const cg_linear_backward_args& g) {
   return p;
 }
 
-// One region serves the column sums and then each product in turn.
+static int products(const cg_linear_backward_args& g, cg_linear_args* p) {
+  int n = 0;
+  if (g.dx) p[n++] = dx_product(g);
+  if (g.dw) p[n++] = dw_product(g);
+  return n;
+}
+
+// One region serves the column sums and then the products.
 static int64_t backward_workspace(const cg_linear_backward_args& g) {
   if (g.m <= 0 || g.n <= 0 || g.k <= 0) return 0;
   int64_t most = g.db ? act_grad_scratch(g.m, g.n) : 0;
-  const int64_t x = g.dx ? workspace_bytes(dx_product(g)) : 0, w = g.dw ? workspace_bytes(dw_product(g)) : 0;
-  if (x > most) most = x;
-  return w > most ? w : most;
+  cg_linear_args p[2];
+  const int count = products(g, p);
+  const int64_t n = count ? workspace_bytes(p, count) : 0;
+  return n > most ? n : most;
 }
 
 static int backward_run(const cg_linear_backward_args* args, void* stream) {
@@ -817,19 +896,9 @@ static int backward_run(const cg_linear_backward_args* args, void* stream) {
     a.scratch_bytes = g.workspace_bytes;
     if ((rc = act_grad_run(&a, stream))) return rc;
   }
-  if (g.dx) {
-    cg_linear_args p = dx_product(g);
-    p.workspace = static_cast<float*>(g.workspace);
-    p.workspace_bytes = g.workspace_bytes;
-    if ((rc = run(&p, stream))) return rc;
-  }
-  if (g.dw) {
-    cg_linear_args p = dw_product(g);
-    p.workspace = static_cast<float*>(g.workspace);
-    p.workspace_bytes = g.workspace_bytes;
-    if ((rc = run(&p, stream))) return rc;
-  }
-  return kOk;
+  cg_linear_args p[2];
+  const int count = products(g, p);
+  return count ? run_products(p, count, g.workspace, g.workspace_bytes, stream) : kOk;
 }
 
 template <class T>
@@ -858,7 +927,7 @@ int cg_linear_half(const cg_linear_args* args, void* stream) { return cg::dense:
 
 int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args) {
   if (args == nullptr || args->m <= 0 || args->n <= 0 || args->k <= 0) return 0;
-  return cg::dense::workspace_bytes(*args);
+  return cg::dense::workspace_bytes(args, 1);
 }
 
 int cg_linear_half_backward(const cg_linear_backward_args* args, void* stream) {

@@ -49,10 +49,21 @@ __host__ __device__ constexpr int threads_of(int epi) { return 32 * (2 + epi); }
 constexpr int kSumSlices = 2;  // k-slices summed in one accumulator when PLANES = 2
 constexpr int kBand = 8;       // m-tiles of one band of the tile walk (a power of two)
 
-// Bounded wait: 2^24 polls are about half a second at the least, hundreds of
-// times the longest tile.
+// Bounded wait of a whole warp, with one outcome for all its lanes: 2^24 polls
+// are about half a second at the least, hundreds of times the longest tile.
 __device__ inline bool wait(uint64_t* bar, uint32_t parity, int* error_word) {
-  return mbar_wait(bar, parity, error_word, 1u << 24);
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, error_word, 1u << 24));
+}
+
+// One lane of a converged warp, the same one every time.
+__device__ inline bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // ---- PTX of the cta_group::2 forms -----------------------------------------
@@ -308,7 +319,10 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
   uint64_t* epi_bars = acc_empty + 2;  // one per epilogue warp, for the blocks it loads
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_bars + WARPS);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the roles run as whole warps, one elected lane issuing, so that what a launch
+  // holds for each group stays in uniform registers (by a single lane, with the
+  // group's index not a constant, every product took 10 to 17% longer)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -333,43 +347,50 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
   int* const error_word = Epi::error_word();
   bool ok = true;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---------------- TMA producer (each CTA of a pair loads its own rows) ----------------
+    const bool issuer = elect_one();
     uint32_t it = 0;
     for (int w = first; w < L.items && ok; w += step) {
       const Item item = item_of<BM, BN>(L, w);
       const auto& g = L.g[item.g];
       const int m0 = item.m0 + (int)rank * kRows, n0 = item.n0 + (int)rank * T::kBRows;
-      for (int kt = item.kt0; kt < item.kt1; ++kt, ++it) {
+      const int kt1 = item.kt1, z0 = item.batch * PLANES;
+      const bool a_mn = g.a_mn != 0, b_mn = g.b_mn != 0;
+      const CUtensorMap *map_a = &g.map_a, *map_b = &g.map_b;
+      for (int kt = item.kt0; kt < kt1; ++kt, ++it) {
         const int s = it % STAGES;
         const uint32_t round = it / STAGES;
         if (it >= STAGES && !(ok = wait(&empty[s], (round - 1) & 1, error_word))) break;
-        if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * T::kStage);
         const int k0 = kt * kBK;
+        if (issuer) {
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * T::kStage);
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-          unsigned char* sa = tiles + s * T::kStage + p * (T::kA + T::kB);
-          unsigned char* sb = sa + T::kA;
-          const int z = item.batch * PLANES + p;
-          if (!g.a_mn) {
-            tma_load_3d<CG>(sa, &g.map_a, &full[s], k0, m0, z);
-          } else {
+          for (int p = 0; p < PLANES; ++p) {
+            unsigned char* sa = tiles + s * T::kStage + p * (T::kA + T::kB);
+            unsigned char* sb = sa + T::kA;
+            if (!a_mn) {
+              tma_load_3d<CG>(sa, map_a, &full[s], k0, m0, z0 + p);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kRows / 64; ++c)
-              tma_load_3d<CG>(sa + c * (kBK * 128), &g.map_a, &full[s], m0 + 64 * c, k0, z);
-          }
-          if (!g.b_mn) {
-            tma_load_3d<CG>(sb, &g.map_b, &full[s], k0, n0, z);
-          } else {
+              for (int c = 0; c < kRows / 64; ++c)
+                tma_load_3d<CG>(sa + c * (kBK * 128), map_a, &full[s], m0 + 64 * c, k0, z0 + p);
+            }
+            if (!b_mn) {
+              tma_load_3d<CG>(sb, map_b, &full[s], k0, n0, z0 + p);
+            } else {
 #pragma unroll
-            for (int c = 0; c < T::kBRows / 64; ++c)
-              tma_load_3d<CG>(sb + c * (kBK * 128), &g.map_b, &full[s], n0 + 64 * c, k0, z);
+              for (int c = 0; c < T::kBRows / 64; ++c)
+                tma_load_3d<CG>(sb + c * (kBK * 128), map_b, &full[s], n0 + 64 * c, k0, z0 + p);
+            }
           }
         }
+        __syncwarp();
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ---------------- UMMA issuer (the pair's leader) ----------------
+    const bool issuer = elect_one();
     uint32_t it = 0;
     int j = 0;
     for (int w = first; w < L.items && ok; w += step) {
@@ -400,20 +421,24 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
           auto db = [&](int p, int kk) {
             return smem_desc(sb + p * (T::kA + T::kB) + kk * b_step, b_lbo, 1024, kSwizzle128B);
           };
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            const bool on = kt > kt0 || kk > 0;
-            if (PLANES == 2) {  // the small cross terms first, then the hi product
-              umma_f16<CG>(acc, da(1, kk), db(0, kk), idesc, on);
-              umma_f16<CG>(acc, da(0, kk), db(1, kk), idesc, true);
-              umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, true);
-            } else {
-              umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, on);
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              const bool on = kt > kt0 || kk > 0;
+              if (PLANES == 2) {  // the small cross terms first, then the hi product
+                umma_f16<CG>(acc, da(1, kk), db(0, kk), idesc, on);
+                umma_f16<CG>(acc, da(0, kk), db(1, kk), idesc, true);
+                umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, true);
+              } else {
+                umma_f16<CG>(acc, da(0, kk), db(0, kk), idesc, on);
+              }
             }
+            umma_commit_cg<CG>(&empty[s]);
           }
-          umma_commit_cg<CG>(&empty[s]);
+          __syncwarp();
         }
-        umma_commit_cg<CG>(&acc_full[b]);
+        if (issuer) umma_commit_cg<CG>(&acc_full[b]);
+        __syncwarp();
       }
     }
   } else if (warp >= 2) {
