@@ -694,10 +694,10 @@ static int run_typed(const cg_linear_args* g, int count, void* workspace, int64_
     for (int i = 0; i < count; ++i) {
       const cg_linear_args& q = g[i];
       auto block_map = [&](CUtensorMap* map, const void* ptr, int64_t ld) {
-        return ptr ? half::make_block_map(map, type, 2, ptr, q.m, q.n, ld, 1, q.m * ld) : kOk;
+        return ptr ? half::make_block_map(map, type, 2, 128, ptr, q.m, q.n, ld, 1, q.m * ld) : kOk;
       };
       if (ea[i].partial)
-        rc = half::make_block_map(&ea[i].map_partial, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ea[i].partial, q.m, q.n,
+        rc = half::make_block_map(&ea[i].map_partial, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 128, ea[i].partial, q.m, q.n,
                                   q.n, p.splits[i], q.m * q.n);
       else if ((rc = block_map(&ea[i].map_y, q.y, q.ld_y)) == kOk && (rc = block_map(&ea[i].map_z, q.z, q.ld_z)) == kOk)
         rc = block_map(&ea[i].map_res, q.residual, q.ld_residual);

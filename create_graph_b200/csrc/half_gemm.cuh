@@ -220,6 +220,7 @@ struct Group {
   int tiles;                 // items per batch entry and split
   Divisor by_tiles, by_batch, by_band, by_last;  // by tiles, batch, a band's tiles, the last band's height
   int first_item;
+  int first_tile;            // PLANES = 2 with splits: place of its partial tiles and counters
   EpiArgs epi;
 };
 
@@ -229,12 +230,18 @@ struct Launch {
   Group<EpiArgs> g[GROUPS];
   int groups, items;
   int bf16;
+  // PLANES = 2 with splits: a tile's splits leave their sums here, and the one
+  // that counts last finishes it (counters are zero before the launch and after)
+  float4* partial;
+  unsigned* counters;
+  int most_splits;  // room per tile
 };
 template <class Epi>
 using LaunchOf = Launch<typename Epi::Args, Epi::kGroups>;
 
 struct Item {
   int g, batch, split, m0, n0, kt0, kt1;
+  int tile;  // place of the output tile among its group's
 };
 
 // Tiles of a symmetric result that reach its lower triangle: row block i (of
@@ -256,6 +263,7 @@ __device__ inline Item item_of(const Launch<EpiArgs, GROUPS>& L, int w) {
   int t = w - which * g.tiles;
   it.split = g.by_batch.div(which);
   it.batch = which - it.split * g.batch;
+  it.tile = it.batch * g.tiles + t;
   int mt, nt;
   if (g.lower) {
     mt = 0;
@@ -298,7 +306,8 @@ __device__ __forceinline__ void stage_read8(const float* stage, int r, int c, fl
 // launch), kWarps, kStagingBytes (shared memory per epilogue warp, a multiple of 1024),
 // Epi(launch, staging, barrier, lane), begin(group, item, row0), fetch(col0)
 // (starts what the next block reads), store(accumulator, col0) (a block of 32
-// rows: 64 columns from TMEM, or 32 summed ones with PLANES = 2), finish(), and
+// rows: 64 columns from TMEM, or 32 summed ones with PLANES = 2), skip() (after a
+// fetch, when another split finishes the tile), finish(), and
 // error_word() (the translation unit's).
 template <int CG, int BN, int PLANES, class Epi>
 __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
@@ -476,18 +485,57 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
           if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
           tc_fence_after();
 #pragma unroll
-          for (int q = 0; q < NB; ++q) {
-            float v[32];
-            tmem_load_32(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + STEP * q, v);
+          for (int q = 0; q < 2 * NB; ++q) {
+            float v[16];
+            tmem_load_16(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + STEP * (q / 2) + 16 * (q % 2), v);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) sum[q][x] += v[x];
+            for (int x = 0; x < 16; ++x) sum[q / 2][16 * (q % 2) + x] += v[x];
           }
           release(b);
         }
         if (!ok) break;
+        if (g.splits > 1) {
+          // leave the sums, thread by thread; the split that arrives last adds
+          // up all of them in split order (the same sum whoever is last)
+          const int slot = ((g.first_tile + item.tile) * CG + (int)rank) * WARPS + e;
+          float4* parts = L.partial + (int64_t)slot * L.most_splits * (NB * 8 * 32) + lane;
+          float4* mine = parts + item.split * (NB * 8 * 32);
+#pragma unroll
+          for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              __stcg(mine + (q * 8 + x) * 32,
+                     make_float4(sum[q][4 * x], sum[q][4 * x + 1], sum[q][4 * x + 2], sum[q][4 * x + 3]));
+          __threadfence();
+          __syncwarp();
+          unsigned before = 0;
+          if (lane == 0) before = atomicAdd(L.counters + slot, 1u);
+          before = __shfl_sync(0xffffffffu, before, 0);
+          if (before + 1 < (unsigned)g.splits) {
+            epi.skip();
+            continue;
+          }
+          __threadfence();
+          if (lane == 0) L.counters[slot] = 0;
+#pragma unroll
+          for (int q = 0; q < NB; ++q) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum[q][x] = 0.0f;
+            for (int z = 0; z < g.splits; ++z) {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const float4 f = __ldcg(parts + z * (NB * 8 * 32) + (q * 8 + x) * 32);
+                sum[q][4 * x] += f.x;
+                sum[q][4 * x + 1] += f.y;
+                sum[q][4 * x + 2] += f.z;
+                sum[q][4 * x + 3] += f.w;
+              }
+            }
+          }
+        }
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
-          epi.store(sum[q], item.n0 + c_first + STEP * q);
+          if (!(ok = ok && epi.store(sum[q], item.n0 + c_first + STEP * q, error_word))) break;
           if (q + 1 < NB) epi.fetch(item.n0 + c_first + STEP * (q + 1));
         }
       } else {
@@ -563,17 +611,18 @@ inline int make_half_map(CUtensorMap* map, const void* ptr, bool bf16, int64_t r
   return kOk;
 }
 
-// 3-D map of a result or residual: blocks of 128 bytes x 32 rows, swizzled.
-inline int make_block_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* ptr, int64_t rows,
-                          int64_t cols, int64_t ld, int64_t planes, int64_t stride) {
+// 3-D map of a result or residual: blocks of `width` (128 or 64) bytes x 32
+// rows, swizzled over that width.
+inline int make_block_map(CUtensorMap* map, CUtensorMapDataType type, int size, int width, const void* ptr,
+                          int64_t rows, int64_t cols, int64_t ld, int64_t planes, int64_t stride) {
   auto fn = encode_fn();
   CG_REQUIRE(fn != nullptr, "half gemm: cuTensorMapEncodeTiled is unavailable");
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
   cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(stride * size)};
-  cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+  cuuint32_t box[3] = {(cuuint32_t)(width / size), 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   CG_REQUIRE(r == CUDA_SUCCESS, "half gemm: cuTensorMapEncodeTiled failed (%d): rows %lld cols %lld ld %lld", (int)r,
              (long long)rows, (long long)cols, (long long)ld);
   return kOk;

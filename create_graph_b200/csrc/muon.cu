@@ -26,6 +26,8 @@
 namespace cg {
 namespace muon {
 
+using namespace cg::sm100;
+
 // device error word of this translation unit's kernels
 __device__ int g_muon_error = 0;
 
@@ -199,39 +201,11 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
 }
 
 // ---- epilogues -----------------------------------------------------------------
-// Eight hi + lo values of an operand, as loaded.
-struct Planes8 {
-  uint4 hi, lo;
-};
-__device__ __forceinline__ void join8(const Planes8& p, float (&v)[8]) {
-  const uint32_t h[4] = {p.hi.x, p.hi.y, p.hi.z, p.hi.w}, l[4] = {p.lo.x, p.lo.y, p.lo.z, p.lo.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&l[i]));
-    v[2 * i] = a.x + b.x;
-    v[2 * i + 1] = a.y + b.y;
-  }
-}
-__device__ __forceinline__ void split8(const float (&v)[8], Planes8& p) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 a = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    const float2 f = __half22float2(a);
-    const __half2 b = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
-    h[i] = *reinterpret_cast<const uint32_t*>(&a);
-    l[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  p.hi = make_uint4(h[0], h[1], h[2], h[3]);
-  p.lo = make_uint4(l[0], l[1], l[2], l[3]);
-}
-
 struct EpiArgs {
-  __half* out;        // planes of the result (split epilogue)
-  const __half* aux;  // planes added to it, or null
-  int64_t out_plane, aux_plane;
-  int out_pitch, aux_pitch;
+  // blocks of 32 x 32 values of the planes added to the result and of the
+  // result's planes (plane index 2 batch + {hi, lo})
+  CUtensorMap map_aux, map_out;
+  int has_aux;
   float alpha, beta;  // alpha aux + beta accumulator
   int lower;          // symmetric result
   // final epilogue: out <- keep out + rate value (keep = 0: out is not read)
@@ -239,18 +213,25 @@ struct EpiArgs {
   float keep, rate;
 };
 
+// A thread owns one row of the warp's 32 x 32 block. The planes that are added
+// come by TMA into the warp's staging block (hi, then lo), where each thread
+// reads and overwrites its own row, and the result leaves by TMA; with results
+// staged in fp32 and stored as 16-byte pieces by the threads the epilogue
+// outlasted the products (the 85M step's 1296 update tiles: 550 us).
 struct EpiBase {
   using Args = EpiArgs;
-  using L = half::Launch<EpiArgs, muon::kGroups>;
   static constexpr int kGroups = muon::kGroups;
+  using L = half::Launch<EpiArgs, kGroups>;
   static constexpr int kWarps = 8;
-  static constexpr int kStagingBytes = 32 * 32 * 4;
-  float* stage;
+  static constexpr int kStagingBytes = 2 * 32 * 64;
   const EpiArgs* a;
-  Planes8 aux[4];
+  unsigned char* staging;
+  uint64_t* bar;
+  uint32_t loads = 0;
   int lane, m, n, batch, row0;
-  __device__ EpiBase(const L&, unsigned char* staging, uint64_t*, int lane_)
-      : stage(reinterpret_cast<float*>(staging)), lane(lane_) {}
+  bool pending = false;  // a load has been started and not waited for
+  __device__ EpiBase(const L&, unsigned char* staging_, uint64_t* bar_, int lane_)
+      : staging(staging_), bar(bar_), lane(lane_) {}
   static __device__ int* error_word() { return &g_muon_error; }
   __device__ void begin(const half::Group<EpiArgs>& g, const half::Item& item, int row) {
     a = &g.epi;
@@ -259,90 +240,108 @@ struct EpiBase {
     batch = item.batch;
     row0 = row;
   }
-  // lane -> rows (lane >> 2) + 8 i, columns 8 (lane & 3) .. + 7 of the block;
-  // planes have pitches of whole groups of eight
-  __device__ void fetch(int col0) {
-    if (a->aux == nullptr) return;
-    const int col = col0 + (lane & 3) * 8;
-    const __half* base = a->aux + batch * 2 * a->aux_plane + col;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + (lane >> 2) + 8 * i;
-      if (row < m && col < n) {
-        const __half* at = base + (int64_t)row * a->aux_pitch;
-        aux[i].hi = *reinterpret_cast<const uint4*>(at);
-        aux[i].lo = *reinterpret_cast<const uint4*>(at + a->aux_plane);
-      } else {
-        aux[i].hi = aux[i].lo = make_uint4(0, 0, 0, 0);
+  // nothing to store: out of range, or above the diagonal, where the mirror
+  // block below it writes
+  __device__ __forceinline__ bool outside(int col0) const {
+    return row0 >= m || col0 >= n || (a->lower && row0 + 31 < col0);
+  }
+  __device__ __forceinline__ void fetch(int col0) {
+    if (outside(col0)) return;
+    fence_proxy_async_shared();  // what the threads wrote here before
+    __syncwarp();
+    if (lane == 0) {
+      half::tma_store_wait_read();
+      if (a->has_aux) {
+        mbar_arrive_expect_tx(bar, kStagingBytes);
+        half::tma_load_3d<1>(staging, &a->map_aux, bar, col0, row0, 2 * batch);
+        half::tma_load_3d<1>(staging + 2048, &a->map_aux, bar, col0, row0, 2 * batch + 1);
       }
     }
-  }
-  __device__ __forceinline__ void put_rows(const float (&v)[32]) {  // row `lane` of the block
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<float4*>(stage + half::stage_idx(lane, 4 * q)) =
-          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    pending = a->has_aux;
     __syncwarp();
   }
-  __device__ __forceinline__ void put_back8(int r, int c, const float (&v)[8]) {
-    *reinterpret_cast<float4*>(stage + half::stage_idx(r, c)) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(stage + half::stage_idx(r, c + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+  __device__ __forceinline__ bool arrived(int* error) {
+    if (!pending) return true;
+    pending = false;
+    const bool ok = half::wait(bar, loads & 1, error);
+    ++loads;
+    return ok;
   }
-  __device__ __forceinline__ void value8(const Planes8& p, float (&v)[8]) const {
-    if (a->aux) {
-      float x[8];
-      join8(p, x);
+  __device__ __forceinline__ void skip() { arrived(error_word()); }
+  // 16-byte group c (8 values) of row r of plane p
+  __device__ __forceinline__ uint4* group(int p, int r, int c) const {
+    return reinterpret_cast<uint4*>(staging + p * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  }
+  // v <- alpha aux + beta v
+  __device__ __forceinline__ bool values(float (&v)[32], int* error) {
+    const float alpha = a->alpha, beta = a->beta;
+    if (!a->has_aux) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = a->alpha * x[e] + a->beta * v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= a->beta;
+      for (int e = 0; e < 32; ++e) v[e] *= beta;
+      return true;
     }
+    const bool ok = arrived(error);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint4 h = *group(0, lane, c), l = *group(1, lane, c);
+      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw[i]));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lw[i]));
+        v[8 * c + 2 * i] = alpha * (x.x + y.x) + beta * v[8 * c + 2 * i];
+        v[8 * c + 2 * i + 1] = alpha * (x.y + y.y) + beta * v[8 * c + 2 * i + 1];
+      }
+    }
+    return ok;
   }
-  __device__ void finish() {}
 };
 
 // The result as planes, for the next product.
 struct SplitEpi : EpiBase {
   using EpiBase::EpiBase;
-  __device__ __forceinline__ void put8(const float (&v)[8], int64_t row, int col) const {
-    __half* at = a->out + batch * 2 * a->out_plane + row * a->out_pitch + col;
-    Planes8 p;
-    split8(v, p);
-    *reinterpret_cast<uint4*>(at) = p.hi;
-    *reinterpret_cast<uint4*>(at + a->out_plane) = p.lo;
-  }
-  __device__ void store(const float (&acc)[32], int col0) {
-    if (a->lower && row0 + 31 < col0) return;  // above the diagonal: its mirror block writes it
-    put_rows(acc);
-    const bool diagonal = a->lower && row0 == col0, mirror = a->lower && !diagonal;
-    const int c = (lane & 3) * 8, col = col0 + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (lane >> 2) + 8 * i, row = row0 + r;
-      float v[8];
-      if (diagonal) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = stage[half::stage_idx(max(r, c + e), min(r, c + e))];
-      } else {
-        half::stage_read8(stage, r, c, v);
-      }
-      value8(aux[i], v);
-      if (mirror) put_back8(r, c, v);
-      if (row < m && col < n) put8(v, row, col);
+  __device__ __forceinline__ void put(int col, int row) {
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+      half::tma_store_3d(&a->map_out, staging, col, row, 2 * batch);
+      half::tma_store_3d(&a->map_out, staging + 2048, col, row, 2 * batch + 1);
     }
-    if (mirror) {
+  }
+  __device__ __forceinline__ bool store(float (&v)[32], int col0, int* error) {
+    if (outside(col0)) return true;
+    const bool ok = values(v, error);
+    // hi = fp16(v), lo = fp16(v - hi)
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      const float2 f = __half22float2(h);
+      const __half2 l = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+      lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      *group(0, lane, c) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+      *group(1, lane, c) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+    }
+    put(col0, row0);
+    if (a->lower && row0 != col0) {  // the mirror block: value c of this row is value `lane` of its row c
+      if (lane == 0) half::tma_store_wait_read();
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = (lane >> 2) + 8 * i;  // row of the mirrored block
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = stage[half::stage_idx(c + e, t)];
-        if (col0 + t < n && row0 + c < m) put8(v, col0 + t, row0 + c);
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t h = hi[i / 2], l = lo[i / 2];
+        reinterpret_cast<uint16_t*>(group(0, i, lane >> 3))[lane & 7] = (uint16_t)(i % 2 ? h >> 16 : h);
+        reinterpret_cast<uint16_t*>(group(1, i, lane >> 3))[lane & 7] = (uint16_t)(i % 2 ? l >> 16 : l);
       }
+      put(row0, col0);
     }
-    __syncwarp();
+    return ok;
+  }
+  __device__ void finish() {
+    if (lane == 0) half::tma_store_wait();
   }
 };
 
@@ -386,36 +385,43 @@ struct FinalEpi : EpiBase {
     for (int e = 0; e < 8; ++e) put_value(h + e, a->rate * v[e]);
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
   }
-  __device__ void store(const float (&acc)[32], int col0) {
-    put_rows(acc);
-    const int c = (lane & 3) * 8, col = col0 + c;
+  // rows of the caller's matrices: fp32 blocks through shared memory
+  __device__ __forceinline__ bool store(float (&v)[32], int col0, int* error) {
+    if (outside(col0)) return true;
+    const bool ok = values(v, error);
+    float* stage = reinterpret_cast<float*>(staging);
+    __syncwarp();  // every row of the planes has been read
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (lane >> 2) + 8 * i, row = row0 + r;
-      float v[8];
-      half::stage_read8(stage, r, c, v);
-      value8(aux[i], v);
-      if (vec) {
-        if (row < m && col < n) put8(v, out + row * ld + col);
-      } else {
-        put_back8(r, c, v);
-      }
-    }
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4*>(stage + half::stage_idx(lane, 4 * q)) =
+          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     __syncwarp();
-    const int cs = col0 + lane;
-    if (!vec && cs < n) {  // odd pitches: one column per lane
+    if (vec) {
+      const int c = (lane & 3) * 8, col = col0 + c;
+      if (col < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (lane >> 2) + 8 * i, row = row0 + r;
+          float x[8];
+          half::stage_read8(stage, r, c, x);
+          if (row < m) put8(x, out + row * ld + col);
+        }
+      }
+    } else if (col0 + lane < n) {  // odd pitches: one column per lane
 #pragma unroll 8
       for (int r = 0; r < 32; ++r) {
         const int row = row0 + r;
         if (row >= m) break;
-        float v = a->rate * stage[half::stage_idx(r, lane)];
-        T* p = out + row * ld + cs;
-        if (sizeof(T) == 4 && a->keep != 0.0f) v += a->keep * *reinterpret_cast<const float*>(p);
-        put_value(p, v);
+        float x = a->rate * stage[half::stage_idx(r, lane)];
+        T* p = out + row * ld + col0 + lane;
+        if (sizeof(T) == 4 && a->keep != 0.0f) x += a->keep * *reinterpret_cast<const float*>(p);
+        put_value(p, x);
       }
     }
     __syncwarp();
+    return ok;
   }
+  __device__ void finish() {}
 };
 
 // ---- host side -------------------------------------------------------------------
@@ -455,8 +461,76 @@ static int gather_shapes(const cg_ns_args& g, int from, Shape* shapes, int* to) 
 
 static int64_t chunks_of(int64_t rows, int64_t cols) { return ceil_div<int64_t>(rows * cols, kChunk); }
 
+enum Step { kGram, kPoly, kUpdate };
+
+// Tile of a launch and the k-splits of its products.
+struct Plan {
+  int cg, bn, splits;
+  int64_t slots, floats;  // with splits: counters and partial sums
+};
+
+// By the time of a slot (SM or SM pair): a tile takes `fixed` and `slice` per
+// 64-wide k-slice (three products), in nanoseconds measured on full waves
+// (NSFIG). Larger tiles feed the tensor cores best, smaller ones and splits of
+// k fill the SMs when there are few.
+static Plan plan_of(const Shape* shapes, int n, Step step) {
+  struct Tile {
+    int cg, bn;
+    double slice, fixed;
+  };
+  static const Tile choices[] = {{2, 256, 1000, 3000}, {2, 128, 600, 2500}, {1, 128, 600, 2500}, {1, 64, 400, 2000}};
+  const int sms = sm_count();
+  Plan best = {2, 256, 1, 0, 0};
+  double least = 0.0;
+  for (const Tile& t : choices) {
+    const int bm = t.cg * half::kRows, slots = sms / t.cg;
+    for (int splits = 1; splits <= 8; ++splits) {
+      double items = 0.0, time = 0.0;
+      int64_t tiles = 0;
+      bool any = splits == 1;
+      for (int i = 0; i < n; ++i) {
+        const Shape& h = shapes[i];
+        const int64_t m = step == kUpdate ? h.rows : h.s, w = step == kUpdate ? h.cols : h.s;
+        const int64_t k = step == kGram ? (h.rows < h.cols ? h.cols : h.rows) : h.s;
+        const int64_t m_tiles = ceil_div<int64_t>(m, bm), n_tiles = ceil_div<int64_t>(w, t.bn);
+        int64_t count = m_tiles * n_tiles;
+        if (step != kUpdate) {
+          count = 0;
+          for (int64_t r = 0; r < m_tiles; ++r) count += half::lower_tiles_of_row((int)r, bm, t.bn, (int)n_tiles);
+        }
+        count *= h.count;
+        const int64_t kts = ceil_div<int64_t>(k, half::kBK), per = ceil_div<int64_t>(kts, splits);
+        const int64_t parts = ceil_div<int64_t>(kts, per);
+        any = any || (parts == splits && per >= 2);
+        tiles += count;
+        items += (double)count * parts;
+        time += (double)count * parts * (per * t.slice + t.fixed + (parts > 1 ? 1000.0 + 300.0 * parts : 0.0));
+      }
+      if (!any) continue;
+      const double cost = ceil(items / slots) * time / items;
+      if (least == 0.0 || cost < least) {
+        least = cost;
+        best.cg = t.cg;
+        best.bn = t.bn;
+        best.splits = splits;
+        best.slots = splits > 1 ? tiles * t.cg * EpiBase::kWarps : 0;
+        best.floats = splits > 1 ? tiles * splits * bm * t.bn : 0;
+      }
+    }
+  }
+  return best;
+}
+
+struct Buffers {
+  double* squares;
+  OutRef* table;
+  float4* partial;
+  unsigned* counters;
+  int64_t counter_bytes;
+};
+
 // Lay the set's buffers out from `base`; returns the bytes they take.
-static int64_t layout(Shape* shapes, int n, char* base, double** partial, OutRef** table) {
+static int64_t layout(Shape* shapes, int n, char* base, Buffers* b) {
   int64_t at = 0, matrices = 0, chunks = 0;
   auto take = [&](int64_t bytes) {
     char* p = base == nullptr ? nullptr : base + at;
@@ -477,8 +551,18 @@ static int64_t layout(Shape* shapes, int n, char* base, double** partial, OutRef
     h.gram = reinterpret_cast<__half*>(take(s));
     h.poly = reinterpret_cast<__half*>(take(s));
   }
-  *partial = reinterpret_cast<double*>(take(chunks * (int64_t)sizeof(double)));
-  *table = reinterpret_cast<OutRef*>(take(matrices * (int64_t)sizeof(OutRef)));
+  b->squares = reinterpret_cast<double*>(take(chunks * (int64_t)sizeof(double)));
+  b->table = reinterpret_cast<OutRef*>(take(matrices * (int64_t)sizeof(OutRef)));
+  int64_t floats = 0, counters = 0;
+  for (int step = 0; step < 3; ++step) {
+    const Plan p = plan_of(shapes, n, (Step)step);
+    if (p.slots == 0) continue;
+    if (p.floats > floats) floats = p.floats;
+    if (p.slots > counters) counters = p.slots;
+  }
+  b->partial = reinterpret_cast<float4*>(take(floats * (int64_t)sizeof(float)));
+  b->counters = reinterpret_cast<unsigned*>(take(counters * (int64_t)sizeof(unsigned)));
+  b->counter_bytes = counters * (int64_t)sizeof(unsigned);
   return at;
 }
 
@@ -487,16 +571,15 @@ static int64_t workspace_bytes(const cg_ns_args& g) {
   Shape shapes[kGroups];
   for (int from = 0, to; from < g.n; from = to) {
     const int n = gather_shapes(g, from, shapes, &to);
-    double* partial;
-    OutRef* table;
-    const int64_t bytes = layout(shapes, n, nullptr, &partial, &table);
+    Buffers b;
+    const int64_t bytes = layout(shapes, n, nullptr, &b);
     if (bytes > most) most = bytes;
   }
   return most;
 }
 
 template <class T, bool MOMENTUM>
-static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, int n, double* partial, OutRef* table,
+static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, int n, const Buffers& b,
                    cudaStream_t s) {
   // both passes need every run's place: the first walks all launches, then the second
   for (int pass = 0; pass < 2; ++pass) {
@@ -507,12 +590,12 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
     p.eps = g.eps;
     p.mu = g.momentum;
     p.nesterov = g.nesterov;
-    p.table = table;
+    p.table = b.table;
     int64_t chunks = 0;
     auto flush = [&]() -> int {
       if (p.runs == 0) return kOk;
       CG_REQUIRE(chunks < (1ll << 31), "newton_schulz: too many elements in one call");
-      p.partial = partial + chunks_before;
+      p.partial = b.squares + chunks_before;
       if (pass == 0) prepare_kernel<T, MOMENTUM, true><<<(unsigned)chunks, 256, 0, s>>>(p);
       else prepare_kernel<T, MOMENTUM, false><<<(unsigned)chunks, 256, 0, s>>>(p);
       CG_LAUNCHED("newton_schulz prepare");
@@ -558,21 +641,23 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
   return kOk;
 }
 
-enum Step { kGram, kPoly, kUpdate };
-
 // One launch over all shapes: A = X X^T (X^T X), B = b A + c A A, or
 // X' = a X + B X (a X + X B).
 template <int CG, int BN, class E>
-static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, bool odd, const OutRef* table,
-                   float keep, const float* rate, cudaStream_t s) {
+static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Plan& plan, const Buffers& b,
+                   bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
   half::LaunchOf<E> L;
   memset(&L, 0, sizeof(L));
-  int64_t items = 0;
+  L.partial = b.partial;
+  L.counters = b.counters;
+  L.most_splits = plan.splits;
+  int64_t items = 0, tiles = 0;
   for (int i = 0; i < n; ++i) {
     const Shape& h = shapes[i];
     auto& G = L.g[i];
     const bool wide = h.rows <= h.cols;
     const __half* x = odd ? h.x1 : h.x0;
+    __half* next = odd ? h.x0 : h.x1;
     const int64_t xplane = h.rows * h.pitch, splane = h.s * h.spitch, planes = 2 * h.count;
     int rc = kOk;
     auto map_x = [&](CUtensorMap* map, bool mn, int box) {
@@ -581,22 +666,31 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, b
     auto map_s = [&](CUtensorMap* map, const __half* p, int box) {
       if (rc == kOk) rc = half::make_half_map(map, p, false, h.s, h.s, h.spitch, planes, splane, false, box);
     };
+    auto blocks_x = [&](CUtensorMap* map, const __half* p) {
+      if (rc == kOk)
+        rc = half::make_block_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, 64, p, h.rows, h.cols, h.pitch, planes,
+                                  xplane);
+    };
+    auto blocks_s = [&](CUtensorMap* map, const __half* p) {
+      if (rc == kOk)
+        rc = half::make_block_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, 64, p, h.s, h.s, h.spitch, planes, splane);
+    };
     const int a_box = half::kRows, b_box = BN / CG;
     EpiArgs& e = G.epi;
     if (step == kGram) {
       G.a_mn = G.b_mn = !wide;
       map_x(&G.map_a, !wide, a_box);
       map_x(&G.map_b, !wide, b_box);
+      blocks_s(&e.map_out, h.gram);
       G.m = G.n = (int)h.s;
       G.k = (int)(wide ? h.cols : h.rows);
-      e.out = h.gram;
       e.beta = 1.0f / kScale;
     } else if (step == kPoly) {
       map_s(&G.map_a, h.gram, a_box);
       map_s(&G.map_b, h.gram, b_box);
+      blocks_s(&e.map_aux, h.gram);
+      blocks_s(&e.map_out, h.poly);
       G.m = G.n = G.k = (int)h.s;
-      e.out = h.poly;
-      e.aux = h.gram;
       e.alpha = g.b;
       e.beta = g.c / kScale;
     } else {
@@ -608,33 +702,34 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, b
         map_x(&G.map_a, false, a_box);
         map_s(&G.map_b, h.poly, b_box);
       }
+      blocks_x(&e.map_aux, x);
+      if (!last) blocks_x(&e.map_out, next);
       G.m = (int)h.rows;
       G.n = (int)h.cols;
       G.k = (int)h.s;
-      e.out = odd ? h.x0 : h.x1;
-      e.aux = x;
       e.alpha = g.a;
       e.beta = 1.0f / kScale;
     }
     if (rc) return rc;
-    const bool square = step != kUpdate;
-    e.lower = G.lower = square;
-    e.out_plane = square ? splane : xplane;
-    e.out_pitch = (int)(square ? h.spitch : h.pitch);
-    e.aux_plane = step == kUpdate ? xplane : splane;
-    e.aux_pitch = (int)(step == kUpdate ? h.pitch : h.spitch);
-    if (table != nullptr) {  // the last product leaves the planes' scale
-      e.table = table + h.first_matrix;
+    e.has_aux = step != kGram;
+    e.lower = G.lower = step != kUpdate;
+    if (last) {  // leaves the planes' scale
+      e.table = b.table + h.first_matrix;
       e.alpha /= kScale;
       e.beta /= kScale;
       e.keep = keep;
       e.rate = rate[i];
     }
     G.batch = (int)h.count;
-    G.splits = 1;
-    G.kt_per = (int)ceil_div<int64_t>(G.k, half::kBK);
+    const int64_t kts = ceil_div<int64_t>(G.k, half::kBK);
+    G.kt_per = (int)ceil_div<int64_t>(kts, plan.splits);
+    G.splits = (int)ceil_div<int64_t>(kts, G.kt_per);
     G.first_item = (int)items;
-    items += half::plan_group<CG, BN>(G);
+    G.first_tile = (int)tiles;
+    const int64_t mine = half::plan_group<CG, BN>(G);
+    items += mine;
+    // a group may have fewer splits than planned: its tiles keep the planned room
+    tiles += mine / G.splits;
     CG_REQUIRE(items < (1ll << 31), "newton_schulz: too many tiles in one call");
   }
   L.groups = n;
@@ -642,47 +737,14 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, b
   return half::launch_half_gemm<CG, BN, 2, E>(L, s);
 }
 
-// Tile of a launch: the larger tiles feed the tensor cores best, the smaller
-// ones fill the SMs when there are few.
 template <class E>
-static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, bool odd, const OutRef* table,
+static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Buffers& b, bool odd, bool last,
                    float keep, const float* rate, cudaStream_t s) {
-  struct Choice {
-    int bm, bn, slots;
-    double clocks;
-  };
-  const int sms = sm_count();
-  const Choice choices[] = {{256, 256, sms / 2, 1600}, {256, 128, sms / 2, 900}, {128, 128, sms, 950}, {128, 64, sms, 650}};
-  int best = 0;
-  double least = 0.0;
-  for (int c = 0; c < 4; ++c) {
-    double tiles = 0.0, slices = 0.0;
-    for (int i = 0; i < n; ++i) {
-      const Shape& h = shapes[i];
-      const int64_t m = step == kUpdate ? h.rows : h.s, w = step == kUpdate ? h.cols : h.s;
-      const int64_t k = step == kGram ? (h.rows < h.cols ? h.cols : h.rows) : h.s;
-      double t = (double)ceil_div<int64_t>(m, choices[c].bm) * ceil_div<int64_t>(w, choices[c].bn);
-      if (step != kUpdate) {
-        t = 0.0;
-        for (int64_t r = 0; r < ceil_div<int64_t>(m, choices[c].bm); ++r)
-          t += half::lower_tiles_of_row((int)r, choices[c].bm, choices[c].bn, (int)ceil_div<int64_t>(w, choices[c].bn));
-      }
-      tiles += t * h.count;
-      slices += t * h.count * (ceil_div<int64_t>(k, half::kBK) + 2);
-    }
-    const double waves = ceil(tiles / choices[c].slots);
-    const double cost = waves * (slices / tiles) * choices[c].clocks;
-    if (c == 0 || cost < least) {
-      least = cost;
-      best = c;
-    }
-  }
-  switch (best) {
-    case 0: return product<2, 256, E>(g, shapes, n, step, odd, table, keep, rate, s);
-    case 1: return product<2, 128, E>(g, shapes, n, step, odd, table, keep, rate, s);
-    case 2: return product<1, 128, E>(g, shapes, n, step, odd, table, keep, rate, s);
-    default: return product<1, 64, E>(g, shapes, n, step, odd, table, keep, rate, s);
-  }
+  const Plan p = plan_of(shapes, n, step);
+  if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
+  if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
+  if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
+  return product<1, 64, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
 }
 
 static int run(const cg_ns_args& g, bool momentum, void* stream) {
@@ -693,13 +755,13 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
   for (int from = 0, to; from < g.n; from = to) {
     const int n = gather_shapes(g, from, shapes, &to);
     if (n == 0) continue;
-    double* partial;
-    OutRef* table;
-    layout(shapes, n, static_cast<char*>(g.workspace), &partial, &table);
-    if (momentum) rc = prepare<float, true>(g, from, to, shapes, n, partial, table, s);
-    else if (g.dtype == CG_F32) rc = prepare<float, false>(g, from, to, shapes, n, partial, table, s);
-    else if (g.dtype == CG_F16) rc = prepare<__half, false>(g, from, to, shapes, n, partial, table, s);
-    else rc = prepare<__nv_bfloat16, false>(g, from, to, shapes, n, partial, table, s);
+    Buffers b;
+    layout(shapes, n, static_cast<char*>(g.workspace), &b);
+    if (b.counter_bytes) CG_CUDA(cudaMemsetAsync(b.counters, 0, b.counter_bytes, s));
+    if (momentum) rc = prepare<float, true>(g, from, to, shapes, n, b, s);
+    else if (g.dtype == CG_F32) rc = prepare<float, false>(g, from, to, shapes, n, b, s);
+    else if (g.dtype == CG_F16) rc = prepare<__half, false>(g, from, to, shapes, n, b, s);
+    else rc = prepare<__nv_bfloat16, false>(g, from, to, shapes, n, b, s);
     if (rc) return rc;
     float rate[kGroups];
     for (int i = 0; i < n; ++i) {
@@ -709,12 +771,12 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     const float keep = momentum ? 1.0f - g.lr * g.weight_decay : 0.0f;
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;
-      if ((rc = product<SplitEpi>(g, shapes, n, kGram, odd, nullptr, 0.0f, nullptr, s))) return rc;
-      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, odd, nullptr, 0.0f, nullptr, s))) return rc;
-      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, odd, nullptr, 0.0f, nullptr, s);
-      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, odd, table, keep, rate, s);
-      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, odd, table, keep, rate, s);
-      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, odd, table, keep, rate, s);
+      if ((rc = product<SplitEpi>(g, shapes, n, kGram, b, odd, false, 0.0f, nullptr, s))) return rc;
+      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, b, odd, false, 0.0f, nullptr, s))) return rc;
+      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, b, odd, false, 0.0f, nullptr, s);
+      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
+      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
+      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
       if (rc) return rc;
     }
   }
