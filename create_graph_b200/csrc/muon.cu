@@ -84,6 +84,20 @@ __device__ inline void load_four(const __nv_bfloat16* p, float (&v)[4]) {
   v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
 }
 
+__device__ inline void put_value(float* p, float v) { *p = v; }
+__device__ inline void put_value(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ inline void put_value(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ inline void store_four(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <class H>
+__device__ inline void store_four(H* p, const float (&v)[4]) {
+  H h[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) put_value(h + e, v[e]);
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+}
+
 struct Momentum {
   float mu;
   int nesterov;
@@ -103,6 +117,14 @@ __device__ inline double block_sum(double s) {
   for (int w = 0; w < 8; ++w) s += sums[w];
   return s;
 }
+
+}  // namespace muon
+}  // namespace cg
+
+#include "muon_small.cuh"
+
+namespace cg {
+namespace muon {
 
 // NORM: advance the momentum and leave each chunk's sum of squares (in 64
 // bits: squares of gradients may leave the range of 32). Otherwise: read the
@@ -346,10 +368,6 @@ struct SplitEpi : EpiBase {
 };
 
 // The last step's result in the caller's matrices.
-__device__ inline void put_value(float* p, float v) { *p = v; }
-__device__ inline void put_value(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ inline void put_value(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 template <class T>
 struct FinalEpi : EpiBase {
   T* out;
@@ -436,6 +454,8 @@ constexpr int64_t kAlign = 256;
 static int64_t up(int64_t n, int64_t to) { return ceil_div<int64_t>(n, to) * to; }
 
 static bool empty(const cg_ns_entry& e) { return e.count == 0 || e.rows == 0 || e.cols == 0; }
+// Runs of matrices that a cluster holds in shared memory (muon_small.cuh).
+static bool is_small(const cg_ns_entry& e) { return small::cluster_of(e.rows, e.cols) > 0; }
 
 // The shapes of up to kGroups different sizes from entry `from` on; *to = the
 // first entry that does not fit.
@@ -443,7 +463,7 @@ static int gather_shapes(const cg_ns_args& g, int from, Shape* shapes, int* to) 
   int n = 0, i = from;
   for (; i < g.n; ++i) {
     const cg_ns_entry& e = g.entries[i];
-    if (empty(e)) continue;
+    if (empty(e) || is_small(e)) continue;
     int k = 0;
     while (k < n && (shapes[k].rows != e.rows || shapes[k].cols != e.cols)) ++k;
     if (k == n) {
@@ -606,7 +626,7 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
     };
     for (int i = from; i < to; ++i) {
       const cg_ns_entry& e = g.entries[i];
-      if (empty(e)) continue;
+      if (empty(e) || is_small(e)) continue;
       int k = 0;
       while (shapes[k].rows != e.rows || shapes[k].cols != e.cols) ++k;
       const Shape& h = shapes[k];
@@ -747,10 +767,88 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
   return product<1, 64, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
 }
 
+static float rate_of(const cg_ns_args& g, bool momentum, int64_t rows, int64_t cols) {
+  if (!momentum) return 1.0f;
+  const double ratio = (double)rows / (double)cols;
+  return (float)(-(double)g.lr * (ratio > 1.0 ? sqrt(ratio) : 1.0));
+}
+
+// The small matrices of a call. One launch with the largest cluster where all
+// fit the SMs at once (the time is that of one matrix, whatever its size), else
+// one per cluster size.
+template <class T, bool MOMENTUM>
+static int run_small(const cg_ns_args& g, cudaStream_t s) {
+  int64_t matrices = 0;
+  int largest = 0;
+  for (int i = 0; i < g.n; ++i) {
+    const cg_ns_entry& e = g.entries[i];
+    if (empty(e) || !is_small(e)) continue;
+    matrices += e.count;
+    const int c = small::cluster_of(e.rows, e.cols);
+    if (c > largest) largest = c;
+  }
+  if (matrices == 0) return kOk;
+  const bool together = matrices * largest <= sm_count();
+  for (int cluster = together ? largest : 1; cluster <= largest; cluster *= 2) {
+    small::Args p;
+    memset(&p, 0, sizeof(p));
+    p.steps = g.steps;
+    p.a = g.a;
+    p.b = g.b;
+    p.c = g.c;
+    p.eps = g.eps;
+    p.rule = {g.momentum, g.nesterov};
+    int64_t in_launch = 0;
+    auto flush = [&]() -> int {
+      if (p.runs == 0) return kOk;
+      CG_REQUIRE(in_launch < (1ll << 31), "newton_schulz: too many matrices in one call");
+      if (int rc = small::launch<T, MOMENTUM>(p, (int)in_launch, cluster, s)) return rc;
+      p.runs = 0;
+      in_launch = 0;
+      return kOk;
+    };
+    for (int i = 0; i < g.n; ++i) {
+      const cg_ns_entry& e = g.entries[i];
+      if (empty(e) || !is_small(e) || (!together && small::cluster_of(e.rows, e.cols) != cluster)) continue;
+      small::Run& r = p.run[p.runs];
+      r.x = e.x;
+      r.momentum = e.momentum;
+      r.out = e.out;
+      r.ld_x = e.ld_x;
+      r.ld_momentum = e.ld_momentum;
+      r.ld_out = e.ld_out;
+      r.stride_x = e.stride_x;
+      r.stride_out = e.stride_out;
+      r.rows = (int)e.rows;
+      r.cols = (int)e.cols;
+      r.count = (int)e.count;
+      r.first = (int)in_launch;
+      const uintptr_t mask = 4 * sizeof(T) - 1;
+      auto fours = [&](const void* p, int64_t ld, int64_t stride, uintptr_t low) {
+        return e.cols % 4 == 0 && ld % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & low) == 0;
+      };
+      r.vec_x = fours(e.x, e.ld_x, e.stride_x, mask) && (!MOMENTUM || fours(e.momentum, e.ld_momentum, 0, 15));
+      r.vec_out = fours(e.out, e.ld_out, e.stride_out, mask);
+      r.keep = MOMENTUM ? 1.0f - g.lr * g.weight_decay : 0.0f;
+      r.rate = rate_of(g, MOMENTUM, e.rows, e.cols);
+      in_launch += e.count;
+      if (++p.runs == small::kRuns)
+        if (int rc = flush()) return rc;
+    }
+    if (int rc = flush()) return rc;
+  }
+  return kOk;
+}
+
 static int run(const cg_ns_args& g, bool momentum, void* stream) {
   cudaStream_t s = as_stream(stream);
   int rc;
   if ((rc = half::bind_context())) return rc;
+  if (momentum) rc = run_small<float, true>(g, s);
+  else if (g.dtype == CG_F32) rc = run_small<float, false>(g, s);
+  else if (g.dtype == CG_F16) rc = run_small<__half, false>(g, s);
+  else rc = run_small<__nv_bfloat16, false>(g, s);
+  if (rc) return rc;
   Shape shapes[kGroups];
   for (int from = 0, to; from < g.n; from = to) {
     const int n = gather_shapes(g, from, shapes, &to);
@@ -764,10 +862,7 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     else rc = prepare<__nv_bfloat16, false>(g, from, to, shapes, n, b, s);
     if (rc) return rc;
     float rate[kGroups];
-    for (int i = 0; i < n; ++i) {
-      const double ratio = (double)shapes[i].rows / (double)shapes[i].cols;
-      rate[i] = momentum ? (float)(-(double)g.lr * (ratio > 1.0 ? sqrt(ratio) : 1.0)) : 1.0f;
-    }
+    for (int i = 0; i < n; ++i) rate[i] = rate_of(g, momentum, shapes[i].rows, shapes[i].cols);
     const float keep = momentum ? 1.0f - g.lr * g.weight_decay : 0.0f;
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;

@@ -54,7 +54,8 @@ def random(*shape, dtype=torch.float32, seed=0, scale=1.0):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (8, 8), (33, 65), (65, 33), (128, 128), (127, 129),
                                    (3, 130, 257), (2, 257, 130), (4, 64, 200), (300, 700), (1031, 260), (2, 3, 40, 24),
-                                   (640, 640), (17, 3000)])
+                                   (640, 640), (17, 3000), (100, 1024), (1024, 100), (128, 512), (385, 128),
+                                   (7, 129, 64), (128, 1025), (40, 16, 16)])
 def test_against_definition(shape, dtype):
     x = random(*shape, dtype=dtype, seed=1)
     got = newton_schulz(x)
@@ -165,9 +166,10 @@ def test_muon_steps(nesterov):
     assert not opt.flat[~inside].any() and not opt.momentum_buffer[~inside].any()
 
 
-def test_muon_many_matrices_in_one_step():
-    # more runs than one prepare launch takes
-    shapes = [(24, 40), (40, 24)] * 40
+@pytest.mark.parametrize("shapes", [[(24, 40), (40, 24)] * 40, [(160, 140), (140, 160)] * 16,
+                                    [(16, 20), (300, 30), (30, 700), (150, 136), (1000, 90)] * 12])
+def test_muon_many_matrices_in_one_step(shapes):
+    # more runs than one launch's table takes, more clusters than the SMs hold at once
     gen = torch.Generator().manual_seed(11)
     params = [torch.nn.Parameter(torch.randn(*s, generator=gen).cuda()) for s in shapes]
     before = [p.detach().double().cpu() for p in params]
@@ -251,11 +253,12 @@ def test_refusals():
         FusedMuon(FlatGradients([torch.nn.Parameter(torch.zeros(4, 4, device="cuda").half())], None))
     args = native.NsArgs()
     entry = native.NsEntry()
-    entry.x = entry.out = x.data_ptr()
-    entry.rows, entry.cols, entry.count, entry.ld_x, entry.ld_out = 8, 6, 1, 6, 6
+    large = random(200, 160)  # smaller matrices need no workspace
+    entry.x = entry.out = large.data_ptr()
+    entry.rows, entry.cols, entry.count, entry.ld_x, entry.ld_out = 200, 160, 1, 160, 160
     args.entries, args.n, args.steps, args.eps = native.ctypes.pointer(entry), 1, 5, 1e-7
     with pytest.raises(NativeError, match="workspace"):
         native.invoke("cg_newton_schulz", args, 0)
-    entry.ld_x = 5
+    entry.ld_x = 159
     with pytest.raises(NativeError, match="pitch"):
         native.invoke("cg_newton_schulz", args, 0)
