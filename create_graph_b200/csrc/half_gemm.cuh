@@ -20,7 +20,7 @@
 // bits) and a k-slice makes the products lo hi + hi lo + hi hi; the dropped
 // lo lo term is 2^-22 relative. The tensor core truncates as it adds to an
 // accumulator (a sum of positive terms over k = 3072, 576 additions, came out
-// 2e-5 low), so accumulators then hold kSumSlices k-slices at a time and the
+// 2e-5 low), so accumulators then hold a few k-slices at a time and the
 // epilogue warps add them up in registers, rounded to nearest.
 // A pair of SMs halves the B bytes each SM stages per flop: a 256 x 256 tile
 // takes 32 KB of shared memory per 64-wide slice and SM against 48 KB for the
@@ -46,7 +46,6 @@ constexpr int kRows = 128;     // accumulator rows per CTA
 // warps of a block: producer, issuer and `epi` epilogue warps (a multiple of
 // four, epi / 4 per TMEM lane quarter)
 __host__ __device__ constexpr int threads_of(int epi) { return 32 * (2 + epi); }
-constexpr int kSumSlices = 2;  // k-slices summed in one accumulator when PLANES = 2
 constexpr int kBand = 8;       // m-tiles of one band of the tile walk (a power of two)
 
 // Bounded wait of a whole warp, with one outcome for all its lanes: 2^24 polls
@@ -235,6 +234,7 @@ struct Launch {
   float4* partial;
   unsigned* counters;
   int most_splits;  // room per tile
+  int sum_slices;   // PLANES = 2: k-slices summed in one accumulator
 };
 template <class Epi>
 using LaunchOf = Launch<typename Epi::Args, Epi::kGroups>;
@@ -411,8 +411,8 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
       // 16 along k = two groups.
       const uint32_t a_lbo = g.a_mn ? kBK * 128 : 16, a_step = g.a_mn ? 2048 : 32;
       const uint32_t b_lbo = g.b_mn ? kBK * 128 : 16, b_step = g.b_mn ? 2048 : 32;
-      // one accumulator per item, or per kSumSlices of it
-      const int per = PLANES == 2 ? kSumSlices : item.kt1 - item.kt0;
+      // one accumulator per item, or per sum_slices of it
+      const int per = PLANES == 2 ? L.sum_slices : item.kt1 - item.kt0;
       for (int kt0 = item.kt0; kt0 < item.kt1 && ok; kt0 += per, ++j) {
         const int b = j & 1, use = j >> 1;
         const int kt1 = kt0 + per < item.kt1 ? kt0 + per : item.kt1;
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
 #pragma unroll
           for (int x = 0; x < 32; ++x) sum[q][x] = 0.0f;
         epi.fetch(item.n0 + c_first);  // beside the wait for the accumulator
-        for (int kt = item.kt0; kt < item.kt1; kt += kSumSlices, ++j) {
+        for (int kt = item.kt0; kt < item.kt1; kt += L.sum_slices, ++j) {
           const int b = j & 1;
           if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
           tc_fence_after();

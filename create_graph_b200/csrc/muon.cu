@@ -229,6 +229,7 @@ struct EpiArgs {
   CUtensorMap map_aux, map_out;
   int has_aux;
   float alpha, beta;  // alpha aux + beta accumulator
+  float diagonal;     // added on the diagonal (of a symmetric result)
   int lower;          // symmetric result
   // final epilogue: out <- keep out + rate value (keep = 0: out is not read)
   const OutRef* table;
@@ -333,6 +334,10 @@ struct SplitEpi : EpiBase {
   __device__ __forceinline__ bool store(float (&v)[32], int col0, int* error) {
     if (outside(col0)) return true;
     const bool ok = values(v, error);
+    if (a->diagonal != 0.0f && row0 == col0) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] += e == lane ? a->diagonal : 0.0f;
+    }
     // hi = fp16(v), lo = fp16(v - hi)
     uint32_t hi[16], lo[16];
 #pragma unroll
@@ -665,12 +670,13 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
 // X' = a X + B X (a X + X B).
 template <int CG, int BN, class E>
 static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Plan& plan, const Buffers& b,
-                   bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
+                   bool coarse, bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
   half::LaunchOf<E> L;
   memset(&L, 0, sizeof(L));
   L.partial = b.partial;
   L.counters = b.counters;
   L.most_splits = plan.splits;
+  L.sum_slices = coarse ? 4 : 2;
   int64_t items = 0, tiles = 0;
   for (int i = 0; i < n; ++i) {
     const Shape& h = shapes[i];
@@ -713,6 +719,7 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       G.m = G.n = G.k = (int)h.s;
       e.alpha = g.b;
       e.beta = g.c / kScale;
+      e.diagonal = coarse ? g.a * kScale : 0.0f;
     } else {
       if (wide) {
         map_s(&G.map_a, h.poly, a_box);
@@ -722,7 +729,7 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
         map_x(&G.map_a, false, a_box);
         map_s(&G.map_b, h.poly, b_box);
       }
-      blocks_x(&e.map_aux, x);
+      if (!coarse) blocks_x(&e.map_aux, x);
       if (!last) blocks_x(&e.map_out, next);
       G.m = (int)h.rows;
       G.n = (int)h.cols;
@@ -731,7 +738,7 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       e.beta = 1.0f / kScale;
     }
     if (rc) return rc;
-    e.has_aux = step != kGram;
+    e.has_aux = step == kPoly || (step == kUpdate && !coarse);
     e.lower = G.lower = step != kUpdate;
     if (last) {  // leaves the planes' scale
       e.table = b.table + h.first_matrix;
@@ -758,13 +765,13 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
 }
 
 template <class E>
-static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Buffers& b, bool odd, bool last,
-                   float keep, const float* rate, cudaStream_t s) {
+static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Buffers& b, bool coarse, bool odd,
+                   bool last, float keep, const float* rate, cudaStream_t s) {
   const Plan p = plan_of(shapes, n, step);
-  if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
-  if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
-  if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
-  return product<1, 64, E>(g, shapes, n, step, p, b, odd, last, keep, rate, s);
+  if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
+  if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
+  if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
+  return product<1, 64, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
 }
 
 static float rate_of(const cg_ns_args& g, bool momentum, int64_t rows, int64_t cols) {
@@ -864,14 +871,21 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     float rate[kGroups];
     for (int i = 0; i < n; ++i) rate[i] = rate_of(g, momentum, shapes[i].rows, shapes[i].cols);
     const float keep = momentum ? 1.0f - g.lr * g.weight_decay : 0.0f;
+    // Results that are rounded to half precision, or added to weights a
+    // hundredth to a thousandth part at a time, are formed a little less exactly
+    // (about 1e-5 relative on strongly decaying spectra instead of 5e-6): B
+    // carries a on its diagonal, so that X <- B X reads no X beside its operand,
+    // and accumulators run for four k-slices instead of two, so that the products
+    // run further ahead of the epilogue. COARSEFIG
+    const bool coarse = momentum || g.dtype != CG_F32;
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;
-      if ((rc = product<SplitEpi>(g, shapes, n, kGram, b, odd, false, 0.0f, nullptr, s))) return rc;
-      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, b, odd, false, 0.0f, nullptr, s))) return rc;
-      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, b, odd, false, 0.0f, nullptr, s);
-      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
-      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
-      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, b, odd, true, keep, rate, s);
+      if ((rc = product<SplitEpi>(g, shapes, n, kGram, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, b, coarse, odd, false, 0.0f, nullptr, s);
+      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
+      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
+      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
       if (rc) return rc;
     }
   }
