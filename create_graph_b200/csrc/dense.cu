@@ -409,6 +409,8 @@ struct PlainEpi : EpiBase {
 // elements as the epilogue does; VEC: groups of eight columns.
 template <class T, bool VEC>
 __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits, int m, int n) {
+  half::allow_next();
+  half::wait_previous();
   const int64_t mn = (int64_t)m * n, stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t first = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (VEC) {
@@ -457,6 +459,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
                                                        const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
                                                        int64_t ld_gz, int rows, int cols, int kind, int rows_per,
                                                        float* __restrict__ partial, T* __restrict__ db) {
+  half::allow_next();
+  half::wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.x * 32 + lane) * V;
   const int r0 = blockIdx.y * rows_per, r1 = min(rows, r0 + rows_per);
@@ -503,6 +507,8 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
 // db[c] = sum of the chunks' sums in chunk order, rounded once.
 template <class T>
 __global__ void join_columns_kernel(const float* __restrict__ partial, int chunks, int cols, T* __restrict__ db) {
+  half::allow_next();
+  half::wait_previous();
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= cols) return;
   float s = 0.0f;
@@ -713,9 +719,10 @@ static int run_typed(const cg_linear_args* g, int count, void* workspace, int64_
     const int64_t blocks = ceil_div<int64_t>(ceil_div<int64_t>(g[i].m * g[i].n, vec ? 8 : 1), 256);
     const int64_t most = (int64_t)sm_count() * 8;
     const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-    if (vec) join_splits_kernel<T, true><<<grid, 256, 0, s>>>(ea[i], p.splits[i], (int)g[i].m, (int)g[i].n);
-    else join_splits_kernel<T, false><<<grid, 256, 0, s>>>(ea[i], p.splits[i], (int)g[i].m, (int)g[i].n);
-    CG_LAUNCHED("linear_half split join");
+    auto kernel = vec ? join_splits_kernel<T, true> : join_splits_kernel<T, false>;
+    if ((rc = half::launch_chained("linear_half split join", kernel, dim3(grid), 256, 0, dim3(1, 1), s, ea[i],
+                                   p.splits[i], (int)g[i].m, (int)g[i].n)))
+      return rc;
   }
   return kOk;
 }
@@ -770,19 +777,15 @@ static int act_grad_typed(const cg_act_grad_args& g, cudaStream_t s) {
   const bool direct = chunks == 1;
   float* partial = g.db && !direct ? g.scratch : nullptr;
   T* db = g.db && direct ? (T*)g.db : nullptr;
-  if (vec)
-    act_grad_kernel<T, 8><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
-                                               (int)g.rows, (int)g.cols, g.act, per, partial, db);
-  else
-    act_grad_kernel<T, 1><<<grid, 256, 0, s>>>((const T*)g.gy, g.ld_gy, (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz,
-                                               (int)g.rows, (int)g.cols, g.act, per, partial, db);
-  CG_LAUNCHED("act_grad_half");
-  if (partial) {
-    join_columns_kernel<T><<<(unsigned)ceil_div<int64_t>(g.cols, 128), 128, 0, s>>>(partial, chunks, (int)g.cols,
-                                                                                    (T*)g.db);
-    CG_LAUNCHED("act_grad_half column join");
-  }
-  return kOk;
+  auto kernel = vec ? act_grad_kernel<T, 8> : act_grad_kernel<T, 1>;
+  if (int rc = half::launch_chained("act_grad_half", kernel, grid, 256, 0, dim3(1, 1), s, (const T*)g.gy, g.ld_gy,
+                                    (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz, (int)g.rows, (int)g.cols, g.act, per,
+                                    partial, db))
+    return rc;
+  if (partial == nullptr) return kOk;
+  return half::launch_chained("act_grad_half column join", join_columns_kernel<T>,
+                              dim3((unsigned)ceil_div<int64_t>(g.cols, 128)), 128, 0, dim3(1, 1), s,
+                              (const float*)partial, chunks, (int)g.cols, (T*)g.db);
 }
 
 static int64_t act_grad_scratch(int64_t rows, int64_t cols) {

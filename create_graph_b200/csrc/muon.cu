@@ -132,6 +132,8 @@ namespace muon {
 // Block = one chunk of kChunk elements of one matrix.
 template <class T, bool MOMENTUM, bool NORM>
 __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Prepare p) {
+  half::allow_next();
+  half::wait_previous();
   int i = 0;
   while (i + 1 < p.runs && (int)blockIdx.x >= p.run[i + 1].first_chunk) ++i;
   const Run& run = p.run[i];
@@ -621,9 +623,9 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
       if (p.runs == 0) return kOk;
       CG_REQUIRE(chunks < (1ll << 31), "newton_schulz: too many elements in one call");
       p.partial = b.squares + chunks_before;
-      if (pass == 0) prepare_kernel<T, MOMENTUM, true><<<(unsigned)chunks, 256, 0, s>>>(p);
-      else prepare_kernel<T, MOMENTUM, false><<<(unsigned)chunks, 256, 0, s>>>(p);
-      CG_LAUNCHED("newton_schulz prepare");
+      auto kernel = pass == 0 ? prepare_kernel<T, MOMENTUM, true> : prepare_kernel<T, MOMENTUM, false>;
+      if (int rc = half::launch_chained("newton_schulz prepare", kernel, dim3((unsigned)chunks), 256, 0, dim3(1, 1), s, p))
+        return rc;
       chunks_before += chunks;
       p.runs = 0;
       chunks = 0;

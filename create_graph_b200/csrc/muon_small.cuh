@@ -174,6 +174,8 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   half::cluster_sync_all();  // every CTA runs before a peer reaches into it
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  half::allow_next();
+  half::wait_previous();
 
   // ---- the update u of this CTA's tile, in registers; the norm over the cluster
   float u[kGroupsOf4][4];
@@ -390,21 +392,8 @@ template <class T, bool MOMENTUM>
 int launch(const Args& p, int matrices, int cluster, cudaStream_t stream) {
   auto kernel = newton_schulz_small_kernel<T, MOMENTUM>;
   CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kBytes));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)matrices, (unsigned)cluster);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Smem::kBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = (unsigned)cluster;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  CG_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
-  CG_LAUNCHED("newton_schulz small");
-  return kOk;
+  return half::launch_chained("newton_schulz small", kernel, dim3((unsigned)matrices, (unsigned)cluster), kThreads,
+                              Smem::kBytes, dim3(1, (unsigned)cluster), stream, p);
 }
 
 }  // namespace small
