@@ -362,24 +362,32 @@ struct BlockEpi : EpiBase {
 };
 
 // Any pitch and alignment: blocks are transposed through shared memory and
-// stored one column per lane.
+// stored one column per lane; the residual of a 32 x 32 block is read before the
+// accumulator is waited for.
 template <class T>
 struct PlainEpi : EpiBase {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = 16;
   static constexpr int kStagingBytes = 32 * 32 * 4;
   using EpiBase::EpiBase;
-  __device__ void fetch(int) {}
-  static __device__ __forceinline__ void finish1(const EpiArgs& a, float v, int64_t row, int col) {
-    if (a.bias) v += to_float(static_cast<const T*>(a.bias)[col]);
+  T res[32];
+  __device__ __forceinline__ void fetch32(int col0) {
+    if (p->residual == nullptr || p->partial != nullptr) return;
+    const int col = col0 + lane;
+    const T* at = static_cast<const T*>(p->residual) + (int64_t)row0 * p->ld_res + col;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (col < n && row0 + r < m) res[r] = at[r * p->ld_res];
+  }
+  __device__ void fetch(int col0) { fetch32(col0); }
+  static __device__ __forceinline__ void finish1(const EpiArgs& a, float v, float residual, int64_t row, int col) {
     if (a.z) static_cast<T*>(a.z)[row * a.ld_z + col] = from_float<T>(v);
-    v = act(v, a.act);
-    if (a.residual) v += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]);
-    static_cast<T*>(a.y)[row * a.ld_y + col] = from_float<T>(v);
+    static_cast<T*>(a.y)[row * a.ld_y + col] = from_float<T>(act(v, a.act) + residual);
   }
   __device__ bool store(uint32_t acc, int col0, int*) {
     float* stage = reinterpret_cast<float*>(staging);
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
+      if (h == 1) fetch32(col0 + 32);
       float v[32];
       tmem_load_32(acc + 32 * h, v);
 #pragma unroll
@@ -389,13 +397,15 @@ struct PlainEpi : EpiBase {
       __syncwarp();
       const int col = col0 + 32 * h + lane;
       if (col < n) {
-#pragma unroll 8
+        const bool partial = p->partial != nullptr, add = p->residual != nullptr;
+        const float bias = p->bias && !partial ? to_float(static_cast<const T*>(p->bias)[col]) : 0.0f;
+#pragma unroll
         for (int r = 0; r < 32; ++r) {
           const int64_t row = row0 + r;
           if (row >= m) break;
           const float x = stage[half::stage_idx(r, lane)];
-          if (p->partial) p->partial[((int64_t)split * m + row) * n + col] = x;
-          else finish1(*p, x, row, col);
+          if (partial) p->partial[((int64_t)split * m + row) * n + col] = x;
+          else finish1(*p, x + bias, add ? to_float(res[r]) : 0.0f, row, col);
         }
       }
       __syncwarp();
@@ -444,7 +454,11 @@ __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits
     for (int64_t i = first; i < mn; i += stride) {
       float v = 0.0f;
       for (int s = 0; s < splits; ++s) v += a.partial[s * mn + i];
-      PlainEpi<T>::finish1(a, v, i / n, (int)(i % n));
+      const int64_t row = i / n;
+      const int col = (int)(i % n);
+      if (a.bias) v += to_float(static_cast<const T*>(a.bias)[col]);
+      PlainEpi<T>::finish1(
+          a, v, a.residual ? to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]) : 0.0f, row, col);
     }
   }
 }
@@ -531,6 +545,33 @@ __global__ void act_grad2_kernel(const T* __restrict__ h, const T* __restrict__ 
   }
 }
 
+// Rows of one or two matrices onto 16-byte boundaries: a thread writes 8 values.
+struct Padded {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t ld_src, ld_dst, rows;
+  int cols;
+};
+__global__ void __launch_bounds__(256) pad_rows_kernel(Padded a, Padded b) {
+  half::allow_next();
+  half::wait_previous();
+  const int64_t first = (a.ld_dst / 8) * a.rows, all = first + (b.ld_dst / 8) * b.rows;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < all; i += stride) {
+    const Padded& p = i < first ? a : b;
+    const int64_t at = i < first ? i : i - first, per = p.ld_dst / 8, row = at / per;
+    const int col = (int)(at - row * per) * 8;
+    const uint16_t* src = p.src + row * p.ld_src + col;
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = col + 2 * e < p.cols ? src[2 * e] : 0, y = col + 2 * e + 1 < p.cols ? src[2 * e + 1] : 0;
+      v[e] = x | y << 16;
+    }
+    *reinterpret_cast<uint4*>(p.dst + row * p.ld_dst + col) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 // ---- host side ---------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -540,16 +581,21 @@ struct Plan {
 };
 
 // Tile of a launch and k-splits of its one or two products, by the time of the
-// slot (SM or SM pair) that gets most: a tile takes `fixed` (its epilogue's
-// tail and pipeline start) and `slice` per 64-wide k-slice, in nanoseconds
-// measured on full waves (PLANFIG).
-static Plan plan_of(const cg_linear_args* g, int count) {
+// slot (SM or SM pair) that gets most: a tile takes `slice` per 64-wide k-slice
+// and `wave` beside it, in nanoseconds measured on launches of one wave and of
+// several, and a launch `once`. 256 x 256 tiles of an SM pair feed the tensor
+// cores best (4096^3: 96 us, 110 us with 256 x 128, 116 with 128 x 128, 223 with
+// 128 x 64), the smaller ones fill the SMs when there are few (512^3: 8.4, 6.7,
+// 5.9 and 5.1 us); a split pays when k is long (3072 x 768 x 8280: 34 us in two
+// parts, 48 us whole).
+static Plan search_plan(const cg_linear_args* g, int count) {
   const int64_t sms = sm_count();
   struct Shape {
     int cg, bn;
-    double slice, fixed;
+    double slice, wave, once;
   };
-  static const Shape shapes[] = {{2, 256, 390, 1300}, {2, 128, 290, 1300}, {1, 128, 330, 1200}, {1, 64, 230, 1000}};
+  static const Shape shapes[] = {
+      {2, 256, 340, 1550, 3900}, {2, 128, 240, 900, 3900}, {1, 128, 260, 800, 3400}, {1, 64, 260, 700, 3200}};
   const int kMost = 24;
   int64_t kts[2] = {1, 1};
   for (int i = 0; i < count; ++i) kts[i] = ceil_div<int64_t>(g[i].k, half::kBK);
@@ -576,9 +622,9 @@ static Plan plan_of(const cg_linear_args* g, int count) {
           per[i] = ceil_div<int64_t>(kts[i], split[i]);
           same = same && ceil_div<int64_t>(kts[i], per[i]) == split[i];
           items[i] = tiles[i] * split[i];
-          time[i] = (double)per[i] * s.slice + s.fixed;
-          // a launch, and the partial tiles written and read at about 4 TB/s
-          if (split[i] > 1) join += 2500.0 + (double)split[i] * g[i].m * g[i].n * 8.0 / 4000.0;
+          time[i] = (double)per[i] * s.slice + s.wave;
+          // the join's launch on both sides, the partial tiles written and read at about 4 TB/s
+          if (split[i] > 1) join += 4500.0 + (double)split[i] * g[i].m * g[i].n * 8.0 / 4000.0;
         }
         if (!same) continue;
         // slot k gets items k, k + slots, ..: at most three different loads
@@ -589,7 +635,7 @@ static Plan plan_of(const cg_linear_args* g, int count) {
           const double load = (double)first * time[0] + (double)(all - first) * time[1];
           if (load > cost) cost = load;
         }
-        cost += join;
+        cost += join + s.once;
         if (least == 0.0 || cost < least) {
           least = cost;
           best.cg = s.cg;
@@ -602,6 +648,27 @@ static Plan plan_of(const cg_linear_args* g, int count) {
       }
   }
   return best;
+}
+
+// The search takes tens of microseconds for two products that may both split, so
+// each host thread keeps the plans of the last sizes it met.
+static Plan plan_of(const cg_linear_args* g, int count) {
+  struct Entry {
+    int64_t key[7];
+    Plan plan;
+  };
+  constexpr int kEntries = 256;
+  static thread_local Entry table[kEntries];
+  const int64_t key[7] = {g[0].m, g[0].n, g[0].k, count > 1 ? g[1].m : 0, count > 1 ? g[1].n : 0,
+                          count > 1 ? g[1].k : 0, sm_count()};
+  uint64_t h = 1469598103934665603ull;
+  for (int64_t v : key) h = (h ^ (uint64_t)v) * 1099511628211ull;
+  Entry& e = table[(h >> 32) % kEntries];
+  if (memcmp(e.key, key, sizeof(key)) != 0) {
+    e.plan = search_plan(g, count);
+    memcpy(e.key, key, sizeof(key));
+  }
+  return e.plan;
 }
 
 static int64_t partial_bytes(const cg_linear_args& g, int splits) {
@@ -757,8 +824,9 @@ static int run(const cg_linear_args* args, void* stream) {
 }
 
 // Row chunks of act_grad: enough blocks to fill the SMs several times, each of
-// at least 32 rows.
+// at least 32 rows; up to 128 rows are one chunk, whose sums need no join.
 static int chunk_rows(int64_t rows, int64_t cols, int v) {
+  if (rows <= 128) return 128;
   const int64_t strips = ceil_div<int64_t>(cols, 32 * v);
   int64_t chunks = ceil_div<int64_t>((int64_t)sm_count() * 8, strips);
   int64_t per = ceil_div<int64_t>(rows, chunks);
@@ -931,6 +999,29 @@ int cg_linear_half(const cg_linear_args* args, void* stream) { return cg::dense:
 int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args) {
   if (args == nullptr || args->m <= 0 || args->n <= 0 || args->k <= 0) return 0;
   return cg::dense::workspace_bytes(args, 1);
+}
+
+int cg_pad_rows_half(const void* src, int64_t ld_src, int64_t rows, int64_t cols, void* dst, int64_t ld_dst,
+                     const void* src2, int64_t ld_src2, int64_t rows2, int64_t cols2, void* dst2, int64_t ld_dst2,
+                     void* stream) {
+  using namespace cg;
+  auto padded = [](const void* from, int64_t ld_from, int64_t r, int64_t c, void* to, int64_t ld_to) {
+    return dense::Padded{static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), ld_from, ld_to, r, (int)c};
+  };
+  auto fine = [](const void* from, int64_t ld_from, int64_t r, int64_t c, const void* to, int64_t ld_to) {
+    return r >= 0 && c >= 0 && c < (1ll << 31) &&
+           (r == 0 || (from != nullptr && to != nullptr && dense::aligned16(to) && ld_to % 8 == 0 && ld_from >= c &&
+                       ld_to >= c));
+  };
+  CG_REQUIRE(fine(src, ld_src, rows, cols, dst, ld_dst) && fine(src2, ld_src2, rows2, cols2, dst2, ld_dst2),
+             "pad_rows_half: bad size, pitch or alignment");
+  const int64_t work = ld_dst / 8 * rows + (rows2 > 0 ? ld_dst2 / 8 * rows2 : 0);
+  if (work == 0) return kOk;
+  const int64_t blocks = ceil_div<int64_t>(work, 256), most = (int64_t)sm_count() * 8;
+  return cg::half::launch_chained("pad_rows_half", dense::pad_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)),
+                              256, 0, dim3(1, 1), as_stream(stream), padded(src, ld_src, rows, cols, dst, ld_dst),
+                              rows2 > 0 ? padded(src2, ld_src2, rows2, cols2, dst2, ld_dst2)
+                                        : dense::Padded{nullptr, nullptr, 0, 8, 0, 0});
 }
 
 int cg_linear_half_backward(const cg_linear_backward_args* args, void* stream) {

@@ -33,6 +33,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -181,6 +183,20 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a
 // each kernel of a chain of small products.
 __device__ inline void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ inline void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Allow a kernel its dynamic shared memory, once per device and kernel (one Tag
+// each; the call takes about half a microsecond).
+template <class Tag, class K>
+int allow_shared(K* kernel, int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  CG_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_acquire) & bit) return kOk;
+  CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return kOk;
+}
 
 template <class... P, class... A>
 int launch_chained(const char* name, void (*kernel)(P...), dim3 grid, int threads, int smem, dim3 cluster,
@@ -689,7 +705,7 @@ template <int CG, int BN, int PLANES, class Epi>
 int launch_half_gemm(const LaunchOf<Epi>& L, cudaStream_t stream) {
   using T = Tile<CG, BN, PLANES, Epi>;
   auto kernel = half_gemm_kernel<CG, BN, PLANES, Epi>;
-  CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kBytes));
+  if (int rc = allow_shared<T>(kernel, T::kBytes)) return rc;
   const int slots = sm_count() / CG;
   return launch_chained("half_gemm", kernel, dim3((unsigned)(CG * (L.items < slots ? L.items : slots))),
                         threads_of(Epi::kWarps), T::kBytes, dim3(CG, 1), stream, L);

@@ -496,16 +496,20 @@ struct Plan {
   int64_t slots, floats;  // with splits: counters and partial sums
 };
 
-// By the time of a slot (SM or SM pair): a tile takes `fixed` and `slice` per
-// 64-wide k-slice (three products), in nanoseconds measured on full waves
-// (NSFIG). Larger tiles feed the tensor cores best, smaller ones and splits of
-// k fill the SMs when there are few.
+// By time, in nanoseconds measured on launches of one wave and of several: a
+// launch takes `once`, and each wave of tiles `slice` per 64-wide k-slice
+// (three products) and `wave`; a split adds the partial sums it leaves and
+// reads. Larger tiles feed the tensor cores best, smaller ones and splits of k
+// fill the SMs when there are few: the gram of one 3072 x 768 matrix takes 50 us
+// on 256 x 256 tiles, 28 us on 128 x 64 and 15 us with k split in three; for
+// twelve of them 59, 101 and (too many tiles to split) 101 us.
 static Plan plan_of(const Shape* shapes, int n, Step step) {
   struct Tile {
     int cg, bn;
-    double slice, fixed;
+    double slice, wave, once;
   };
-  static const Tile choices[] = {{2, 256, 1000, 3000}, {2, 128, 600, 2500}, {1, 128, 600, 2500}, {1, 64, 400, 2000}};
+  static const Tile choices[] = {
+      {2, 256, 840, 7400, 3000}, {2, 128, 580, 4000, 3200}, {1, 128, 600, 2700, 4300}, {1, 64, 475, 1300, 4000}};
   const int sms = sm_count();
   Plan best = {2, 256, 1, 0, 0};
   double least = 0.0;
@@ -531,10 +535,11 @@ static Plan plan_of(const Shape* shapes, int n, Step step) {
         any = any || (parts == splits && per >= 2);
         tiles += count;
         items += (double)count * parts;
-        time += (double)count * parts * (per * t.slice + t.fixed + (parts > 1 ? 1000.0 + 300.0 * parts : 0.0));
+        const double join = parts > 1 ? 1300.0 + t.bn / 64 * (300.0 + 250.0 * parts) : 0.0;
+        time += (double)count * parts * (per * t.slice + t.wave + join);
       }
       if (!any) continue;
-      const double cost = ceil(items / slots) * time / items;
+      const double cost = t.once + ceil(items / slots) * time / items;
       if (least == 0.0 || cost < least) {
         least = cost;
         best.cg = t.cg;
@@ -878,7 +883,8 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     // (about 1e-5 relative on strongly decaying spectra instead of 5e-6): B
     // carries a on its diagonal, so that X <- B X reads no X beside its operand,
     // and accumulators run for four k-slices instead of two, so that the products
-    // run further ahead of the epilogue. COARSEFIG
+    // run further ahead of the epilogue: an update product of the 85M step takes
+    // 273 us against 350.
     const bool coarse = momentum || g.dtype != CG_F32;
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;

@@ -391,7 +391,8 @@ inline int cluster_of(int64_t rows, int64_t cols) {
 template <class T, bool MOMENTUM>
 int launch(const Args& p, int matrices, int cluster, cudaStream_t stream) {
   auto kernel = newton_schulz_small_kernel<T, MOMENTUM>;
-  CG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kBytes));
+  struct Tag {};
+  if (int rc = half::allow_shared<Tag>(kernel, Smem::kBytes)) return rc;
   return half::launch_chained("newton_schulz small", kernel, dim3((unsigned)matrices, (unsigned)cluster), kThreads,
                               Smem::kBytes, dim3(1, (unsigned)cluster), stream, p);
 }

@@ -54,19 +54,55 @@ def _fits_tma(t: Tensor, row: int, col: int) -> bool:
         and t.data_ptr() % 16 == 0
 
 
-def _operand(t: Tensor) -> tuple[Tensor, int, bool]:
-    """(tensor, row pitch, MN-major) of a logical (rows, K) operand."""
+def _stream(t: Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _in_place(t: Tensor):
+    """(tensor, row pitch, MN-major) of a logical (rows, K) operand that the
+    products can read as it is stored; None when its rows need copying."""
+    if t.is_contiguous():  # the usual case, in few steps
+        k = t.shape[1]
+        if k % 8 == 0 and t.data_ptr() % 16 == 0:
+            return t, k, False
     if _fits_tma(t, 0, 1):
         return t, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8, False
     if _fits_tma(t, 1, 0):
         return t, t.stride(1) if t.shape[1] > 1 else -(-t.shape[0] // 8) * 8, True
-    if t.stride(0) == 1 and t.shape[0] > 1:  # transposed with an odd pitch: keep its layout
-        copy = _pitched(t.shape[1], t.shape[0], t)
-        copy.copy_(t.t())
-        return copy, copy.stride(0), True
-    copy = _pitched(t.shape[0], t.shape[1], t)
-    copy.copy_(t)
-    return copy, copy.stride(0), False
+    return None
+
+
+def _operands(*ts: Tensor) -> list:
+    """_in_place of each of one or two operands, those that need it copied into
+    one padded buffer by one launch (in their own layout: a transposed view
+    stays transposed)."""
+    ops = [_in_place(t) for t in ts]
+    if None not in ops:
+        return ops
+    todo = []
+    for i, t in enumerate(ts):
+        if ops[i] is None:
+            mn = t.stride(0) == 1 and t.stride(1) >= t.shape[0]
+            stored = t.t() if mn else _rows(t)
+            todo.append((i, stored, mn, -(-stored.shape[1] // 8) * 8))
+    flat = torch.empty(sum(s.shape[0] * pitch for _, s, _, pitch in todo), dtype=ts[0].dtype, device=ts[0].device)
+    at, args = flat.data_ptr(), []
+    for i, s, mn, pitch in todo:
+        args += [s.data_ptr(), max(s.stride(0), s.shape[1]), s.shape[0], s.shape[1], at, pitch]
+        ops[i] = (_Copy(flat, at), pitch, mn)
+        at += 2 * s.shape[0] * pitch
+    native.invoke("cg_pad_rows_half", *args, *([None, 0, 0, 0, None, 0] if len(todo) == 1 else []), _stream(ts[0]))
+    return ops
+
+
+class _Copy:
+    """A padded copy inside a buffer that it keeps alive."""
+
+    def __init__(self, buffer: Tensor, address: int):
+        self.buffer, self.address = buffer, address
+
+    def data_ptr(self) -> int:
+        return self.address
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -89,14 +125,10 @@ def _backward_workspace_bytes(m: int, n: int, k: int, act: int, dx: bool, dw: bo
     return native.lib().cg_linear_half_backward_workspace_bytes(ctypes.byref(args))
 
 
-def _stream(t: Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
 def _forward(a_op, b_op, shape, bias, activation, residual, keep_z, like):
     """(y, z) of one product of operands as _operand gives them."""
     m, n, k = shape
-    y = torch.empty((m, n), dtype=like.dtype, device=like.device)
+    y = like.new_empty((m, n))
     z = torch.empty_like(y) if keep_z else None
     args = native.LinearArgs()
     args.m, args.n, args.k = m, n, k
@@ -133,7 +165,7 @@ def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = 
         return y, torch.empty_like(y) if keep_z else None
     if k == 0:  # an empty sum: zero columns give it
         a, b, k = a.new_zeros(m, 8), b.new_zeros(n, 8), 8
-    return _forward(_operand(a), _operand(b), (m, n, k), bias, activation, residual, keep_z, a)
+    return _forward(*_operands(a, b), (m, n, k), bias, activation, residual, keep_z, a)
 
 
 def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
@@ -143,11 +175,11 @@ def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
     args.m, args.n, args.k, args.act, args.dtype = m, n, k, activation, native.HALF_DTYPES[gy.dtype]
     gz = None
     if activation == native.ACT_NONE:
-        if not _fits_tma(gy, 0, 1):
-            copy = _pitched(m, n, gy)
-            copy.copy_(gy)
-            gy = copy
-        args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
+        if _fits_tma(gy, 0, 1):
+            args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
+        else:
+            kept, args.ld_gy, _ = _operands(gy.contiguous())[0]
+            args.gy = kept.data_ptr()
     else:
         gy = _rows(gy)
         gz = _pitched(m, n, gy)
@@ -157,9 +189,9 @@ def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
     x, args.ld_x, args.x_mn_major = x_op
     w, args.ld_w, args.w_mn_major = w_op
     args.x, args.w = x.data_ptr(), w.data_ptr()
-    dx = torch.empty((m, k), dtype=gy.dtype, device=gy.device) if want_dx else None
-    dw = torch.empty((n, k), dtype=gy.dtype, device=gy.device) if want_dw else None
-    db = torch.empty(n, dtype=gy.dtype, device=gy.device) if want_db else None
+    dx = gy.new_empty((m, k)) if want_dx else None
+    dw = gy.new_empty((n, k)) if want_dw else None
+    db = gy.new_empty(n) if want_db else None
     args.dx, args.dw, args.db = native.ptr(dx), native.ptr(dw), native.ptr(db)
     nbytes = _backward_workspace_bytes(m, n, k, activation, want_dx, want_dw, want_db)
     workspace = None
@@ -252,9 +284,9 @@ class _ActGrad2(_Fused):
         raise NativeError("dense.linear: third derivatives are not supported")
 
 
-# below this many flops a product takes less time than finding out whether its
-# result was asked for (a few microseconds per input, on the host)
-_SMALL_FLOPS = 4e9
+# below this many flops a product takes less time (15 us) than finding out which
+# results were asked for (8 us per input, on the host)
+_SMALL_FLOPS = 2e10
 
 
 class _Linear(_Fused):
@@ -273,7 +305,7 @@ class _Linear(_Fused):
         else:
             # the operands as the products read them: x and w themselves, or
             # copies whose rows start on 16-byte boundaries
-            ctx.operands = x_op, w_op = _operand(x), _operand(w)
+            ctx.operands = x_op, w_op = _operands(x, w)
             y, z = _forward(x_op, w_op, ctx.save, b, activation, r, keep_z, x)
         ctx.save_for_backward(x, w, z)
         ctx.inputs = (True, True, b is not None)

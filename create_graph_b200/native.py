@@ -275,6 +275,7 @@ _SIGNATURES = {
     "cg_linear_half_workspace_bytes": (i64, [ctypes.POINTER(LinearArgs)]),
     "cg_linear_half_backward": (_I, [ctypes.POINTER(LinearBackwardArgs), vp]),
     "cg_linear_half_backward_workspace_bytes": (i64, [ctypes.POINTER(LinearBackwardArgs)]),
+    "cg_pad_rows_half": (_I, [vp, i64, i64, i64, vp, i64, vp, i64, i64, i64, vp, i64, vp]),
     "cg_act_grad_half": (_I, [ctypes.POINTER(ActGradArgs), vp]),
     "cg_act_grad_half_scratch_bytes": (i64, [i64, i64]),
     "cg_act_grad2_half": (_I, [vp, vp, vp, vp, vp, vp, i64, i64, _I, _I, vp]),

@@ -281,6 +281,14 @@ int cg_linear_half(const cg_linear_args* args, void* stream);
 /* Workspace bytes cg_linear_half needs for these args (0: no split). */
 int64_t cg_linear_half_workspace_bytes(const cg_linear_args* args);
 
+/* Copies of one or two half-precision matrices (2-byte values, any alignment
+ * and pitch) with rows on 16-byte boundaries, what cg_linear_half reads:
+ * dst[r * ld_dst + c] = src[r * ld_src + c]; dst 16-byte aligned, ld_dst a
+ * multiple of 8 values, columns up to it zeroed. rows2 = 0: one matrix. */
+int cg_pad_rows_half(const void* src, int64_t ld_src, int64_t rows, int64_t cols, void* dst, int64_t ld_dst,
+                     const void* src2, int64_t ld_src2, int64_t rows2, int64_t cols2, void* dst2, int64_t ld_dst2,
+                     void* stream);
+
 /* gz = gy f'(z) and db[c] = sum over rows of gz, in one pass. gz NULL: gz is
  * gy itself (no activation) and only db is formed; db NULL: only gz. */
 typedef struct cg_act_grad_args {
