@@ -595,7 +595,7 @@ static Plan search_plan(const cg_linear_args* g, int count) {
     double slice, wave, once;
   };
   static const Shape shapes[] = {
-      {2, 256, 340, 1550, 3900}, {2, 128, 240, 900, 3900}, {1, 128, 260, 800, 3400}, {1, 64, 260, 700, 3200}};
+      {2, 256, 340, 1550, 3900}, {2, 192, 270, 1300, 3900}, {2, 128, 240, 900, 3900}, {1, 128, 260, 800, 3400}, {1, 64, 260, 700, 3200}};
   const int kMost = 24;
   int64_t kts[2] = {1, 1};
   for (int i = 0; i < count; ++i) kts[i] = ceil_div<int64_t>(g[i].k, half::kBK);
@@ -728,6 +728,7 @@ template <class E>
 static int launch_plan(const cg_linear_args* g, int count, const Plan& p, const EpiArgs* ea, bool bf16,
                        cudaStream_t s) {
   if (p.cg == 2 && p.bn == 256) return launch<2, 256, E>(g, count, p, ea, bf16, s);
+  if (p.cg == 2 && p.bn == 192) return launch<2, 192, E>(g, count, p, ea, bf16, s);
   if (p.cg == 2) return launch<2, 128, E>(g, count, p, ea, bf16, s);
   if (p.bn == 128) return launch<1, 128, E>(g, count, p, ea, bf16, s);
   return launch<1, 64, E>(g, count, p, ea, bf16, s);

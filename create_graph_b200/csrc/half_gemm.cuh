@@ -225,14 +225,16 @@ template <int CG, int BN, int PLANES, class Epi>
 struct Tile {
   static constexpr int kBRows = BN / CG;                       // B rows this CTA stages
   static constexpr int kA = kRows * kBK * 2;
-  static constexpr int kB = kBRows * kBK * 2;
+  static constexpr int kBBlocks = (kBRows + 63) / 64;          // 64-wide boxes of an MN-major operand
+  static constexpr int kB = kBBlocks * 64 * kBK * 2;
   static constexpr int kStage = PLANES * (kA + kB);
   static constexpr int kStaging = Epi::kWarps * Epi::kStagingBytes;  // the epilogue warps' own blocks
   static constexpr int kStagesFit = (227 * 1024 - kStaging - 1024 - 512) / kStage;
   static constexpr int kStages = kStagesFit < 8 ? kStagesFit : 8;
   static constexpr int kBytes = kStages * kStage + kStaging + 1024 /*alignment*/ + 512 /*barriers*/;
-  static constexpr uint32_t kTmemCols = 2 * BN;
-  static_assert(kBRows % 64 == 0, "MN-major boxes are 64 wide");
+  static constexpr uint32_t kAccCols = BN <= 64 ? 64 : BN <= 128 ? 128 : 256;  // of one accumulator
+  static constexpr uint32_t kTmemCols = 2 * kAccCols;
+  static_assert(kBRows % 32 == 0, "rows of B");
   static_assert(kStages >= 3 && kTmemCols <= 512, "tile");
 };
 
@@ -420,13 +422,15 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
       const int kt1 = item.kt1, z0 = item.batch * PLANES;
       const bool a_mn = g.a_mn != 0, b_mn = g.b_mn != 0;
       const CUtensorMap *map_a = &g.map_a, *map_b = &g.map_b;
+      // a K-major B brings its own rows, an MN-major one whole boxes
+      const uint32_t stage_bytes = CG * PLANES * (T::kA + (b_mn ? T::kB : T::kBRows * kBK * 2));
       for (int kt = item.kt0; kt < kt1; ++kt, ++it) {
         const int s = it % STAGES;
         const uint32_t round = it / STAGES;
         if (it >= STAGES && !(ok = wait(&empty[s], (round - 1) & 1, error_word))) break;
         const int k0 = kt * kBK;
         if (issuer) {
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * T::kStage);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], stage_bytes);
 #pragma unroll
           for (int p = 0; p < PLANES; ++p) {
             unsigned char* sa = tiles + s * T::kStage + p * (T::kA + T::kB);
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
               tma_load_3d<CG>(sb, map_b, &full[s], k0, n0, z0 + p);
             } else {
 #pragma unroll
-              for (int c = 0; c < T::kBRows / 64; ++c)
+              for (int c = 0; c < T::kBBlocks; ++c)
                 tma_load_3d<CG>(sb + c * (kBK * 128), map_b, &full[s], n0 + 64 * c, k0, z0 + p);
             }
           }
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
         const int kt1 = kt0 + per < item.kt1 ? kt0 + per : item.kt1;
         if (use > 0 && !(ok = wait(&acc_empty[b], (use - 1) & 1, error_word))) break;
         tc_fence_after();
-        const uint32_t acc = tmem + b * BN;
+        const uint32_t acc = tmem + b * T::kAccCols;
         for (int kt = kt0; kt < kt1; ++kt, ++it) {
           const int s = it % STAGES;
           if (!(ok = wait(&full[s], (it / STAGES) & 1, error_word))) break;
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
 #pragma unroll
           for (int q = 0; q < 2 * NB; ++q) {
             float v[16];
-            tmem_load_16(tmem + b * BN + ((uint32_t)(quarter * 32) << 16) + c_first + STEP * (q / 2) + 16 * (q % 2), v);
+            tmem_load_16(tmem + b * T::kAccCols + ((uint32_t)(quarter * 32) << 16) + c_first + STEP * (q / 2) + 16 * (q % 2), v);
 #pragma unroll
             for (int x = 0; x < 16; ++x) sum[q / 2][16 * (q % 2) + x] += v[x];
           }
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
         // 64-column blocks turn, turn + WARPS / 4, ..
         constexpr int STEP = 16 * WARPS;
         const int b = j & 1;
-        const uint32_t acc = tmem + b * BN + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t acc = tmem + b * T::kAccCols + ((uint32_t)(quarter * 32) << 16);
         if (64 * turn < BN) epi.fetch(item.n0 + 64 * turn);  // beside the wait for the accumulator
         if (!(ok = wait(&acc_full[b], (j >> 1) & 1, error_word))) break;
         tc_fence_after();
