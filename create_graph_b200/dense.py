@@ -264,20 +264,23 @@ class _ActGrad(_Fused):
         return *_ActGrad2.apply(h, hb, gy, z, ctx.activation), None, None
 
 
+def _act_grad2(h: Tensor | None, hb: Tensor | None, gy: Tensor, z: Tensor, activation: int):
+    """((h + hb) f'(z), (h + hb) gy f''(z)); either cotangent may be None."""
+    h = None if h is None else h.contiguous()
+    hb = None if hb is None else hb.contiguous()
+    gy, z = gy.contiguous(), z.contiguous()
+    dgy, dz = torch.empty_like(gy), torch.empty_like(z)
+    native.invoke("cg_act_grad2_half", native.ptr(h), native.ptr(hb), gy.data_ptr(), z.data_ptr(), dgy.data_ptr(),
+                  dz.data_ptr(), gy.shape[0], gy.shape[1], activation, native.HALF_DTYPES[gy.dtype], _stream(gy))
+    return dgy, dz
+
+
 class _ActGrad2(_Fused):
-    """(dgy, dz) = ((h + hb) f'(z), (h + hb) gy f''(z)): the last derivative the
-    force training needs."""
+    """_act_grad2: the last derivative the force training needs."""
 
     @staticmethod
     def forward(ctx, h, hb, gy, z, activation):
-        h = None if h is None else h.contiguous()
-        hb = None if hb is None else hb.contiguous()
-        gy, z = gy.contiguous(), z.contiguous()
-        dgy, dz = torch.empty_like(gy), torch.empty_like(z)
-        native.invoke("cg_act_grad2_half", native.ptr(h), native.ptr(hb), gy.data_ptr(), z.data_ptr(),
-                      dgy.data_ptr(), dz.data_ptr(), gy.shape[0], gy.shape[1], activation,
-                      native.HALF_DTYPES[gy.dtype], _stream(gy))
-        return dgy, dz
+        return _act_grad2(h, hb, gy, z, activation)
 
     @staticmethod
     def backward(ctx, *grads):
@@ -390,7 +393,10 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation:
 
 
 class Linear(nn.Module):
-    """A half-precision layer y = f(x W^T + b) + r, initialised as torch.nn.Linear."""
+    """A half-precision layer y = f(x W^T + b) + r, initialised as
+    torch.nn.Linear. The parameters are kept in float32, as the optimizers and
+    ``ddp.FlatGradients`` want them, and rounded to ``dtype`` for each product;
+    their gradients come back as float32."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "none",
                  dtype: torch.dtype = torch.bfloat16, device=None):
@@ -399,10 +405,10 @@ class Linear(nn.Module):
             raise NativeError(f"dense.Linear: float16 or bfloat16 expected, got {dtype}")
         if activation not in ACTIVATIONS:
             raise NativeError(f"dense.Linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-        self.activation = activation
-        like = nn.Linear(in_features, out_features, bias=bias, device=device)
-        self.weight = nn.Parameter(like.weight.detach().to(dtype))
-        self.bias = nn.Parameter(like.bias.detach().to(dtype)) if bias else None
+        self.activation, self.dtype = activation, dtype
+        like = nn.Linear(in_features, out_features, bias=bias, device=device, dtype=torch.float32)
+        self.weight, self.bias = like.weight, like.bias
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
-        return linear(x, self.weight, self.bias, activation=self.activation, residual=residual)
+        bias = None if self.bias is None else self.bias.to(self.dtype)
+        return linear(x, self.weight.to(self.dtype), bias, activation=self.activation, residual=residual)

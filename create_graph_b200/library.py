@@ -19,6 +19,11 @@ too and the chains that create_graph differentiates twice stay differentiable:
     segment_sum_csr / gather_csr            each other's backward
     edge_geom -> edge_geom_bwd1 -> edge_geom_bwd2   (pos -> rbf, env)
     neighbor_list                           integer outputs, no gradient
+    dense_linear(x, w, b, r, activation) = (f(z) + r, z), z = x w^T + b
+                                            backward: act_grad, dense_linear
+    act_grad(gy, z, activation) = (gy f'(z), its column sums)
+                                            backward: act_grad2
+    newton_schulz                           orthogonalised matrices, no gradient
     edge_attn, edge_attn_tf32               registered by create_graph_b200.edge_attn
 
 CSR arguments are (index, row_ptr, perm, rows) as in ``nn.Csr``; neighbour
@@ -32,8 +37,9 @@ import ctypes
 import torch
 from torch import Tensor
 
-from create_graph_b200 import native
+from create_graph_b200 import dense, native
 from create_graph_b200 import nn as cgnn
+from create_graph_b200 import optim
 from create_graph_b200.gemm import ACT_SILU
 
 
@@ -364,3 +370,104 @@ def _neighbor_list_fake(pos, sys_ptr, max_atoms, cutoff, k):
     i32 = torch.int32
     return _empty(pos, n, k, dtype=i32), _empty(pos, n, dtype=i32), _empty(pos, n + 1, dtype=i32), _empty(
         pos, max(n * k, 1), dtype=i32)
+
+
+# ---------------------------------------------------------------------------
+# the half-precision dense layer and the matrix optimizer's products
+# ---------------------------------------------------------------------------
+
+
+@torch.library.custom_op("cg_b200::dense_linear", mutates_args=())
+def dense_linear(x: Tensor, w: Tensor, b: Tensor | None, r: Tensor | None, activation: str) -> tuple[Tensor, Tensor]:
+    """(f(z) + r, z) with z = x @ w.T + b for (M, K) x, in half precision (see
+    create_graph_b200.dense; x and w may be transposed views)."""
+    act = dense._checked(x, w, b, r, activation)
+    return dense.product(x, w, b, act, r, keep_z=True)
+
+
+@dense_linear.register_fake
+def _dense_linear_fake(x, w, b, r, activation):
+    return _empty(x, x.shape[0], w.shape[0]), _empty(x, x.shape[0], w.shape[0])
+
+
+@torch.library.custom_op("cg_b200::act_grad", mutates_args=())
+def act_grad(gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
+    """(gy f'(z), the sums of its columns) of (M, N) half-precision tensors."""
+    gz, db = dense._act_grad(gy, z, dense.ACTIVATIONS[activation], True)
+    return (gy.clone() if gz.data_ptr() == gy.data_ptr() else gz.contiguous()), db
+
+
+@act_grad.register_fake
+def _act_grad_fake(gy, z, activation):
+    return torch.empty_like(gy, memory_format=torch.contiguous_format), _empty(gy, gy.shape[1])
+
+
+@torch.library.custom_op("cg_b200::act_grad2", mutates_args=())
+def act_grad2(h: Tensor, hb: Tensor, gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
+    """((h + hb) f'(z), (h + hb) gy f''(z)) for cotangents h, hb of act_grad's outputs."""
+    return dense._act_grad2(h, hb, gy, z, dense.ACTIVATIONS[activation])
+
+
+@act_grad2.register_fake
+def _act_grad2_fake(h, hb, gy, z, activation):
+    return (torch.empty_like(gy, memory_format=torch.contiguous_format),
+            torch.empty_like(z, memory_format=torch.contiguous_format))
+
+
+def _dense_product(a: Tensor, b: Tensor) -> Tensor:
+    return dense_linear(a, b, None, None, "none")[0]
+
+
+def _dense_linear_setup(ctx, inputs, output):
+    x, w, b, r, activation = inputs
+    ctx.save_for_backward(x, w, output[1])
+    ctx.given = (b is not None, r is not None)
+    ctx.activation = activation
+    ctx.set_materialize_grads(False)
+
+
+def _dense_linear_backward(ctx, gy, gz_direct):
+    x, w, z = ctx.saved_tensors
+    has_b, has_r = ctx.given
+    if gy is None and gz_direct is None:
+        return None, None, None, None, None
+    gz = db = None
+    if gy is not None:
+        gz, db = act_grad(gy, z, ctx.activation)
+    if gz_direct is not None:
+        gz = gz_direct if gz is None else gz + gz_direct
+        db = act_grad(gz, z, "none")[1]
+    dx = _dense_product(gz, w.t()) if ctx.needs_input_grad[0] else None
+    dw = _dense_product(gz.t(), x.t()) if ctx.needs_input_grad[1] else None
+    return dx, dw, db if has_b else None, gy if has_r else None, None
+
+
+dense_linear.register_autograd(_dense_linear_backward, setup_context=_dense_linear_setup)
+
+
+def _act_grad_setup(ctx, inputs, output):
+    gy, z, activation = inputs
+    ctx.save_for_backward(gy, z)
+    ctx.activation = activation
+    ctx.set_materialize_grads(True)
+
+
+def _act_grad_backward(ctx, h, hb):
+    gy, z = ctx.saved_tensors
+    return *act_grad2(h, hb, gy, z, ctx.activation), None
+
+
+act_grad.register_autograd(_act_grad_backward, setup_context=_act_grad_setup)
+
+
+@torch.library.custom_op("cg_b200::newton_schulz", mutates_args=())
+def newton_schulz(x: Tensor, steps: int = 5, a: float = optim.NS_COEFFICIENTS[0], b: float = optim.NS_COEFFICIENTS[1],
+                  c: float = optim.NS_COEFFICIENTS[2], eps: float = 1e-7) -> Tensor:
+    """optim.newton_schulz (no gradient)."""
+    with torch.no_grad():
+        return optim.newton_schulz(x.detach(), steps, (a, b, c), eps)
+
+
+@newton_schulz.register_fake
+def _newton_schulz_fake(x, steps=5, a=0.0, b=0.0, c=0.0, eps=1e-7):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)

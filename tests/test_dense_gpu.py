@@ -258,3 +258,29 @@ def test_refusals():
     args.lda, args.a = 8, x.data_ptr() + 2
     with pytest.raises(NativeError, match="aligned"):
         native.invoke("cg_linear_half", args, 0)
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+def test_library_operators(act):
+    """torch.ops.cg_b200.dense_linear, differentiated twice, and newton_schulz."""
+    import create_graph_b200.library  # noqa: F401
+    from create_graph_b200.optim import newton_schulz
+
+    dtype = torch.float16
+    x, w, b, r, gy = tensors(72, 40, 24, dtype, seed=11)
+    v = torch.randn(72, 24, generator=torch.Generator().manual_seed(12)).to(dtype).cuda()
+
+    def run(f, x, w, b, r, gy, v):
+        y = f(x, w, b, r)
+        dx, dw, db, dr = torch.autograd.grad(y, (x, w, b, r), gy, create_graph=True)
+        second = torch.autograd.grad((dx * v).sum(), (w, gy), allow_unused=True)
+        return y, dx, dw, db, dr, *second
+
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b, r, gy)]
+    got = run(lambda x, w, b, r: torch.ops.cg_b200.dense_linear(x, w, b, r, act)[0], *leaves, v)
+    ref = doubled(x, w, b, r, gy)
+    want = run(lambda *t: formula(*t, act), *ref, v.double().cpu())
+    for i, (g, e) in enumerate(zip(got, want)):
+        assert rel(g.detach(), e.detach()) < (1.1 if i == 0 else 3.0 if i < 5 else 8.0) * UNIT[dtype], i
+    m = torch.randn(30, 20, device="cuda")
+    assert torch.equal(torch.ops.cg_b200.newton_schulz(m), newton_schulz(m))
