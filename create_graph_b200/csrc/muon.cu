@@ -33,7 +33,7 @@ __device__ int g_muon_error = 0;
 
 constexpr int kGroups = 8;         // shapes per launch
 constexpr int kEntries = 24;       // runs of matrices per prepare launch
-constexpr int kChunk = 8192;       // elements per block of the prepare passes
+constexpr int kMostChunk = 8192;   // elements per block of the prepare passes
 constexpr float kScale = 4096.0f;  // of the stored planes
 
 struct OutRef {
@@ -51,6 +51,7 @@ struct Run {
   int64_t ld_x, ld_momentum, ld_out, stride_x, stride_out;
   int rows, cols, pitch, count;
   int first_chunk, chunks;  // chunks of one matrix
+  half::Divisor by_cols;
   int first_matrix;         // its place in the table of outputs
   int vec;                  // groups of four along the rows
 };
@@ -60,6 +61,7 @@ struct Prepare {
   int runs;
   float eps, mu;
   int nesterov;
+  int chunk;                // elements per block
   double* partial;
   OutRef* table;
 };
@@ -105,16 +107,17 @@ struct Momentum {
   __device__ float update(float m, float g) const { return nesterov ? m + (1.0f - mu) * (g - m) : m; }
 };
 
-// Sum over the block in a fixed order.
+// Sum over a block of WARPS warps in a fixed order.
+template <int WARPS>
 __device__ inline double block_sum(double s) {
-  __shared__ double sums[8];
+  __shared__ double sums[WARPS];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_down_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
   __syncthreads();
   s = 0.0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) s += sums[w];
+  for (int w = 0; w < WARPS; ++w) s += sums[w];
   return s;
 }
 
@@ -142,8 +145,10 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
   const T* x = static_cast<const T*>(run.x) + matrix * run.stride_x;
   float* mom = MOMENTUM ? run.momentum : nullptr;
   const Momentum rule = {p.mu, p.nesterov};
-  const int64_t n = (int64_t)run.rows * run.cols;
-  const int64_t e0 = (int64_t)chunk * kChunk, e1 = e0 + kChunk < n ? e0 + kChunk : n;
+  // the chunk's first place; the others follow by 32-bit steps
+  const int64_t n = (int64_t)run.rows * run.cols, e0 = (int64_t)chunk * p.chunk;
+  const int row0 = (int)(e0 / run.cols), col0 = (int)(e0 - (int64_t)row0 * run.cols);
+  const int size = (int)(e0 + p.chunk < n ? p.chunk : n - e0);
   double sum = 0.0;
   float scale = 0.0f;
   __half *hi = nullptr, *lo = nullptr;
@@ -156,7 +161,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     double s = 0.0;
     const double* part = p.partial + run.first_chunk + (int64_t)matrix * run.chunks;
     for (int c = threadIdx.x; c < run.chunks; c += 256) s += part[c];
-    s = block_sum(s);
+    s = block_sum<8>(s);
     const double norm = sqrt(s);
     scale = (float)(kScale / (norm > (double)p.eps ? norm : (double)p.eps));
     if (isnan(s)) scale = __int_as_float(0x7fc00000);
@@ -165,12 +170,12 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
   }
   if (run.vec) {
 #pragma unroll 2
-    for (int64_t e = e0 + 4 * threadIdx.x; e < e1; e += 4 * 256) {
-      const int row = (int)(e / run.cols), col = (int)(e % run.cols);
+    for (int e = 4 * threadIdx.x; e < size; e += 4 * 256) {
+      const int down = run.by_cols.div(col0 + e), row = row0 + down, col = col0 + e - down * run.cols;
       float v[4];
-      load_four(x + row * run.ld_x + col, v);
+      load_four(x + (int64_t)row * run.ld_x + col, v);
       if (MOMENTUM) {
-        float4* mp = reinterpret_cast<float4*>(mom + row * run.ld_momentum + col);
+        float4* mp = reinterpret_cast<float4*>(mom + (int64_t)row * run.ld_momentum + col);
         float4 m = *mp;
         if (NORM) {
           m = make_float4(rule.next(m.x, v[0]), rule.next(m.y, v[1]), rule.next(m.z, v[2]), rule.next(m.w, v[3]));
@@ -198,11 +203,12 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
       }
     }
   } else {
-    for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
-      const int row = (int)(e / run.cols), col = (int)(e % run.cols);
-      float v = load_value(x + row * run.ld_x + col);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < size; e += 256) {
+      const int down = run.by_cols.div(col0 + e), row = row0 + down, col = col0 + e - down * run.cols;
+      float v = load_value(x + (int64_t)row * run.ld_x + col);
       if (MOMENTUM) {
-        float* mp = mom + row * run.ld_momentum + col;
+        float* mp = mom + (int64_t)row * run.ld_momentum + col;
         float m = *mp;
         if (NORM) *mp = m = rule.next(m, v);
         v = rule.update(m, v);
@@ -219,7 +225,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     }
   }
   if (NORM) {
-    sum = block_sum(sum);
+    sum = block_sum<8>(sum);
     if (threadIdx.x == 0) p.partial[blockIdx.x] = sum;
   }
 }
@@ -486,7 +492,7 @@ static int gather_shapes(const cg_ns_args& g, int from, Shape* shapes, int* to) 
   return n;
 }
 
-static int64_t chunks_of(int64_t rows, int64_t cols) { return ceil_div<int64_t>(rows * cols, kChunk); }
+static int64_t chunks_of(int64_t rows, int64_t cols, int chunk) { return ceil_div<int64_t>(rows * cols, chunk); }
 
 enum Step { kGram, kPoly, kUpdate };
 
@@ -559,11 +565,16 @@ struct Buffers {
   float4* partial;
   unsigned* counters;
   int64_t counter_bytes;
+  int chunk;  // elements per block of the prepare passes
 };
 
 // Lay the set's buffers out from `base`; returns the bytes they take.
 static int64_t layout(Shape* shapes, int n, char* base, Buffers* b) {
-  int64_t at = 0, matrices = 0, chunks = 0;
+  int64_t at = 0, matrices = 0, chunks = 0, elements = 0;
+  for (int i = 0; i < n; ++i) elements += shapes[i].count * shapes[i].rows * shapes[i].cols;
+  // enough blocks to fill the SMs several times where there are few elements
+  const int64_t per = up(ceil_div<int64_t>(elements, (int64_t)sm_count() * 8), 1024);
+  b->chunk = (int)(per < kMostChunk ? per : kMostChunk);
   auto take = [&](int64_t bytes) {
     char* p = base == nullptr ? nullptr : base + at;
     at += up(bytes, kAlign);
@@ -576,7 +587,7 @@ static int64_t layout(Shape* shapes, int n, char* base, Buffers* b) {
     h.spitch = up(h.s, 8);
     h.first_matrix = matrices;
     matrices += h.count;
-    chunks += h.count * chunks_of(h.rows, h.cols);
+    chunks += h.count * chunks_of(h.rows, h.cols, b->chunk);
     const int64_t x = h.count * 2 * h.rows * h.pitch * 2, s = h.count * 2 * h.s * h.spitch * 2;
     h.x0 = reinterpret_cast<__half*>(take(x));
     h.x1 = reinterpret_cast<__half*>(take(x));
@@ -623,6 +634,7 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
     p.mu = g.momentum;
     p.nesterov = g.nesterov;
     p.table = b.table;
+    p.chunk = b.chunk;
     int64_t chunks = 0;
     auto flush = [&]() -> int {
       if (p.runs == 0) return kOk;
@@ -657,7 +669,8 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
       r.pitch = (int)h.pitch;
       r.count = (int)e.count;
       r.first_chunk = (int)chunks;
-      r.chunks = (int)chunks_of(e.rows, e.cols);
+      r.chunks = (int)chunks_of(e.rows, e.cols, b.chunk);
+      r.by_cols = half::divisor(e.cols);
       r.first_matrix = (int)(h.first_matrix + filled[k]);
       const uintptr_t mask = 4 * sizeof(T) - 1;
       r.vec = e.cols % 4 == 0 && e.ld_x % 4 == 0 && e.stride_x % 4 == 0 &&

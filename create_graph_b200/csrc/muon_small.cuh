@@ -25,7 +25,7 @@ namespace small {
 
 constexpr int kSide = 128;
 constexpr int kMostCluster = 8;
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;  // a warp owns 32 rows x 32 columns of the tile
 constexpr int kPlane = kSide * kSide * 2;  // bytes of one plane of a tile
 constexpr int kRuns = 24;
 constexpr int kGroupsOf4 = kSide * kSide / 4 / kThreads;  // per thread
@@ -143,6 +143,13 @@ __device__ __forceinline__ void blend_row(unsigned char* planes, int row, int co
   }
 }
 
+// 32 values of a row into the fp32 block.
+__device__ __forceinline__ void put_row(float4* part, int row, int col0, const float (&v)[32]) {
+#pragma unroll
+  for (int g = 0; g < 8; ++g)
+    part[part_at(row, col0 / 4 + g)] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+}
+
 template <class T, bool MOMENTUM>
 __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const __grid_constant__ Args p) {
   extern __shared__ unsigned char smem_raw[];
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
       for (int e = 0; e < 4; ++e) sum += (double)u[g][e] * u[g][e];
     }
   }
-  sum = block_sum(sum);
+  sum = block_sum<kThreads / 32>(sum);
   // every CTA's tile in every CTA, added up in rank order
   if (tid < ranks) peer_store_double(peer_address(smem_u32(sums + rank), tid), sum);
   half::cluster_sync_all();
@@ -241,9 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   }
 
   // ---- the steps
-  const int quarter = warp & 3, half_of = warp >> 2;  // TMEM lanes, 64 columns
+  const int quarter = warp & 3, col0 = 32 * (warp >> 2);  // TMEM lanes, 32 columns
   const int row = quarter * 32 + lane;
-  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + half_of * 64;
+  const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + col0;
   uint32_t phase = 0;
   // one product: what the threads wrote is visible to the tensor core, and the
   // accumulator to the threads after it
@@ -265,22 +272,12 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   };
   for (int t = 0; t < p.steps; ++t) {
     product(Z, !wide, Z, !wide);
+    float v[32];
+    tmem_load_32(acc, v);
     if (ranks == 1) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        tmem_load_32(acc + 32 * h, v);
-        blend_row<false, true>(A, row, half_of * 64 + 32 * h, 0.0f, 1.0f / kScale, v);
-      }
+      blend_row<false, true>(A, row, col0, 0.0f, 1.0f / kScale, v);
     } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        tmem_load_32(acc + 32 * h, v);
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          part[part_at(row, half_of * 16 + 8 * h + g)] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-      }
+      put_row(part, row, col0, v);
       half::cluster_sync_all();
       // this rank's share of the 4096 groups of four, from every CTA, to every CTA
       const int share = (kSide * 32 + ranks - 1) / ranks, g0 = rank * share;
@@ -288,19 +285,19 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
       for (int at = g0 + tid; at < g1; at += kThreads) {
         const int r = at >> 5, g = at & 31;
         const uint32_t from = smem_u32(part + part_at(r, g));
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int q = 0; q < ranks; ++q) {
           const float4 f = peer_load4(peer_address(from, q));
-          v[0] += f.x;
-          v[1] += f.y;
-          v[2] += f.z;
-          v[3] += f.w;
+          x[0] += f.x;
+          x[1] += f.y;
+          x[2] += f.z;
+          x[3] += f.w;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= 1.0f / kScale;
+        for (int e = 0; e < 4; ++e) x[e] *= 1.0f / kScale;
         uint2 h, l;
-        split4(v, h, l);
+        split4(x, h, l);
         const uint32_t to = smem_u32(A + plane_at(r, 4 * g));
 #pragma unroll 4
         for (int q = 0; q < ranks; ++q) {
@@ -312,31 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
       half::cluster_sync_all();
     }
     product(A, false, A, false);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[32];
-      tmem_load_32(acc + 32 * h, v);
-      blend_row<true, true>(A, row, half_of * 64 + 32 * h, p.b, p.c / kScale, v);
-    }
+    tmem_load_32(acc, v);
+    blend_row<true, true>(A, row, col0, p.b, p.c / kScale, v);
     if (wide) product(A, false, Z, true);
     else product(Z, false, A, false);
+    tmem_load_32(acc, v);
     if (t + 1 < p.steps) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        tmem_load_32(acc + 32 * h, v);
-        blend_row<true, true>(Z, row, half_of * 64 + 32 * h, p.a, 1.0f / kScale, v);
-      }
+      blend_row<true, true>(Z, row, col0, p.a, 1.0f / kScale, v);
     } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        tmem_load_32(acc + 32 * h, v);
-        blend_row<true, false>(Z, row, half_of * 64 + 32 * h, p.a / kScale, 1.0f / (kScale * kScale), v);
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          part[part_at(row, half_of * 16 + 8 * h + g)] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-      }
+      blend_row<true, false>(Z, row, col0, p.a / kScale, 1.0f / (kScale * kScale), v);
+      put_row(part, row, col0, v);
     }
   }
   tc_fence_before();
