@@ -356,7 +356,8 @@ __device__ __forceinline__ void stage_read8(const float* stage, int r, int c, fl
 // Epi(launch, staging, barrier, lane), begin(group, item, row0), fetch(col0)
 // (starts what the next block reads), store(accumulator, col0) (a block of 32
 // rows: 64 columns from TMEM, or 32 summed ones with PLANES = 2), skip() (after a
-// fetch, when another split finishes the tile), finish(), and
+// fetch, when another split finishes the tile), spread() (the last tile's blocks
+// may use memory of their own), finish(), and
 // error_word() (the translation unit's).
 template <int CG, int BN, int PLANES, class Epi>
 __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
@@ -590,10 +591,15 @@ __global__ void __launch_bounds__(threads_of(Epi::kWarps), 1)
             }
           }
         }
+        // a CTA's last tile leaves through the ring, which nothing uses any more
+        const bool final = w + step >= L.items;
+        static_assert(STAGES * T::kStage / WARPS >= 6 * Epi::kStagingBytes, "room of spread()");
+        if (final)
+          ok = epi.spread(tiles + e * (STAGES * T::kStage / WARPS), item.n0 + c_first, STEP, NB, error_word);
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
-          if (!(ok = ok && epi.store(sum[q], item.n0 + c_first + STEP * q, error_word))) break;
-          if (q + 1 < NB) epi.fetch(item.n0 + c_first + STEP * (q + 1));
+          if (!(ok = ok && epi.store(sum[q], item.n0 + c_first + STEP * q, q, error_word))) break;
+          if (!final && q + 1 < NB) epi.fetch(item.n0 + c_first + STEP * (q + 1));
         }
       } else {
         // 64-column blocks turn, turn + WARPS / 4, ..

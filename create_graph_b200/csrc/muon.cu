@@ -255,12 +255,15 @@ struct EpiBase {
   using L = half::Launch<EpiArgs, kGroups>;
   static constexpr int kWarps = 8;
   static constexpr int kStagingBytes = 2 * 32 * 64;
+  static constexpr int kBlock = kStagingBytes;
   const EpiArgs* a;
   unsigned char* staging;
+  unsigned char* room = nullptr;  // six blocks more, for the last tile
   uint64_t* bar;
   uint32_t loads = 0;
   int lane, m, n, batch, row0;
   bool pending = false;  // a load has been started and not waited for
+  bool later = false;    // the same of the last tile's blocks after its first
   __device__ EpiBase(const L&, unsigned char* staging_, uint64_t* bar_, int lane_)
       : staging(staging_), bar(bar_), lane(lane_) {}
   static __device__ int* error_word() { return &g_muon_error; }
@@ -299,22 +302,54 @@ struct EpiBase {
     return ok;
   }
   __device__ __forceinline__ void skip() { arrived(error_word()); }
+  // Memory of the tile's block q: the staging block, or in the last tile one of
+  // its own, so that no block waits for the one before it to leave (gram of
+  // 12 x 768 x 768: SPREADFIG).
+  __device__ __forceinline__ unsigned char* block(int q) const {
+    return room == nullptr || q == 0 ? staging : room + (2 * q - 1) * kBlock;
+  }
+  // The last tile: start what blocks 1 .. count - 1 read, all at once.
+  __device__ __forceinline__ bool spread(unsigned char* room_, int col0, int step, int count, int* error) {
+    room = room_;
+    const bool ok = arrived(error);
+    if (!a->has_aux) return ok;
+    int loads_now = 0;
+    for (int q = 1; q < count; ++q) loads_now += !outside(col0 + step * q);
+    if (loads_now == 0) return ok;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bar, loads_now * kBlock);
+      for (int q = 1; q < count; ++q) {
+        const int col = col0 + step * q;
+        if (outside(col)) continue;
+        half::tma_load_3d<1>(block(q), &a->map_aux, bar, col, row0, 2 * batch);
+        half::tma_load_3d<1>(block(q) + 2048, &a->map_aux, bar, col, row0, 2 * batch + 1);
+      }
+    }
+    later = true;
+    __syncwarp();
+    return ok;
+  }
   // 16-byte group c (8 values) of row r of plane p
-  __device__ __forceinline__ uint4* group(int p, int r, int c) const {
-    return reinterpret_cast<uint4*>(staging + p * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  __device__ __forceinline__ static uint4* group(unsigned char* at, int p, int r, int c) {
+    return reinterpret_cast<uint4*>(at + p * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
   }
   // v <- alpha aux + beta v
-  __device__ __forceinline__ bool values(float (&v)[32], int* error) {
+  __device__ __forceinline__ bool values(float (&v)[32], int q, int* error) {
     const float alpha = a->alpha, beta = a->beta;
     if (!a->has_aux) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] *= beta;
       return true;
     }
+    if (q > 0 && later) {
+      pending = true;
+      later = false;
+    }
     const bool ok = arrived(error);
+    unsigned char* at = block(q);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 h = *group(0, lane, c), l = *group(1, lane, c);
+      const uint4 h = *group(at, 0, lane, c), l = *group(at, 1, lane, c);
       const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -328,20 +363,34 @@ struct EpiBase {
   }
 };
 
+// Four 8 x 8 matrices of 16-bit values: lane l gives the address of row l & 7 of
+// matrix l >> 3. Read transposed, and written as they are held.
+__device__ __forceinline__ void load_transposed(const void* row, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(smem_u32(row))
+               : "memory");
+}
+__device__ __forceinline__ void store_matrices(void* row, const uint32_t (&v)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
 // The result as planes, for the next product.
 struct SplitEpi : EpiBase {
   using EpiBase::EpiBase;
-  __device__ __forceinline__ void put(int col, int row) {
+  __device__ __forceinline__ void put(unsigned char* at, int col, int row) {
     fence_proxy_async_shared();
     __syncwarp();
     if (lane == 0) {
-      half::tma_store_3d(&a->map_out, staging, col, row, 2 * batch);
-      half::tma_store_3d(&a->map_out, staging + 2048, col, row, 2 * batch + 1);
+      half::tma_store_3d(&a->map_out, at, col, row, 2 * batch);
+      half::tma_store_3d(&a->map_out, at + 2048, col, row, 2 * batch + 1);
     }
   }
-  __device__ __forceinline__ bool store(float (&v)[32], int col0, int* error) {
+  __device__ __forceinline__ bool store(float (&v)[32], int col0, int q, int* error) {
     if (outside(col0)) return true;
-    const bool ok = values(v, error);
+    const bool ok = values(v, q, error);
     if (a->diagonal != 0.0f && row0 == col0) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] += e == lane ? a->diagonal : 0.0f;
@@ -356,22 +405,31 @@ struct SplitEpi : EpiBase {
       hi[i] = *reinterpret_cast<const uint32_t*>(&h);
       lo[i] = *reinterpret_cast<const uint32_t*>(&l);
     }
+    unsigned char* at = block(q);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      *group(0, lane, c) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-      *group(1, lane, c) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+      *group(at, 0, lane, c) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+      *group(at, 1, lane, c) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
     }
-    put(col0, row0);
-    if (a->lower && row0 != col0) {  // the mirror block: value c of this row is value `lane` of its row c
-      if (lane == 0) half::tma_store_wait_read();
-      __syncwarp();
+    put(at, col0, row0);
+    if (a->lower && row0 != col0) {  // the mirror block, transposed 8 x 8 values at a time
+      uint32_t t[2][4][4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint32_t h = hi[i / 2], l = lo[i / 2];
-        reinterpret_cast<uint16_t*>(group(0, i, lane >> 3))[lane & 7] = (uint16_t)(i % 2 ? h >> 16 : h);
-        reinterpret_cast<uint16_t*>(group(1, i, lane >> 3))[lane & 7] = (uint16_t)(i % 2 ? l >> 16 : l);
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) load_transposed(group(at, p, lane, g), t[p][g]);
+      if (room != nullptr && q < 3) {
+        at = room + 2 * q * kBlock;
+      } else {  // in the staging block, once it has left
+        at = staging;
+        if (lane == 0) half::tma_store_wait_read();
+        __syncwarp();
       }
-      put(row0, col0);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) store_matrices(group(at, p, 8 * g + (lane & 7), lane >> 3), t[p][g]);
+      put(at, row0, col0);
     }
     return ok;
   }
@@ -417,10 +475,10 @@ struct FinalEpi : EpiBase {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
   }
   // rows of the caller's matrices: fp32 blocks through shared memory
-  __device__ __forceinline__ bool store(float (&v)[32], int col0, int* error) {
+  __device__ __forceinline__ bool store(float (&v)[32], int col0, int q, int* error) {
     if (outside(col0)) return true;
-    const bool ok = values(v, error);
-    float* stage = reinterpret_cast<float*>(staging);
+    const bool ok = values(v, q, error);
+    float* stage = reinterpret_cast<float*>(block(q));
     __syncwarp();  // every row of the planes has been read
 #pragma unroll
     for (int q = 0; q < 8; ++q)
