@@ -195,6 +195,49 @@ __device__ __forceinline__ float2 gelu2(float2 z) {
   return fma2(make_float2(z.x + fabsf(z.x), z.y + fabsf(z.y)), both(0.5f), make_float2(-w.x, -w.y));
 }
 
+// f' of two values, as act_grad.
+__device__ __forceinline__ float2 silu_grad2(float2 z) {
+  const float2 x = mul2(z, both(-kLog2e));
+  const float2 e = make_float2(exp2_approx(fminf(x.x, 60.0f)), exp2_approx(fminf(x.y, 60.0f)));
+  const float2 s = rcp2(make_float2(1.0f + e.x, 1.0f + e.y));
+  // s (1 + z (1 - s)) = s + (z s - z s s)
+  const float2 zs = mul2(z, s);
+  return fma2(fma2(zs, make_float2(-s.x, -s.y), zs), both(1.0f), s);
+}
+__device__ __forceinline__ float2 gelu_grad2(float2 z) {
+  const float2 a = make_float2(fminf(fabsf(z.x), 64.0f), fminf(fabsf(z.y), 64.0f));
+  const float2 t = rcp2(fma2(a, both(0.3275911f * 0.70710678f), both(1.0f)));
+  const float2 u = mul2(mul2(a, a), both(-0.5f * kLog2e));
+  const float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
+  float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+  p = fma2(t, p, both(0.7107068705f));
+  p = fma2(t, p, both(-0.142248368f));
+  p = fma2(t, p, both(0.127414796f));
+  const float2 tail = mul2(mul2(p, t), e);
+  // Phi(z) = 1/2 + sign(z) (1/2 - tail)
+  const float2 phi = make_float2(0.5f + copysignf(0.5f - tail.x, z.x), 0.5f + copysignf(0.5f - tail.y, z.y));
+  return fma2(mul2(z, both(kInvSqrt2Pi)), e, phi);
+}
+// g <- g f'(z); the branch on the kind is outside the loop.
+template <int N>
+__device__ __forceinline__ void act_grad_all(float (&g)[N], const float (&z)[N], int kind) {
+  if (kind == CG_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] = z[e] > 0.0f ? g[e] : 0.0f * g[e];
+  } else if (N % 2 == 0 && (kind == CG_ACT_SILU || kind == CG_ACT_GELU)) {
+#pragma unroll
+    for (int e = 0; e + 1 < N; e += 2) {
+      const float2 x = make_float2(z[e], z[e + 1]);
+      const float2 d = kind == CG_ACT_SILU ? silu_grad2(x) : gelu_grad2(x);
+      g[e] *= d.x;
+      g[e + 1] *= d.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) g[e] *= act_grad(z[e], kind);
+  }
+}
+
 // f applied to a thread's values; the branch on the kind is outside the loop.
 template <int N>
 __device__ __forceinline__ void act_all(float (&v)[N], int kind) {
@@ -493,8 +536,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
         if (gz) x[0] = to_float(z[r * ld_z + col]);
       }
       if (gz) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) g[e] *= act_grad(x[e], kind);
+        act_grad_all(g, x, kind);
         if constexpr (V == 8) *reinterpret_cast<uint4*>(gz + r * ld_gz + col) = pack8<T>(g);
         else gz[r * ld_gz + col] = from_float<T>(g[0]);
       }

