@@ -59,50 +59,48 @@ def _stream(t: Tensor) -> int:
 
 
 def _in_place(t: Tensor):
-    """(tensor, row pitch, MN-major) of a logical (rows, K) operand that the
+    """(None, row pitch, MN-major) of a logical (rows, K) operand that the
     products can read as it is stored; None when its rows need copying."""
     if t.is_contiguous():  # the usual case, in few steps
         k = t.shape[1]
         if k % 8 == 0 and t.data_ptr() % 16 == 0:
-            return t, k, False
+            return None, k, False
     if _fits_tma(t, 0, 1):
-        return t, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8, False
+        return None, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8, False
     if _fits_tma(t, 1, 0):
-        return t, t.stride(1) if t.shape[1] > 1 else -(-t.shape[0] // 8) * 8, True
+        return None, t.stride(1) if t.shape[1] > 1 else -(-t.shape[0] // 8) * 8, True
     return None
 
 
-def _operands(*ts: Tensor) -> list:
-    """_in_place of each of one or two operands, those that need it copied into
-    one padded buffer by one launch (in their own layout: a transposed view
-    stays transposed)."""
+def _operands(*ts: Tensor) -> tuple[list, Tensor | None]:
+    """How the products read one or two operands, as (offset, row pitch,
+    MN-major) each, and a buffer: an offset of None is the tensor itself, else
+    the place (in values) of its copy in the buffer, with padded rows and in the
+    operand's own layout (a transposed view stays transposed). One launch copies
+    them all."""
     ops = [_in_place(t) for t in ts]
     if None not in ops:
-        return ops
-    todo = []
+        return ops, None
+    todo, at = [], 0
     for i, t in enumerate(ts):
         if ops[i] is None:
             mn = t.stride(0) == 1 and t.stride(1) >= t.shape[0]
             stored = t.t() if mn else _rows(t)
-            todo.append((i, stored, mn, -(-stored.shape[1] // 8) * 8))
-    flat = torch.empty(sum(s.shape[0] * pitch for _, s, _, pitch in todo), dtype=ts[0].dtype, device=ts[0].device)
-    at, args = flat.data_ptr(), []
-    for i, s, mn, pitch in todo:
-        args += [s.data_ptr(), max(s.stride(0), s.shape[1]), s.shape[0], s.shape[1], at, pitch]
-        ops[i] = (_Copy(flat, at), pitch, mn)
-        at += 2 * s.shape[0] * pitch
+            pitch = -(-stored.shape[1] // 8) * 8
+            ops[i] = (at, pitch, mn)
+            todo.append((stored, at, pitch))
+            at += stored.shape[0] * pitch
+    flat = ts[0].new_empty(at)
+    args = []
+    for stored, at, pitch in todo:
+        rows, cols = stored.shape
+        args += [stored.data_ptr(), max(stored.stride(0), cols), rows, cols, flat.data_ptr() + 2 * at, pitch]
     native.invoke("cg_pad_rows_half", *args, *([None, 0, 0, 0, None, 0] if len(todo) == 1 else []), _stream(ts[0]))
-    return ops
+    return ops, flat
 
 
-class _Copy:
-    """A padded copy inside a buffer that it keeps alive."""
-
-    def __init__(self, buffer: Tensor, address: int):
-        self.buffer, self.address = buffer, address
-
-    def data_ptr(self) -> int:
-        return self.address
+def _address(t: Tensor, op, flat: Tensor | None) -> int:
+    return t.data_ptr() if op[0] is None else flat.data_ptr() + 2 * op[0]
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -125,16 +123,15 @@ def _backward_workspace_bytes(m: int, n: int, k: int, act: int, dx: bool, dw: bo
     return native.lib().cg_linear_half_backward_workspace_bytes(ctypes.byref(args))
 
 
-def _forward(a_op, b_op, shape, bias, activation, residual, keep_z, like):
-    """(y, z) of one product of operands as _operand gives them."""
+def _forward(a, b, ops, flat, shape, bias, activation, residual, keep_z):
+    """(y, z) of one product of operands a and b as _operands gives them."""
     m, n, k = shape
-    y = like.new_empty((m, n))
+    y = a.new_empty((m, n))
     z = torch.empty_like(y) if keep_z else None
     args = native.LinearArgs()
     args.m, args.n, args.k = m, n, k
-    a, args.lda, args.a_mn_major = a_op
-    b, args.ldb, args.b_mn_major = b_op
-    args.a, args.b = a.data_ptr(), b.data_ptr()
+    (_, args.lda, args.a_mn_major), (_, args.ldb, args.b_mn_major) = ops
+    args.a, args.b = _address(a, ops[0], flat), _address(b, ops[1], flat)
     if bias is not None:
         bias = bias.contiguous()
         args.bias = bias.data_ptr()
@@ -144,13 +141,13 @@ def _forward(a_op, b_op, shape, bias, activation, residual, keep_z, like):
     if z is not None:
         args.z, args.ld_z = z.data_ptr(), n
     args.y, args.ld_y = y.data_ptr(), n
-    args.act, args.dtype = activation, native.HALF_DTYPES[like.dtype]
+    args.act, args.dtype = activation, native.HALF_DTYPES[a.dtype]
     nbytes = _workspace_bytes(m, n, k)
     workspace = None
     if nbytes > 0:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
-    native.invoke("cg_linear_half", ctypes.byref(args), _stream(like), info=(m, n, k))
+    native.invoke("cg_linear_half", ctypes.byref(args), _stream(a), info=(m, n, k))
     return y, z
 
 
@@ -165,10 +162,10 @@ def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = 
         return y, torch.empty_like(y) if keep_z else None
     if k == 0:  # an empty sum: zero columns give it
         a, b, k = a.new_zeros(m, 8), b.new_zeros(n, 8), 8
-    return _forward(*_operands(a, b), (m, n, k), bias, activation, residual, keep_z, a)
+    return _forward(a, b, *_operands(a, b), (m, n, k), bias, activation, residual, keep_z)
 
 
-def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
+def _backward(gy, z, x, w, ops, flat, shape, activation, want_dx, want_dw, want_db):
     """(dx, dw, db) in one call; None for what is not wanted."""
     m, n, k = shape
     args = native.LinearBackwardArgs()
@@ -178,17 +175,17 @@ def _backward(gy, z, x_op, w_op, shape, activation, want_dx, want_dw, want_db):
         if _fits_tma(gy, 0, 1):
             args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
         else:
-            kept, args.ld_gy, _ = _operands(gy.contiguous())[0]
-            args.gy = kept.data_ptr()
+            gy = gy.contiguous()
+            (op,), kept = _operands(gy)
+            args.gy, args.ld_gy = _address(gy, op, kept), op[1]
     else:
         gy = _rows(gy)
         gz = _pitched(m, n, gy)
         args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), n)
         args.z, args.ld_z = z.data_ptr(), n
         args.gz, args.ld_gz = gz.data_ptr(), -(-n // 8) * 8
-    x, args.ld_x, args.x_mn_major = x_op
-    w, args.ld_w, args.w_mn_major = w_op
-    args.x, args.w = x.data_ptr(), w.data_ptr()
+    (_, args.ld_x, args.x_mn_major), (_, args.ld_w, args.w_mn_major) = ops
+    args.x, args.w = _address(x, ops[0], flat), _address(w, ops[1], flat)
     dx = gy.new_empty((m, k)) if want_dx else None
     dw = gy.new_empty((n, k)) if want_dw else None
     db = gy.new_empty(n) if want_db else None
@@ -298,19 +295,17 @@ class _Linear(_Fused):
     @staticmethod
     def forward(ctx, x, w, b, r, activation):
         ctx.activation = activation
-        ctx.save = m, n, k = x.shape[0], w.shape[0], x.shape[1]
+        ctx.shape = m, n, k = x.shape[0], w.shape[0], x.shape[1]
         # z is seldom used: its gradient arrives as None, not as zeros
         ctx.set_materialize_grads(False)
         keep_z = activation != native.ACT_NONE
-        ctx.operands = None
+        ctx.operands = flat = None
         if min(m, n, k) == 0:
             y, z = product(x, w, b, activation, r, keep_z)
         else:
-            # the operands as the products read them: x and w themselves, or
-            # copies whose rows start on 16-byte boundaries
-            ctx.operands = x_op, w_op = _operands(x, w)
-            y, z = _forward(x_op, w_op, ctx.save, b, activation, r, keep_z, x)
-        ctx.save_for_backward(x, w, z)
+            ctx.operands, flat = _operands(x, w)
+            y, z = _forward(x, w, ctx.operands, flat, ctx.shape, b, activation, r, keep_z)
+        ctx.save_for_backward(x, w, z, flat)
         ctx.inputs = (True, True, b is not None)
         return y, z
 
@@ -318,7 +313,7 @@ class _Linear(_Fused):
     def _wanted(ctx):
         """Which of x, w, b the backward pass running now needs."""
         need = ctx.needs_input_grad[:3]
-        m, n, k = ctx.save
+        m, n, k = ctx.shape
         if 2.0 * m * n * k < _SMALL_FLOPS and not torch.is_grad_enabled():
             return need
         nodes = iter(ctx.next_functions)
@@ -327,13 +322,14 @@ class _Linear(_Fused):
 
     @staticmethod
     def backward(ctx, gy, gz_direct):
-        x, w, z = ctx.saved_tensors
+        x, w, z, flat = ctx.saved_tensors
         want = _Linear._wanted(ctx)
         dr = gy if ctx.needs_input_grad[3] else None
         if not torch.is_grad_enabled() and gz_direct is None and gy is not None and ctx.operands is not None:
             if not any(want):
                 return None, None, None, dr, None
-            return *_backward(gy, z, *ctx.operands, ctx.save, ctx.activation, *want), dr, None
+            grads = _backward(gy, z, x, w, ctx.operands, flat, ctx.shape, ctx.activation, *want)
+            return *grads, dr, None
         # the differentiable path: products and passes that record their own backward
         gz, db = gz_direct, None
         if gy is not None and any(want):
