@@ -462,7 +462,7 @@ struct PlainEpi : EpiBase {
 // elements as the epilogue does; VEC: groups of eight columns.
 template <class T, bool VEC>
 __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits, int m, int n) {
-  half::allow_next();
+  half::allow_next_if_few();
   half::wait_previous();
   const int64_t mn = (int64_t)m * n, stride = (int64_t)gridDim.x * blockDim.x;
   const int64_t first = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
                                                        const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
                                                        int64_t ld_gz, int rows, int cols, int kind, int rows_per,
                                                        float* __restrict__ partial, T* __restrict__ db) {
-  half::allow_next();
+  half::allow_next_if_few();
   half::wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.x * 32 + lane) * V;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
 // db[c] = sum of the chunks' sums in chunk order, rounded once.
 template <class T>
 __global__ void join_columns_kernel(const float* __restrict__ partial, int chunks, int cols, T* __restrict__ db) {
-  half::allow_next();
+  half::allow_next_if_few();
   half::wait_previous();
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= cols) return;
@@ -595,7 +595,7 @@ struct Padded {
   int cols;
 };
 __global__ void __launch_bounds__(256) pad_rows_kernel(Padded a, Padded b) {
-  half::allow_next();
+  half::allow_next_if_few();
   half::wait_previous();
   const int64_t first = (a.ld_dst / 8) * a.rows, all = first + (b.ld_dst / 8) * b.rows;
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;

@@ -135,7 +135,7 @@ namespace muon {
 // Block = one chunk of kChunk elements of one matrix.
 template <class T, bool MOMENTUM, bool NORM>
 __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Prepare p) {
-  half::allow_next();
+  half::allow_next_if_few();
   half::wait_previous();
   int i = 0;
   while (i + 1 < p.runs && (int)blockIdx.x >= p.run[i + 1].first_chunk) ++i;
@@ -169,37 +169,52 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     lo = hi + (int64_t)run.rows * run.pitch;
   }
   if (run.vec) {
-#pragma unroll 2
-    for (int e = 4 * threadIdx.x; e < size; e += 4 * 256) {
-      const int down = run.by_cols.div(col0 + e), row = row0 + down, col = col0 + e - down * run.cols;
-      float v[4];
-      load_four(x + (int64_t)row * run.ld_x + col, v);
-      if (MOMENTUM) {
-        float4* mp = reinterpret_cast<float4*>(mom + (int64_t)row * run.ld_momentum + col);
-        float4 m = *mp;
-        if (NORM) {
-          m = make_float4(rule.next(m.x, v[0]), rule.next(m.y, v[1]), rule.next(m.z, v[2]), rule.next(m.w, v[3]));
-          *mp = m;
+    // two groups of four per thread and turn, their loads ahead of the stores
+    constexpr int U = 2;
+    for (int base = 4 * threadIdx.x; base < size; base += U * 4 * 256) {
+      int row[U], col[U];
+      float v[U][4];
+      float4 m[U];
+#pragma unroll
+      for (int g = 0; g < U; ++g) {
+        const int e = base + g * 4 * 256;
+        if (e < size) {
+          const int down = run.by_cols.div(col0 + e);
+          row[g] = row0 + down;
+          col[g] = col0 + e - down * run.cols;
+          load_four(x + (int64_t)row[g] * run.ld_x + col[g], v[g]);
+          if (MOMENTUM) m[g] = *reinterpret_cast<const float4*>(mom + (int64_t)row[g] * run.ld_momentum + col[g]);
         }
-        v[0] = rule.update(m.x, v[0]);
-        v[1] = rule.update(m.y, v[1]);
-        v[2] = rule.update(m.z, v[2]);
-        v[3] = rule.update(m.w, v[3]);
       }
-      if (NORM) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum += (double)v[q] * v[q];
-      } else {
-        __half h[4], l[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float f = v[q] * scale;
-          h[q] = __float2half_rn(f);
-          l[q] = __float2half_rn(f - __half2float(h[q]));
+      for (int g = 0; g < U; ++g) {
+        if (base + g * 4 * 256 >= size) break;
+        if (MOMENTUM) {
+          if (NORM) {
+            m[g] = make_float4(rule.next(m[g].x, v[g][0]), rule.next(m[g].y, v[g][1]), rule.next(m[g].z, v[g][2]),
+                               rule.next(m[g].w, v[g][3]));
+            *reinterpret_cast<float4*>(mom + (int64_t)row[g] * run.ld_momentum + col[g]) = m[g];
+          }
+          v[g][0] = rule.update(m[g].x, v[g][0]);
+          v[g][1] = rule.update(m[g].y, v[g][1]);
+          v[g][2] = rule.update(m[g].z, v[g][2]);
+          v[g][3] = rule.update(m[g].w, v[g][3]);
         }
-        const int64_t o = (int64_t)row * run.pitch + col;
-        *reinterpret_cast<uint2*>(hi + o) = *reinterpret_cast<const uint2*>(h);
-        *reinterpret_cast<uint2*>(lo + o) = *reinterpret_cast<const uint2*>(l);
+        if (NORM) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sum += (double)v[g][q] * v[g][q];
+        } else {
+          __half h[4], l[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float f = v[g][q] * scale;
+            h[q] = __float2half_rn(f);
+            l[q] = __float2half_rn(f - __half2float(h[q]));
+          }
+          const int64_t o = (int64_t)row[g] * run.pitch + col[g];
+          *reinterpret_cast<uint2*>(hi + o) = *reinterpret_cast<const uint2*>(h);
+          *reinterpret_cast<uint2*>(lo + o) = *reinterpret_cast<const uint2*>(l);
+        }
       }
     }
   } else {
@@ -453,22 +468,17 @@ struct FinalEpi : EpiBase {
     constexpr int kGroup = 16 / sizeof(T);
     vec = n % 8 == 0 && ld % kGroup == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   }
-  __device__ __forceinline__ void put8(const float (&v)[8], float* p) const {
+  // eight values of a row and what is there (old, zeros where keep is 0)
+  __device__ __forceinline__ void put8(const float (&v)[8], const float (&old)[8], float* p) const {
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = a->keep * old[e] + a->rate * v[e];
     float4* q = reinterpret_cast<float4*>(p);
-    const float rate = a->rate, keep = a->keep;
-    if (keep != 0.0f) {
-      const float4 x = q[0], y = q[1];
-      q[0] = make_float4(keep * x.x + rate * v[0], keep * x.y + rate * v[1], keep * x.z + rate * v[2],
-                         keep * x.w + rate * v[3]);
-      q[1] = make_float4(keep * y.x + rate * v[4], keep * y.y + rate * v[5], keep * y.z + rate * v[6],
-                         keep * y.w + rate * v[7]);
-    } else {
-      q[0] = make_float4(rate * v[0], rate * v[1], rate * v[2], rate * v[3]);
-      q[1] = make_float4(rate * v[4], rate * v[5], rate * v[6], rate * v[7]);
-    }
+    q[0] = make_float4(o[0], o[1], o[2], o[3]);
+    q[1] = make_float4(o[4], o[5], o[6], o[7]);
   }
   template <class H>
-  __device__ __forceinline__ void put8(const float (&v)[8], H* p) const {
+  __device__ __forceinline__ void put8(const float (&v)[8], const float (&)[8], H* p) const {
     H h[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) put_value(h + e, a->rate * v[e]);
@@ -488,12 +498,31 @@ struct FinalEpi : EpiBase {
     if (vec) {
       const int c = (lane & 3) * 8, col = col0 + c;
       if (col < n) {
+        T* at = out + (int64_t)(row0 + (lane >> 2)) * ld + col;
+        // the four rows' weights at once, ahead of the stores
+        float old[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) old[i][e] = 0.0f;
+        if constexpr (sizeof(T) == 4) {
+          if (a->keep != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (row0 + (lane >> 2) + 8 * i >= m) break;
+              const float4* q = reinterpret_cast<const float4*>(at + (int64_t)8 * i * ld);
+              const float4 x = q[0], y = q[1];
+              old[i][0] = x.x; old[i][1] = x.y; old[i][2] = x.z; old[i][3] = x.w;
+              old[i][4] = y.x; old[i][5] = y.y; old[i][6] = y.z; old[i][7] = y.w;
+            }
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = (lane >> 2) + 8 * i, row = row0 + r;
+          if (row0 + (lane >> 2) + 8 * i >= m) break;
           float x[8];
-          half::stage_read8(stage, r, c, x);
-          if (row < m) put8(x, out + row * ld + col);
+          half::stage_read8(stage, (lane >> 2) + 8 * i, c, x);
+          put8(x, old[i], at + (int64_t)8 * i * ld);
         }
       }
     } else if (col0 + lane < n) {  // odd pitches: one column per lane
@@ -502,7 +531,7 @@ struct FinalEpi : EpiBase {
         const int row = row0 + r;
         if (row >= m) break;
         float x = a->rate * stage[half::stage_idx(r, lane)];
-        T* p = out + row * ld + col0 + lane;
+        T* p = out + (int64_t)row * ld + col0 + lane;
         if (sizeof(T) == 4 && a->keep != 0.0f) x += a->keep * *reinterpret_cast<const float*>(p);
         put_value(p, x);
       }
@@ -754,7 +783,9 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
   L.partial = b.partial;
   L.counters = b.counters;
   L.most_splits = plan.splits;
-  L.sum_slices = coarse ? 4 : 2;
+  // one slice per accumulator where the epilogue adds them up faster than they
+  // come (256-wide tiles' sums take as long as a slice)
+  L.sum_slices = coarse ? 4 : BN == 256 ? 2 : 1;
   int64_t items = 0, tiles = 0;
   for (int i = 0; i < n; ++i) {
     const Shape& h = shapes[i];
@@ -953,8 +984,8 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     // hundredth to a thousandth part at a time, are formed a little less exactly
     // (about 1e-5 relative on strongly decaying spectra instead of 5e-6): B
     // carries a on its diagonal, so that X <- B X reads no X beside its operand,
-    // and accumulators run for four k-slices instead of two, so that the products
-    // run further ahead of the epilogue: an update product of the 85M step takes
+    // and accumulators run for four k-slices instead of one or two, so that the
+    // products run further ahead of the epilogue: an update product of the 85M step takes
     // 273 us against 350.
     const bool coarse = momentum || g.dtype != CG_F32;
     for (int t = 0; t < g.steps; ++t) {
