@@ -13,7 +13,7 @@
 //               the epilogue (two accumulators: an item's epilogue runs beside
 //               the next item's products);
 //   warps 2..   epilogue: tcgen05.ld (thread = row), the layer's own arithmetic,
-//              and the result through shared memory to global memory.
+//               and the result through shared memory to global memory.
 // Operands are K-major (contiguous along k) or MN-major (contiguous along m or
 // n), so x W^T, g W and g^T x read their operands as they are stored.
 // PLANES = 2: every operand is a pair of fp16 planes hi + lo (22 significant
@@ -24,7 +24,11 @@
 // epilogue warps add them up in registers, rounded to nearest.
 // A pair of SMs halves the B bytes each SM stages per flop: a 256 x 256 tile
 // takes 32 KB of shared memory per 64-wide slice and SM against 48 KB for the
-// 128 x 256 tile of one SM, which is what lets six stages fit.
+// 128 x 256 tile of one SM, so that a ring of five stages fits beside the
+// epilogue's blocks (three stages: 12% slower).
+// Measured (bf16, one plane): 8192^3 in 709 us, 1.55 PFLOP/s, 94% of the measured
+// cuBLAS rate; 65536 x 3072 x 768 in 236 us, 1.31 PFLOP/s, where the output's
+// way through shared memory takes 30 us from the products.
 // Every wait is bounded: on timeout the kernel records an error in the
 // translation unit's error word, lets its copies land and unwinds.
 #pragma once
