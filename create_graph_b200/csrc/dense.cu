@@ -330,17 +330,21 @@ struct BlockEpi : EpiBase {
   }
   // 32 pre-activations of this thread's row
   __device__ __forceinline__ void load(uint32_t acc, int col0, float (&v)[32]) const {
+    uint4 b[4];  // on their way beside the accumulator's
+    if (p->bias) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        b[c] = col0 + 8 * c < n ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p->bias) + col0 + 8 * c))
+                                : make_uint4(0, 0, 0, 0);
+    }
     tmem_load_32(acc, v);
     if (p->bias == nullptr) return;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int col = col0 + 8 * c;
-      if (col < n) {
-        float b[8];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p->bias) + col)), b);
+      float f[8];
+      unpack8<T>(b[c], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * c + e] += b[e];
-      }
+      for (int e = 0; e < 8; ++e) v[8 * c + e] += f[e];
     }
   }
   __device__ __forceinline__ bool store(uint32_t acc, int col0, int* error) {
