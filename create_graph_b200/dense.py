@@ -175,9 +175,13 @@ def _backward(gy, z, x, w, ops, flat, shape, activation, want_dx, want_dw, want_
         if _fits_tma(gy, 0, 1):
             args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
         else:
+            # rows on 16-byte boundaries, whatever other layout would do
             gy = gy.contiguous()
-            (op,), kept = _operands(gy)
-            args.gy, args.ld_gy = _address(gy, op, kept), op[1]
+            args.ld_gy = -(-n // 8) * 8
+            kept = gy.new_empty(m * args.ld_gy)
+            args.gy = kept.data_ptr()
+            native.invoke("cg_pad_rows_half", gy.data_ptr(), n, m, n, args.gy, args.ld_gy, None, 0, 0, 0, None, 0,
+                          _stream(gy))
     else:
         gy = _rows(gy)
         gz = _pitched(m, n, gy)

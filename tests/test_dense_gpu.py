@@ -85,6 +85,30 @@ def test_gradients(mnk, act, dtype):
     assert native.device_error() == 0
 
 
+@pytest.mark.parametrize("act", sorted(ACTIVATIONS))
+@pytest.mark.parametrize("mnk", [(2, 1, 19), (35, 1, 8), (300, 1, 264), (1, 1, 1), (70, 2, 1), (1, 37, 50)])
+def test_gradients_of_thin_layers(mnk, act):
+    """One or two columns, one row: incoming gradients whose layout says little.
+    A gradient may be a single sum of signed terms here, so the error is held
+    against the sum of their magnitudes: 3 u |gy| (|f'| + |z f''| <= 1.5)."""
+    dtype = torch.bfloat16
+    x, w, b, _, gy = tensors(*mnk, dtype, seed=13)
+    wide = torch.zeros(mnk[0], mnk[1] + 7, dtype=dtype, device="cuda")
+    column = wide[:, 3 : 3 + mnk[1]]
+    column.copy_(gy)
+    ref = doubled(x, w, b)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    # the last one: a gradient of ones with no memory of its own
+    for g in (gy, column, gy.t().contiguous().t(), torch.ones((), dtype=dtype, device="cuda").expand(mnk[:2])):
+        got = torch.autograd.grad(linear(x, w, b, activation=act), leaves, g)
+        gd = g.double().cpu()
+        want = torch.autograd.grad(formula(*ref, None, act), ref, gd)
+        size = 1.5 * gd.abs()
+        sizes = (size @ ref[1].detach().abs(), size.t() @ ref[0].detach().abs(), size.sum(0))
+        for a, e, s in zip(got, want, sizes):
+            assert float((a.double().cpu() - e).norm()) < 3.0 * UNIT[dtype] * float(s.norm())
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gradient_against_differences(act):
     # directional derivative of <gy, y> along a random direction of x, central
