@@ -634,10 +634,10 @@ struct Plan {
 // slot (SM or SM pair) that gets most: a tile takes `slice` per 64-wide k-slice
 // and `wave` beside it, in nanoseconds measured on launches of one wave and of
 // several, and a launch `once`. 256 x 256 tiles of an SM pair feed the tensor
-// cores best (4096^3: 96 us, 110 us with 256 x 128, 116 with 128 x 128, 223 with
-// 128 x 64), the smaller ones fill the SMs when there are few (512^3: 8.4, 6.7,
-// 5.9 and 5.1 us); a split pays when k is long (3072 x 768 x 8280: 34 us in two
-// parts, 48 us whole).
+// cores best (4096^3: 97 us, 108 us with 256 x 128, 125 with 128 x 128, 223 with
+// 128 x 64), the smaller ones fill the SMs when there are few (512^3: 7.7, 6.0,
+// 5.8 and 5.1 us); a split pays when k is long (3072 x 768 x 8280: 40 us in two
+// parts, 55 us whole).
 static Plan search_plan(const cg_linear_args* g, int count) {
   const int64_t sms = sm_count();
   struct Shape {
@@ -645,7 +645,7 @@ static Plan search_plan(const cg_linear_args* g, int count) {
     double slice, wave, once;
   };
   static const Shape shapes[] = {
-      {2, 256, 340, 1550, 3900}, {2, 192, 270, 1300, 3900}, {2, 128, 240, 900, 3900}, {1, 128, 260, 800, 3400}, {1, 64, 260, 700, 3200}};
+      {2, 256, 320, 1450, 4200}, {2, 192, 278, 950, 4000}, {2, 128, 215, 810, 4000}, {1, 128, 205, 1400, 2900}, {1, 64, 195, 900, 2700}};
   const int kMost = 24;
   int64_t kts[2] = {1, 1};
   for (int i = 0; i < count; ++i) kts[i] = ceil_div<int64_t>(g[i].k, half::kBK);

@@ -599,44 +599,52 @@ struct Plan {
 // By time, in nanoseconds measured on launches of one wave and of several: a
 // launch takes `once`, and each wave of tiles `slice` per 64-wide k-slice
 // (three products) and `wave`; a split adds the partial sums it leaves and
-// reads. Larger tiles feed the tensor cores best, smaller ones and splits of k
-// fill the SMs when there are few: the gram of one 3072 x 768 matrix takes 50 us
-// on 256 x 256 tiles, 28 us on 128 x 64 and 15 us with k split in three; for
-// twelve of them 59, 101 and (too many tiles to split) 101 us.
-static Plan plan_of(const Shape* shapes, int n, Step step) {
+// reads. `coarse` products (see run) keep the epilogue warps less busy, and their
+// updates read no planes. Larger tiles feed the tensor cores best, smaller ones
+// and splits of k fill the SMs when there are few: the gram of one 3072 x 768
+// matrix takes 49 us on 256 x 256 tiles, 27 us on 256 x 128, 31 us on 128 x 64 and
+// 17 us there with k split in three; for twelve of them 53, 54, 115 and (too many
+// tiles to split) 115 us.
+static Plan plan_of(const Shape* shapes, int n, Step step, bool coarse) {
   struct Tile {
     int cg, bn;
-    double slice, wave, once;
+    double slice, coarse_slice, wave, coarse_update, once;
   };
-  static const Tile choices[] = {
-      {2, 256, 840, 7400, 3000}, {2, 128, 580, 4000, 3200}, {1, 128, 600, 2700, 4300}, {1, 64, 475, 1300, 4000}};
+  static const Tile choices[] = {{2, 256, 800, 800, 6200, 2200, 5000},
+                                 {2, 128, 395, 395, 3700, 1600, 4300},
+                                 {1, 128, 658, 522, 2800, 1300, 4500},
+                                 {1, 64, 525, 430, 1400, 750, 4200}};
   const int sms = sm_count();
   Plan best = {2, 256, 1, 0, 0};
   double least = 0.0;
   for (const Tile& t : choices) {
     const int bm = t.cg * half::kRows, slots = sms / t.cg;
+    const double slice = coarse ? t.coarse_slice : t.slice;
+    const double wave = coarse && step == kUpdate ? t.coarse_update : t.wave;
+    int64_t tiles = 0, counts[kGroups], slices[kGroups];
+    for (int i = 0; i < n; ++i) {
+      const Shape& h = shapes[i];
+      const int64_t m = step == kUpdate ? h.rows : h.s, w = step == kUpdate ? h.cols : h.s;
+      const int64_t k = step == kGram ? (h.rows < h.cols ? h.cols : h.rows) : h.s;
+      const int64_t m_tiles = ceil_div<int64_t>(m, bm), n_tiles = ceil_div<int64_t>(w, t.bn);
+      counts[i] = m_tiles * n_tiles;
+      if (step != kUpdate) {
+        counts[i] = 0;
+        for (int64_t r = 0; r < m_tiles; ++r) counts[i] += half::lower_tiles_of_row((int)r, bm, t.bn, (int)n_tiles);
+      }
+      counts[i] *= h.count;
+      slices[i] = ceil_div<int64_t>(k, half::kBK);
+      tiles += counts[i];
+    }
     for (int splits = 1; splits <= 8; ++splits) {
       double items = 0.0, time = 0.0;
-      int64_t tiles = 0;
       bool any = splits == 1;
       for (int i = 0; i < n; ++i) {
-        const Shape& h = shapes[i];
-        const int64_t m = step == kUpdate ? h.rows : h.s, w = step == kUpdate ? h.cols : h.s;
-        const int64_t k = step == kGram ? (h.rows < h.cols ? h.cols : h.rows) : h.s;
-        const int64_t m_tiles = ceil_div<int64_t>(m, bm), n_tiles = ceil_div<int64_t>(w, t.bn);
-        int64_t count = m_tiles * n_tiles;
-        if (step != kUpdate) {
-          count = 0;
-          for (int64_t r = 0; r < m_tiles; ++r) count += half::lower_tiles_of_row((int)r, bm, t.bn, (int)n_tiles);
-        }
-        count *= h.count;
-        const int64_t kts = ceil_div<int64_t>(k, half::kBK), per = ceil_div<int64_t>(kts, splits);
-        const int64_t parts = ceil_div<int64_t>(kts, per);
+        const int64_t per = ceil_div<int64_t>(slices[i], splits), parts = ceil_div<int64_t>(slices[i], per);
         any = any || (parts == splits && per >= 2);
-        tiles += count;
-        items += (double)count * parts;
+        items += (double)counts[i] * parts;
         const double join = parts > 1 ? 1300.0 + t.bn / 64 * (300.0 + 250.0 * parts) : 0.0;
-        time += (double)count * parts * (per * t.slice + t.wave + join);
+        time += (double)counts[i] * parts * (per * slice + wave + join);
       }
       if (!any) continue;
       const double cost = t.once + ceil(items / slots) * time / items;
@@ -691,8 +699,8 @@ static int64_t layout(Shape* shapes, int n, char* base, Buffers* b) {
   b->squares = reinterpret_cast<double*>(take(chunks * (int64_t)sizeof(double)));
   b->table = reinterpret_cast<OutRef*>(take(matrices * (int64_t)sizeof(OutRef)));
   int64_t floats = 0, counters = 0;
-  for (int step = 0; step < 3; ++step) {
-    const Plan p = plan_of(shapes, n, (Step)step);
+  for (int i = 0; i < 6; ++i) {  // a workspace serves exact and coarse products alike
+    const Plan p = plan_of(shapes, n, (Step)(i / 2), i % 2 != 0);
     if (p.slots == 0) continue;
     if (p.floats > floats) floats = p.floats;
     if (p.slots > counters) counters = p.slots;
@@ -881,9 +889,9 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
 }
 
 template <class E>
-static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Buffers& b, bool coarse, bool odd,
-                   bool last, float keep, const float* rate, cudaStream_t s) {
-  const Plan p = plan_of(shapes, n, step);
+static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Plan* plans, const Buffers& b,
+                   bool coarse, bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
+  const Plan& p = plans[step];
   if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
   if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
   if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
@@ -995,14 +1003,16 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     // products run further ahead of the epilogue: an update product of the 85M step takes
     // 273 us against 350.
     const bool coarse = momentum || g.dtype != CG_F32;
+    Plan plans[3];
+    for (int i = 0; i < 3; ++i) plans[i] = plan_of(shapes, n, (Step)i, coarse);
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;
-      if ((rc = product<SplitEpi>(g, shapes, n, kGram, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
-      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
-      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, b, coarse, odd, false, 0.0f, nullptr, s);
-      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
-      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
-      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, b, coarse, odd, true, keep, rate, s);
+      if ((rc = product<SplitEpi>(g, shapes, n, kGram, plans, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, plans, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, plans, b, coarse, odd, false, 0.0f, nullptr, s);
+      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
+      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
+      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
       if (rc) return rc;
     }
   }
