@@ -180,19 +180,27 @@ __device__ __forceinline__ float2 silu2(float2 z) {
   const float2 e = make_float2(exp2_approx(fminf(x.x, 60.0f)), exp2_approx(fminf(x.y, 60.0f)));
   return mul2(z, rcp2(make_float2(1.0f + e.x, 1.0f + e.y)));
 }
-// gelu of two values: max(z, 0) - |z| (1 - Phi(|z|)), the tail (0 long before
-// 64) as in normal_tail
+// gelu of two values: max(z, 0) - |z| (1 - Phi(|z|)). The tail 1 - Phi goes
+// through one reciprocal and no exponential: its 32nd root's reciprocal grows
+// like exp(z^2 / 64) and is a polynomial of degree 7 to 5e-7 (minimax relative
+// error on [0, 6.5], fitted to the normal distribution's logarithm), so the tail
+// is right to 2e-5 there, far below the rounding to 2^-9 or 2^-11, and to 1e-2
+// at 8, where gelu is 5e-15; at -12 and beyond it is held at 2^-107.
 __device__ __forceinline__ float2 gelu2(float2 z) {
-  const float2 a = make_float2(fminf(fabsf(z.x), 64.0f), fminf(fabsf(z.y), 64.0f));
-  const float2 t = rcp2(fma2(a, both(0.3275911f * 0.70710678f), both(1.0f)));
-  const float2 u = mul2(mul2(a, a), both(-0.5f * kLog2e));
-  const float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
-  float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
-  p = fma2(t, p, both(0.7107068705f));
-  p = fma2(t, p, both(-0.142248368f));
-  p = fma2(t, p, both(0.127414796f));
-  const float2 w = mul2(mul2(mul2(p, t), e), a);
-  return fma2(make_float2(z.x + fabsf(z.x), z.y + fabsf(z.y)), both(0.5f), make_float2(-w.x, -w.y));
+  const float2 a = make_float2(fmaxf(-fabsf(z.x), -12.0f), fmaxf(-fabsf(z.y), -12.0f));
+  float2 p = fma2(a, both(-1.763030895e-07f), both(-2.591498287e-06f));
+  p = fma2(a, p, both(-3.504646520e-05f));
+  p = fma2(a, p, both(-1.234932133e-04f));
+  p = fma2(a, p, both(-1.482319436e-03f));
+  p = fma2(a, p, both(1.043934096e-02f));
+  p = fma2(a, p, both(-2.549119666e-02f));
+  p = fma2(a, p, both(1.021896601f));
+  p = mul2(p, p);
+  p = mul2(p, p);
+  p = mul2(p, p);
+  p = mul2(p, p);           // at most 2^54
+  const float2 r = rcp2(p);  // the tail's square root
+  return fma2(mul2(a, r), r, make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f)));
 }
 
 // f' of two values, as act_grad.
@@ -288,13 +296,15 @@ struct EpiBase {
 // by TMA into the same block beforehand (each thread reads and overwrites its
 // own row); the pre-activation follows through the same block, read from TMEM
 // once more. Sixteen warps, one block each of a 256-wide tile, hide one
-// another's latencies (65536 x 3072 x 768 with gelu: 287 us, eight warps 323 us).
+// another's latencies (65536 x 3072 x 768 with gelu: 287 us, eight warps 323 us,
+// before the activation's and the barriers' later steps: 255 to 270 us).
 // Against staging fp32 blocks and storing 64-byte row segments from the
 // threads this halves the shared-memory traffic that competes with the
-// operands: 65536 x 3072 x 768 with no activation takes 236 us (298 us before,
-// 203 us without any stores), with a residual 282, with gelu, residual and
-// pre-activation 360 to 380 (three 400 MB streams: 200 us at the copy rate; the
-// blocks' waits for residual and pre-activation are what is left).
+// operands: 65536 x 3072 x 768 with no activation takes 230 us (298 us before,
+// 203 us without any stores), with a residual 275, with gelu, residual and
+// pre-activation 340 to 370 (three 400 MB streams: 200 us at the copy rate; the
+// activation's arithmetic, the block's second use for the pre-activation and the
+// power limit are what is left).
 template <class T>
 struct BlockEpi : EpiBase {
   static constexpr int kWarps = 16;
