@@ -523,14 +523,18 @@ __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits
 }
 
 // ---- elementwise passes of the derivatives -----------------------------------------
-// Bound by HBM: three streams of rows x cols values (65536 x 3072 bf16: 1.2 GB in
-// 230 to 260 us, 4.6 to 5.2 TB/s; without the arithmetic 230).
+// Bound by HBM: three streams of rows x cols values (65536 x 3072 bf16: 1.2 GB with
+// silu in 195 us, 6.2 TB/s, 94% of the measured copy rate, with gelu in 209 us;
+// 8280 x 3072 31 and 34 us).
 // gz = gy f'(z) and the column sums of gz (the bias gradient) in one pass over
 // gy and z: block (x, y) owns 32 x V columns and the rows of chunk y; its eight
 // warps walk the rows, each lane adding up V columns in fp32, and the warps'
-// sums meet in shared memory in warp order. V = 8 (16-byte groups) or 1.
+// sums meet in shared memory in warp order. V = 8 (16-byte groups) or 1. Four
+// blocks an SM with two rows of a warp in flight: with five or six the registers
+// spill (229 and 267 us with silu), with three or two too little is in flight (205
+// and 245), one row at a time waits (236).
 template <class T, int V>
-__global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
+__global__ void __launch_bounds__(256, V == 8 ? 4 : 1) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
                                                        const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
                                                        int64_t ld_gz, int rows, int cols, int kind, int rows_per,
                                                        float* __restrict__ partial, T* __restrict__ db) {
@@ -542,24 +546,42 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const T* __restrict__ gy,
   float sum[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sum[e] = 0.0f;
-  if (col < cols) {
+  if constexpr (V == 8) {
+    // two rows' loads on their way before the first is used
+    if (col < cols) {
+      for (int64_t r = r0 + warp; r < r1; r += 16) {
+        uint4 ga[2], za[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (r + 8 * i >= r1) break;
+          ga[i] = *reinterpret_cast<const uint4*>(gy + (r + 8 * i) * ld_gy + col);
+          if (gz) za[i] = *reinterpret_cast<const uint4*>(z + (r + 8 * i) * ld_z + col);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (r + 8 * i >= r1) break;
+          float g[8], x[8];
+          unpack8<T>(ga[i], g);
+          if (gz) {
+            unpack8<T>(za[i], x);
+            act_grad_all(g, x, kind);
+            *reinterpret_cast<uint4*>(gz + (r + 8 * i) * ld_gz + col) = pack8<T>(g);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] += g[e];
+        }
+      }
+    }
+  } else if (col < cols) {
 #pragma unroll 4
     for (int64_t r = r0 + warp; r < r1; r += 8) {
-      float g[V], x[V];
-      if constexpr (V == 8) {
-        unpack8<T>(*reinterpret_cast<const uint4*>(gy + r * ld_gy + col), g);
-        if (gz) unpack8<T>(*reinterpret_cast<const uint4*>(z + r * ld_z + col), x);
-      } else {
-        g[0] = to_float(gy[r * ld_gy + col]);
-        if (gz) x[0] = to_float(z[r * ld_z + col]);
-      }
+      float g[1] = {to_float(gy[r * ld_gy + col])};
       if (gz) {
+        const float x[1] = {to_float(z[r * ld_z + col])};
         act_grad_all(g, x, kind);
-        if constexpr (V == 8) *reinterpret_cast<uint4*>(gz + r * ld_gz + col) = pack8<T>(g);
-        else gz[r * ld_gz + col] = from_float<T>(g[0]);
+        gz[r * ld_gz + col] = from_float<T>(g[0]);
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += g[e];
+      sum[0] += g[0];
     }
   }
   if (partial == nullptr && db == nullptr) return;
@@ -884,12 +906,14 @@ static int run(const cg_linear_args* args, void* stream) {
   return run_products(args, 1, args->workspace, args->workspace_bytes, stream);
 }
 
-// Row chunks of act_grad: enough blocks to fill the SMs several times, each of
-// at least 32 rows; up to 128 rows are one chunk, whose sums need no join.
+// Row chunks of act_grad, each of at least 32 rows: as many blocks as the SMs
+// hold at once (V = 8: four an SM), for single columns enough to fill them
+// several times; up to 128 rows are one chunk, whose sums need no join.
 static int chunk_rows(int64_t rows, int64_t cols, int v) {
   if (rows <= 128) return 128;
   const int64_t strips = ceil_div<int64_t>(cols, 32 * v);
-  int64_t chunks = ceil_div<int64_t>((int64_t)sm_count() * 8, strips);
+  int64_t chunks = v == 8 ? (int64_t)sm_count() * 4 / strips : ceil_div<int64_t>((int64_t)sm_count() * 8, strips);
+  if (chunks < 1) chunks = 1;
   int64_t per = ceil_div<int64_t>(rows, chunks);
   per = ceil_div<int64_t>(per < 32 ? 32 : per, 8) * 8;
   const int64_t least = ceil_div<int64_t>(rows, 65535);  // gridDim.y
