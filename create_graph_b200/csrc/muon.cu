@@ -20,10 +20,10 @@
 // A and B are symmetric: only tiles that reach the lower triangle are formed,
 // and their epilogue stores each value at both places.
 // Matrices of one shape are one batch; all shapes of a call share each launch.
-// What bounds it: many large matrices (the 85M model's 48: 3.7 ms a step) the
+// What bounds it: many large matrices (the 85M model's 48: 3.6 ms a step) the
 // three products, an update launch running at 1.35 PFLOP/s of plane products and
 // a gram launch at 1.2 (its tiles cross the diagonal); one matrix (3072 x 768:
-// 208 us) the chain of 15 launches, each 10 to 15 us of which 3 to 4 are the
+// 207 us) the chain of 15 launches, each 10 to 15 us of which 3 to 4 are the
 // way from one launch's end to the next one's first product.
 #include "half_gemm.cuh"
 #include "../../include/cg_b200.h"
