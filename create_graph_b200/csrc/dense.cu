@@ -420,9 +420,13 @@ struct BlockEpi : EpiBase {
   }
 };
 
-// Any pitch and alignment: blocks are transposed through shared memory and
-// stored one column per lane; the residual of a 32 x 32 block is read before the
-// accumulator is waited for.
+// Any pitch and alignment: bias and activation are applied a row per thread, then
+// the block is transposed through shared memory and stored one column per lane
+// (z the same way before the activation); the residual of a 32 x 32 block is read
+// before the accumulator is waited for. 4099 x 1031 x 515 fp16 with gelu, residual
+// and z: 41 us (47 with the activation applied value by value behind the
+// transpose), its gradients dx + dW 39 us (47), against 8 us of bytes: the
+// two-byte stores, 64 bytes a warp and across sectors, are what is left.
 template <class T>
 struct PlainEpi : EpiBase {
   static constexpr int kWarps = 16;
@@ -442,32 +446,53 @@ struct PlainEpi : EpiBase {
     if (a.z) static_cast<T*>(a.z)[row * a.ld_z + col] = from_float<T>(v);
     static_cast<T*>(a.y)[row * a.ld_y + col] = from_float<T>(act(v, a.act) + residual);
   }
-  __device__ bool store(uint32_t acc, int col0, int*) {
+  // a thread's row of the block goes to shared memory, a lane's column comes back
+  __device__ __forceinline__ void put(const float (&v)[32]) const {
     float* stage = reinterpret_cast<float*>(staging);
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4*>(stage + half::stage_idx(lane, 4 * q)) =
+          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    __syncwarp();
+  }
+  template <class Out>
+  __device__ __forceinline__ void columns(Out* at, int64_t ld, bool add) const {
+    const float* stage = reinterpret_cast<const float*>(staging);
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      if (row0 + r >= m) break;
+      float x = stage[half::stage_idx(r, lane)];
+      if (add) x += to_float(res[r]);
+      if constexpr (sizeof(Out) == 4) at[r * ld] = x;
+      else at[r * ld] = from_float<T>(x);
+    }
+  }
+  __device__ bool store(uint32_t acc, int col0, int*) {
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
+      const int col = col0 + 32 * h + lane;
+      const bool mine = col < n;
       if (h == 1) fetch32(col0 + 32);
       float v[32];
       tmem_load_32(acc + 32 * h, v);
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        *reinterpret_cast<float4*>(stage + half::stage_idx(lane, 4 * q)) =
-            make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-      __syncwarp();
-      const int col = col0 + 32 * h + lane;
-      if (col < n) {
-        const bool partial = p->partial != nullptr, add = p->residual != nullptr;
-        const float bias = p->bias && !partial ? to_float(static_cast<const T*>(p->bias)[col]) : 0.0f;
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-          const int64_t row = row0 + r;
-          if (row >= m) break;
-          const float x = stage[half::stage_idx(r, lane)];
-          if (partial) p->partial[((int64_t)split * m + row) * n + col] = x;
-          else finish1(*p, x + bias, add ? to_float(res[r]) : 0.0f, row, col);
-        }
+      if (p->partial != nullptr) {
+        put(v);
+        if (mine) columns(p->partial + ((int64_t)split * m + row0) * n + col, n, false);
+        continue;
       }
-      __syncwarp();
+      if (p->bias) {
+        const float b = mine ? to_float(static_cast<const T*>(p->bias)[col]) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] += __shfl_sync(0xffffffffu, b, c);
+      }
+      if (p->z) {
+        put(v);
+        if (mine) columns(static_cast<T*>(p->z) + (int64_t)row0 * p->ld_z + col, p->ld_z, false);
+      }
+      act_all(v, p->act);
+      put(v);
+      if (mine) columns(static_cast<T*>(p->y) + (int64_t)row0 * p->ld_y + col, p->ld_y, p->residual != nullptr);
     }
     return true;
   }
