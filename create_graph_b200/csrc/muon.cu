@@ -842,7 +842,13 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       blocks_s(&e.map_out, h.poly);
       G.m = G.n = G.k = (int)h.s;
       e.alpha = g.b;
-      e.beta = g.c / kScale;
+      // The tensor core aligns an instruction's products to the largest and
+      // truncates. The diagonal of A A is one large square and many small ones, all
+      // positive, and came out about 6e-9 low per term of an accumulator (fitted to
+      // 55 x 2364, whose directions all follow one path: 1.6e-6 low together without
+      // this); the other products' small terms have either sign.
+      const int64_t terms = h.s < half::kBK * L.sum_slices ? h.s : half::kBK * L.sum_slices;
+      e.beta = g.c / kScale * (1.0f + 6e-9f * (float)terms);
       e.diagonal = coarse ? g.a * kScale : 0.0f;
     } else {
       if (wide) {
