@@ -99,6 +99,25 @@ def _operands(*ts: Tensor) -> tuple[list, Tensor | None]:
     return ops, flat
 
 
+def _saved_operands(ops, flat: Tensor | None, *ts: Tensor) -> tuple[list, Tensor | None]:
+    """The forward's operands as a backward may read them from the saved tensors:
+    a copy where the forward left it in the buffer; a tensor that was read in
+    place asked for its layout again, since a saved-tensor hook (save_on_cpu, or
+    any pack that clones) may give it back in another one."""
+    if flat is None or (flat.is_contiguous() and flat.data_ptr() % 16 == 0):
+        ops = [_in_place(t) if op[0] is None else op for op, t in zip(ops, ts)]
+        if None not in ops:
+            return ops, flat
+    return _operands(*ts)
+
+
+def _require_saved(t: Tensor, shape: tuple[int, int], like: Tensor) -> None:
+    """A saved tensor as it was saved, but for its strides."""
+    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+        raise NativeError(f"dense.linear: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}, "
+                          f"{shape} {like.dtype} on {like.device} was saved")
+
+
 def _address(t: Tensor, op, flat: Tensor | None) -> int:
     return t.data_ptr() if op[0] is None else flat.data_ptr() + 2 * op[0]
 
@@ -185,8 +204,9 @@ def _backward(gy, z, x, w, ops, flat, shape, activation, want_dx, want_dw, want_
     else:
         gy = _rows(gy)
         gz = _pitched(m, n, gy)
+        z = _rows(z)
         args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), n)
-        args.z, args.ld_z = z.data_ptr(), n
+        args.z, args.ld_z = z.data_ptr(), max(z.stride(0), n)
         args.gz, args.ld_gz = gz.data_ptr(), -(-n // 8) * 8
     (_, args.ld_x, args.x_mn_major), (_, args.ld_w, args.w_mn_major) = ops
     args.x, args.w = _address(x, ops[0], flat), _address(w, ops[1], flat)
@@ -213,6 +233,7 @@ def _act_grad(gy: Tensor, z: Tensor | None, activation: int, want_db: bool):
     args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), cols)
     gz, db, scratch = gy, None, None
     if activation != native.ACT_NONE:
+        z = _rows(z)
         gz = _pitched(rows, cols, gy)
         args.z, args.ld_z = z.data_ptr(), max(z.stride(0), cols)
         args.gz, args.ld_gz = gz.data_ptr(), max(gz.stride(0), cols)
@@ -332,7 +353,13 @@ class _Linear(_Fused):
         if not torch.is_grad_enabled() and gz_direct is None and gy is not None and ctx.operands is not None:
             if not any(want):
                 return None, None, None, dr, None
-            grads = _backward(gy, z, x, w, ctx.operands, flat, ctx.shape, ctx.activation, *want)
+            m, n, k = ctx.shape
+            _require_saved(x, (m, k), gy)
+            _require_saved(w, (n, k), gy)
+            if z is not None:
+                _require_saved(z, (m, n), gy)
+            ops, flat = _saved_operands(ctx.operands, flat, x, w)
+            grads = _backward(gy, z, x, w, ops, flat, ctx.shape, ctx.activation, *want)
             return *grads, dr, None
         # the differentiable path: products and passes that record their own backward
         gz, db = gz_direct, None
