@@ -111,11 +111,11 @@ def _saved_operands(ops, flat: Tensor | None, *ts: Tensor) -> tuple[list, Tensor
     return _operands(*ts)
 
 
-def _require_saved(t: Tensor, shape: tuple[int, int], like: Tensor) -> None:
-    """A saved tensor as it was saved, but for its strides."""
+def _require(what: str, t: Tensor, shape: tuple[int, ...], like: Tensor) -> None:
+    """Refuse a tensor that the kernels would misread (its strides may be any)."""
     if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
-        raise NativeError(f"dense.linear: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}, "
-                          f"{shape} {like.dtype} on {like.device} was saved")
+        raise NativeError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(shape)} {like.dtype} "
+                          f"on {like.device}")
 
 
 def _address(t: Tensor, op, flat: Tensor | None) -> int:
@@ -226,6 +226,8 @@ def _backward(gy, z, x, w, ops, flat, shape, activation, want_dx, want_dw, want_
 def _act_grad(gy: Tensor, z: Tensor | None, activation: int, want_db: bool):
     """(gz, db): gz = gy f'(z) (gy itself without an activation), db its column
     sums or None."""
+    if z is not None:
+        _require("dense.act_grad: z", z, gy.shape, gy)
     gy = _rows(gy)
     rows, cols = gy.shape
     args = native.ActGradArgs()
@@ -252,6 +254,7 @@ class _Product(_Fused):
 
     @staticmethod
     def forward(ctx, a, b):
+        _require("dense.linear: operand of a gradient product", b, (b.shape[0], a.shape[1]), a)
         ctx.save_for_backward(a, b)
         ctx.edges = _edges(a, b)
         return product(a, b)[0]
@@ -288,6 +291,11 @@ class _ActGrad(_Fused):
 
 def _act_grad2(h: Tensor | None, hb: Tensor | None, gy: Tensor, z: Tensor, activation: int):
     """((h + hb) f'(z), (h + hb) gy f''(z)); either cotangent may be None."""
+    _require("dense.act_grad2: z", z, gy.shape, gy)
+    if h is not None:
+        _require("dense.act_grad2: h", h, gy.shape, gy)
+    if hb is not None:
+        _require("dense.act_grad2: hb", hb, gy.shape[1:], gy)
     h = None if h is None else h.contiguous()
     hb = None if hb is None else hb.contiguous()
     gy, z = gy.contiguous(), z.contiguous()
@@ -354,10 +362,10 @@ class _Linear(_Fused):
             if not any(want):
                 return None, None, None, dr, None
             m, n, k = ctx.shape
-            _require_saved(x, (m, k), gy)
-            _require_saved(w, (n, k), gy)
+            _require("dense.linear: saved tensor x", x, (m, k), gy)
+            _require("dense.linear: saved tensor weight", w, (n, k), gy)
             if z is not None:
-                _require_saved(z, (m, n), gy)
+                _require("dense.linear: saved tensor z", z, (m, n), gy)
             ops, flat = _saved_operands(ctx.operands, flat, x, w)
             grads = _backward(gy, z, x, w, ops, flat, ctx.shape, ctx.activation, *want)
             return *grads, dr, None
@@ -377,10 +385,24 @@ class _Linear(_Fused):
         return dx, dw, db, dr, None
 
 
-def _checked(x, weight, bias, residual, activation) -> int:
-    act = ACTIVATIONS.get(activation)
+def _activation(who: str, name: str) -> int:
+    act = ACTIVATIONS.get(name)
     if act is None:
-        raise NativeError(f"dense.linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+        raise NativeError(f"{who}: activation must be one of {sorted(ACTIVATIONS)}, got {name!r}")
+    return act
+
+
+def _checked_matrix(who: str, gy: Tensor, activation: str) -> int:
+    """The activation's code; refuses a gy that is no half-precision matrix on the GPU."""
+    act = _activation(who, activation)
+    if gy.dim() != 2 or gy.dtype not in native.HALF_DTYPES:
+        raise NativeError(f"{who}: a float16 or bfloat16 matrix expected, got {tuple(gy.shape)} {gy.dtype}")
+    native.require_cuda(gy)
+    return act
+
+
+def _checked(x, weight, bias, residual, activation) -> int:
+    act = _activation("dense.linear", activation)
     dtype, device = x.dtype, x.device
     if dtype not in native.HALF_DTYPES:
         raise NativeError(f"dense.linear: float16 or bfloat16 expected, got {dtype} (the fp32 layers are in "
@@ -430,8 +452,7 @@ class Linear(nn.Module):
         super().__init__()
         if dtype not in native.HALF_DTYPES:
             raise NativeError(f"dense.Linear: float16 or bfloat16 expected, got {dtype}")
-        if activation not in ACTIVATIONS:
-            raise NativeError(f"dense.Linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+        _activation("dense.Linear", activation)
         self.activation, self.dtype = activation, dtype
         like = nn.Linear(in_features, out_features, bias=bias, device=device, dtype=torch.float32)
         self.weight, self.bias = like.weight, like.bias

@@ -40,6 +40,7 @@ from torch import Tensor
 from create_graph_b200 import dense, native
 from create_graph_b200 import nn as cgnn
 from create_graph_b200 import optim
+from create_graph_b200.errors import NativeError
 from create_graph_b200.gemm import ACT_SILU
 
 
@@ -382,6 +383,8 @@ def dense_linear(x: Tensor, w: Tensor, b: Tensor | None, r: Tensor | None, activ
     """(f(z) + r, z) with z = x @ w.T + b for (M, K) x, in half precision (see
     create_graph_b200.dense; x and w may be transposed views)."""
     act = dense._checked(x, w, b, r, activation)
+    if x.dim() != 2:
+        raise NativeError(f"dense_linear: x must be a matrix, got {tuple(x.shape)}")
     return dense.product(x, w, b, act, r, keep_z=True)
 
 
@@ -393,7 +396,8 @@ def _dense_linear_fake(x, w, b, r, activation):
 @torch.library.custom_op("cg_b200::act_grad", mutates_args=())
 def act_grad(gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """(gy f'(z), the sums of its columns) of (M, N) half-precision tensors."""
-    gz, db = dense._act_grad(gy, z, dense.ACTIVATIONS[activation], True)
+    act = dense._checked_matrix("act_grad", gy, activation)
+    gz, db = dense._act_grad(gy, z, act, True)
     return (gy.clone() if gz.data_ptr() == gy.data_ptr() else gz.contiguous()), db
 
 
@@ -405,7 +409,7 @@ def _act_grad_fake(gy, z, activation):
 @torch.library.custom_op("cg_b200::act_grad2", mutates_args=())
 def act_grad2(h: Tensor, hb: Tensor, gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """((h + hb) f'(z), (h + hb) gy f''(z)) for cotangents h, hb of act_grad's outputs."""
-    return dense._act_grad2(h, hb, gy, z, dense.ACTIVATIONS[activation])
+    return dense._act_grad2(h, hb, gy, z, dense._checked_matrix("act_grad2", gy, activation))
 
 
 @act_grad2.register_fake
