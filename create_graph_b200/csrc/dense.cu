@@ -146,6 +146,13 @@ struct EpiArgs {
   int act;
 };
 
+// The larger of two values, NaN if either is (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Two fp32 values per instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
@@ -185,7 +192,9 @@ __device__ __forceinline__ float2 silu2(float2 z) {
 // like exp(z^2 / 64) and is a polynomial of degree 7 to 5e-7 (minimax relative
 // error on [0, 6.5], fitted to the normal distribution's logarithm), so the tail
 // is right to 2e-5 there, far below the rounding to 2^-9 or 2^-11, and to 1e-2
-// at 8, where gelu is 5e-15; at -12 and beyond it is held at 2^-107.
+// at 8, where gelu is 5e-15; at -12 and beyond it is held at 2^-107. A NaN goes
+// through the positive part alone: in the tail it would reach the other value
+// of the pair through the shared reciprocal.
 __device__ __forceinline__ float2 gelu2(float2 z) {
   const float2 a = make_float2(fmaxf(-fabsf(z.x), -12.0f), fmaxf(-fabsf(z.y), -12.0f));
   float2 p = fma2(a, both(-1.763030895e-07f), both(-2.591498287e-06f));
@@ -200,7 +209,7 @@ __device__ __forceinline__ float2 gelu2(float2 z) {
   p = mul2(p, p);
   p = mul2(p, p);           // at most 2^54
   const float2 r = rcp2(p);  // the tail's square root
-  return fma2(mul2(a, r), r, make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f)));
+  return fma2(mul2(a, r), r, make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)));
 }
 
 // f' of two values, as act_grad.
