@@ -98,16 +98,6 @@ __device__ __forceinline__ float normal_tail(float z, float& e) {
   return poly * e;
 }
 
-__device__ __forceinline__ float act(float z, int kind) {
-  if (kind == CG_ACT_SILU) return z * sigmoid(z);
-  if (kind == CG_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| (1 - Phi(|z|))
-    float e;
-    const float tail = normal_tail(z, e);
-    return fmaxf(z, 0.0f) - fminf(fabsf(z), 64.0f) * tail;  // the tail is 0 long before 64
-  }
-  if (kind == CG_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  return z;
-}
 __device__ __forceinline__ float act_grad(float z, int kind) {
   if (kind == CG_ACT_SILU) {
     const float s = sigmoid(z);
@@ -172,7 +162,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// 1 / d for two values of at most 2^60 with one reciprocal: the special
+// 1 / d for two values of at most 2^62 with one reciprocal: the special
 // function unit (16 results per clock and SM) bounds these epilogues, two
 // per element of a 128 x 256 tile are 4096 clocks.
 __device__ __forceinline__ float2 rcp2(float2 d) {
@@ -180,11 +170,15 @@ __device__ __forceinline__ float2 rcp2(float2 d) {
   return make_float2(r * d.y, r * d.x);
 }
 
-// silu of two values. 2^-x is held to 2^60, so below z = -41 the sigmoid stays
-// at 2^-60 (times z: 4e-17, where the exact value is smaller still).
+// silu of two values. z is held at -43 and above, where silu is -9e-18, so that
+// 2^-x stays below 2^62 for the pair's reciprocal; below it, down to -infinity,
+// silu is smaller still and 0 in the limit. A NaN stays in z and does not enter
+// the reciprocal, which is the other value's too.
+constexpr float kSiluFar = 43.0f;
 __device__ __forceinline__ float2 silu2(float2 z) {
+  z = make_float2(max_nan(z.x, -kSiluFar), max_nan(z.y, -kSiluFar));
   const float2 x = mul2(z, both(-kLog2e));
-  const float2 e = make_float2(exp2_approx(fminf(x.x, 60.0f)), exp2_approx(fminf(x.y, 60.0f)));
+  const float2 e = make_float2(exp2_approx(fminf(x.x, 62.0f)), exp2_approx(fminf(x.y, 62.0f)));
   return mul2(z, rcp2(make_float2(1.0f + e.x, 1.0f + e.y)));
 }
 // gelu of two values: max(z, 0) - |z| (1 - Phi(|z|)). The tail 1 - Phi goes
@@ -255,6 +249,13 @@ __device__ __forceinline__ void act_grad_all(float (&g)[N], const float (&z)[N],
   }
 }
 
+// f of one value, as act_all's.
+__device__ __forceinline__ float act(float z, int kind) {
+  if (kind == CG_ACT_SILU) return silu2(both(z)).x;
+  if (kind == CG_ACT_GELU) return gelu2(both(z)).x;
+  if (kind == CG_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  return z;
+}
 // f applied to a thread's values; the branch on the kind is outside the loop.
 template <int N>
 __device__ __forceinline__ void act_all(float (&v)[N], int kind) {
