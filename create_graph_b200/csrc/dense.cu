@@ -89,28 +89,6 @@ constexpr float kInvSqrt2Pi = 0.39894228f;
 
 __device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.0f + exp2_approx(-kLog2e * z)); }
 
-// 1 - Phi(|z|), and e = exp(-z^2 / 2)
-__device__ __forceinline__ float normal_tail(float z, float& e) {
-  const float t = rcp_approx(1.0f + (0.3275911f * 0.70710678f) * fabsf(z));
-  e = exp2_approx(z * z * (-0.5f * kLog2e));
-  const float poly =
-      t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-  return poly * e;
-}
-
-__device__ __forceinline__ float act_grad(float z, int kind) {
-  if (kind == CG_ACT_SILU) {
-    const float s = sigmoid(z);
-    return s * (1.0f + z * (1.0f - s));
-  }
-  if (kind == CG_ACT_GELU) {  // Phi(z) + z phi(z)
-    float e;
-    const float tail = normal_tail(z, e);
-    return (z < 0.0f ? tail : 1.0f - tail) + kInvSqrt2Pi * z * e;
-  }
-  if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  return 1.0f;
-}
 __device__ __forceinline__ float act_grad2(float z, int kind) {
   if (kind == CG_ACT_SILU) {
     const float s = sigmoid(z);
@@ -140,6 +118,13 @@ struct EpiArgs {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// z held to [-most, most]; NaN stays NaN.
+__device__ __forceinline__ float hold_nan(float z, float most) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(max_nan(z, -most)), "f"(most));
   return r;
 }
 
@@ -206,10 +191,14 @@ __device__ __forceinline__ float2 gelu2(float2 z) {
   return fma2(mul2(a, r), r, make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)));
 }
 
-// f' of two values, as act_grad.
+// f' of two values. At the bounds that z is held to, f' is 0 to 1e-17 or 1, its
+// limits at the infinities: a pre-activation that left the range of its type and
+// was kept as -infinity (fp16 below -65504) has the gradient 0 that goes with its
+// output 0. silu's 1 - s is off by an ulp, times z: 5e-6 at the most once z is held.
 __device__ __forceinline__ float2 silu_grad2(float2 z) {
+  z = make_float2(hold_nan(z.x, kSiluFar), hold_nan(z.y, kSiluFar));
   const float2 x = mul2(z, both(-kLog2e));
-  const float2 e = make_float2(exp2_approx(fminf(x.x, 60.0f)), exp2_approx(fminf(x.y, 60.0f)));
+  const float2 e = make_float2(exp2_approx(fminf(x.x, 62.0f)), exp2_approx(fminf(x.y, 62.0f)));
   const float2 s = rcp2(make_float2(1.0f + e.x, 1.0f + e.y));
   // s (1 + z (1 - s)) = s + (z s - z s s)
   const float2 zs = mul2(z, s);
@@ -227,7 +216,15 @@ __device__ __forceinline__ float2 gelu_grad2(float2 z) {
   const float2 tail = mul2(mul2(p, t), e);
   // Phi(z) = 1/2 + sign(z) (1/2 - tail)
   const float2 phi = make_float2(0.5f + copysignf(0.5f - tail.x, z.x), 0.5f + copysignf(0.5f - tail.y, z.y));
+  z = make_float2(hold_nan(z.x, 64.0f), hold_nan(z.y, 64.0f));
   return fma2(mul2(z, both(kInvSqrt2Pi)), e, phi);
+}
+// f' of one value, as act_grad_all's.
+__device__ __forceinline__ float act_grad(float z, int kind) {
+  if (kind == CG_ACT_SILU) return silu_grad2(both(z)).x;
+  if (kind == CG_ACT_GELU) return gelu_grad2(both(z)).x;
+  if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  return 1.0f;
 }
 // g <- g f'(z); the branch on the kind is outside the loop.
 template <int N>
