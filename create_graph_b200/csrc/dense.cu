@@ -89,15 +89,6 @@ constexpr float kInvSqrt2Pi = 0.39894228f;
 
 __device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.0f + exp2_approx(-kLog2e * z)); }
 
-__device__ __forceinline__ float act_grad2(float z, int kind) {
-  if (kind == CG_ACT_SILU) {
-    const float s = sigmoid(z);
-    return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
-  }
-  if (kind == CG_ACT_GELU) return kInvSqrt2Pi * exp2_approx(z * z * (-0.5f * kLog2e)) * (2.0f - z * z);
-  return 0.0f;
-}
-
 // ---- epilogue --------------------------------------------------------------------
 struct EpiArgs {
   // blocks of 32 rows x 128 bytes of y, z, the residual and the fp32 partial
@@ -225,6 +216,19 @@ __device__ __forceinline__ float act_grad(float z, int kind) {
   if (kind == CG_ACT_GELU) return gelu_grad2(both(z)).x;
   if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
+}
+// f'' of one value, with z held as in f': its square would leave fp32.
+__device__ __forceinline__ float act_grad2(float z, int kind) {
+  if (kind == CG_ACT_SILU) {
+    z = hold_nan(z, kSiluFar);
+    const float s = sigmoid(z);
+    return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
+  }
+  if (kind == CG_ACT_GELU) {
+    z = hold_nan(z, 64.0f);
+    return kInvSqrt2Pi * exp2_approx(z * z * (-0.5f * kLog2e)) * (2.0f - z * z);
+  }
+  return 0.0f;
 }
 // g <- g f'(z); the branch on the kind is outside the loop.
 template <int N>

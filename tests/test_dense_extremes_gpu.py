@@ -13,6 +13,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from create_graph_b200 import library  # noqa: F401  (registers the operators)
 from create_graph_b200 import native
 from create_graph_b200.dense import linear
 
@@ -147,3 +148,26 @@ def test_derivative_of_nan(n, act):
     assert torch.isnan(got[6])
     got[6] = clean[6]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_second_derivative_far_from_zero(act, dtype):
+    """f'' is 0 at both ends; bounds as for f'."""
+    z = torch.cat([far_values(dtype), torch.tensor([NAN], dtype=torch.float64)])
+    if act == "silu":
+        s = torch.sigmoid(z)
+        want = s * torch.sigmoid(-z) * (2.0 + z * (torch.sigmoid(-z) - s))
+    elif act == "gelu":
+        want = torch.exp(-0.5 * z * z) * (2.0 - z * z) / (2.0 * torch.pi) ** 0.5
+    else:
+        want = torch.zeros_like(z)
+    want = torch.where(z.abs() > 1e4, torch.zeros_like(z), want)  # below 1e-1000
+    one = torch.ones(1, z.numel(), dtype=dtype, device="cuda")
+    none = torch.zeros(z.numel(), dtype=dtype, device="cuda")
+    got = torch.ops.cg_b200.act_grad2(one, none, one.clone(), z.to(dtype).cuda()[None], act)[1].double().cpu()[0]
+    if act in ("silu", "gelu"):
+        assert torch.isnan(got[-1])
+    step = 2.0**-25 if dtype == torch.float16 else 0.0
+    error = (got - want)[:-1].abs()
+    assert (error <= 1.1 * UNIT[dtype] * want[:-1].abs() + 5.2e-6 + step).all(), z[error.argmax()]
