@@ -356,6 +356,7 @@ class _Linear(_Fused):
     @staticmethod
     def backward(ctx, gy, gz_direct):
         x, w, z, flat = ctx.saved_tensors
+        native.refuse_tangents("dense.linear", gy, gz_direct, x, w, z)
         want = _Linear._wanted(ctx)
         dr = gy if ctx.needs_input_grad[3] else None
         if not torch.is_grad_enabled() and gz_direct is None and gy is not None and ctx.operands is not None:
@@ -392,9 +393,11 @@ def _activation(who: str, name: str) -> int:
     return act
 
 
-def _checked_matrix(who: str, gy: Tensor, activation: str) -> int:
-    """The activation's code; refuses a gy that is no half-precision matrix on the GPU."""
+def _checked_matrix(who: str, gy: Tensor, activation: str, *others: Tensor) -> int:
+    """The activation's code; refuses a gy that is no half-precision matrix on
+    the GPU, and tangents of it or the others."""
     act = _activation(who, activation)
+    native.refuse_tangents(who, gy, *others)
     if gy.dim() != 2 or gy.dtype not in native.HALF_DTYPES:
         raise NativeError(f"{who}: a float16 or bfloat16 matrix expected, got {tuple(gy.shape)} {gy.dtype}")
     native.require_cuda(gy)
@@ -403,6 +406,7 @@ def _checked_matrix(who: str, gy: Tensor, activation: str) -> int:
 
 def _checked(x, weight, bias, residual, activation) -> int:
     act = _activation("dense.linear", activation)
+    native.refuse_tangents("dense.linear", x, weight, bias, residual)
     dtype, device = x.dtype, x.device
     if dtype not in native.HALF_DTYPES:
         raise NativeError(f"dense.linear: float16 or bfloat16 expected, got {dtype} (the fp32 layers are in "

@@ -396,7 +396,7 @@ def _dense_linear_fake(x, w, b, r, activation):
 @torch.library.custom_op("cg_b200::act_grad", mutates_args=())
 def act_grad(gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """(gy f'(z), the sums of its columns) of (M, N) half-precision tensors."""
-    act = dense._checked_matrix("act_grad", gy, activation)
+    act = dense._checked_matrix("act_grad", gy, activation, z)
     gz, db = dense._act_grad(gy, z, act, True)
     return (gy.clone() if gz.data_ptr() == gy.data_ptr() else gz.contiguous()), db
 
@@ -409,7 +409,7 @@ def _act_grad_fake(gy, z, activation):
 @torch.library.custom_op("cg_b200::act_grad2", mutates_args=())
 def act_grad2(h: Tensor, hb: Tensor, gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """((h + hb) f'(z), (h + hb) gy f''(z)) for cotangents h, hb of act_grad's outputs."""
-    return dense._act_grad2(h, hb, gy, z, dense._checked_matrix("act_grad2", gy, activation))
+    return dense._act_grad2(h, hb, gy, z, dense._checked_matrix("act_grad2", gy, activation, h, hb, z))
 
 
 @act_grad2.register_fake
@@ -468,6 +468,7 @@ act_grad.register_autograd(_act_grad_backward, setup_context=_act_grad_setup)
 def newton_schulz(x: Tensor, steps: int = 5, a: float = optim.NS_COEFFICIENTS[0], b: float = optim.NS_COEFFICIENTS[1],
                   c: float = optim.NS_COEFFICIENTS[2], eps: float = 1e-7) -> Tensor:
     """optim.newton_schulz (no gradient)."""
+    native.refuse_tangents("newton_schulz", x)
     with torch.no_grad():
         return optim.newton_schulz(x.detach(), steps, (a, b, c), eps)
 

@@ -15,6 +15,7 @@ import functools
 import pathlib
 
 import torch
+from torch.autograd import forward_ad
 
 from create_graph_b200.errors import NativeError
 
@@ -378,6 +379,16 @@ def require_cuda(*tensors: torch.Tensor) -> None:
                 "create_graph_b200 fused ops run on CUDA tensors only (no CPU fallback); got a "
                 f"{t.device} tensor"
             )
+
+
+def refuse_tangents(who: str, *tensors: torch.Tensor | None) -> None:
+    """Raise for tensors that carry a forward-mode tangent: a kernel called on
+    their memory would return a value without one."""
+    if forward_ad._current_level < 0:  # no dual level is open: the usual case
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NativeError(f"{who}: forward-mode derivatives are not supported")
 
 
 def device_error(reset: bool = False) -> int:

@@ -115,6 +115,7 @@ def newton_schulz(x: Tensor, steps: int = 5, coefficients: tuple[float, float, f
     iteration itself runs at fp32-level accuracy whatever the type, because it
     multiplies the error of the weak directions by a in every step. A matrix of
     zeros stays zero. Not differentiable."""
+    native.refuse_tangents("newton_schulz", x)
     native.require_cuda(x)
     if x.dim() < 2:
         raise NativeError(f"newton_schulz: a matrix or a stack of matrices expected, got {tuple(x.shape)}")
