@@ -126,6 +126,20 @@ __device__ inline double block_sum(double s) {
   return s;
 }
 
+// kScale / max(norm, eps), what the planes of an update are scaled by, as a power
+// of two and the rest: below a norm of 1.2e-35 the quotient alone leaves fp32's
+// range (and a matrix of zeros would become NaN), above 2^138 its normal numbers.
+struct PlaneScale {
+  float power, rest;
+  __device__ __forceinline__ float operator()(float v) const { return v * power * rest; }
+};
+__device__ inline PlaneScale plane_scale(double squares, float eps) {
+  const double norm = sqrt(squares), d = norm > (double)eps ? norm : (double)eps;
+  const double power = d < 0x1p-60 ? 0x1p64 : d > 0x1p60 ? 0x1p-64 : 1.0;
+  const float rest = isnan(squares) ? __int_as_float(0x7fc00000) : (float)((double)kScale / (d * power));
+  return {(float)power, rest};
+}
+
 }  // namespace muon
 }  // namespace cg
 
@@ -157,7 +171,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
   const int row0 = (int)(e0 / run.cols), col0 = (int)(e0 - (int64_t)row0 * run.cols);
   const int size = (int)(e0 + p.chunk < n ? p.chunk : n - e0);
   double sum = 0.0;
-  float scale = 0.0f;
+  PlaneScale scaled = {};
   __half *hi = nullptr, *lo = nullptr;
   if (NORM) {
     if (chunk == 0 && threadIdx.x == 0) {
@@ -169,9 +183,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     const double* part = p.partial + run.first_chunk + (int64_t)matrix * run.chunks;
     for (int c = threadIdx.x; c < run.chunks; c += 256) s += part[c];
     s = block_sum<8>(s);
-    const double norm = sqrt(s);
-    scale = (float)(kScale / (norm > (double)p.eps ? norm : (double)p.eps));
-    if (isnan(s)) scale = __int_as_float(0x7fc00000);
+    scaled = plane_scale(s, p.eps);
     hi = run.planes + (int64_t)matrix * 2 * run.rows * run.pitch;
     lo = hi + (int64_t)run.rows * run.pitch;
   }
@@ -214,7 +226,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
           __half h[4], l[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float f = v[g][q] * scale;
+            const float f = scaled(v[g][q]);
             h[q] = __float2half_rn(f);
             l[q] = __float2half_rn(f - __half2float(h[q]));
           }
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
       if (NORM) {
         sum += (double)v * v;
       } else {
-        const float f = v * scale;
+        const float f = scaled(v);
         const __half h = __float2half_rn(f);
         const int64_t o = (int64_t)row * run.pitch + col;
         hi[o] = h;

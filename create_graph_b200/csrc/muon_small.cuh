@@ -240,13 +240,11 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   half::cluster_sync_all();
   double total = 0.0;
   for (int r = 0; r < ranks; ++r) total += sums[r];
-  const double norm = sqrt(total);
-  float scale = (float)(kScale / (norm > (double)p.eps ? norm : (double)p.eps));
-  if (isnan(total)) scale = __int_as_float(0x7fc00000);
+  const PlaneScale scaled = plane_scale(total, p.eps);
 #pragma unroll
   for (int g = 0; g < kGroupsOf4; ++g) {
     const int at = g * kThreads + tid;
-    const float v[4] = {u[g][0] * scale, u[g][1] * scale, u[g][2] * scale, u[g][3] * scale};
+    const float v[4] = {scaled(u[g][0]), scaled(u[g][1]), scaled(u[g][2]), scaled(u[g][3])};
     uint2 h, l;
     split4(v, h, l);
     unsigned char* to = Z + plane_at(at >> 5, (at & 31) * 4);
