@@ -565,12 +565,37 @@ __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits
 // gz = gy f'(z) and the column sums of gz (the bias gradient) in one pass over
 // gy and z: block (x, y) owns 32 x V columns and the rows of chunk y; its eight
 // warps walk the rows, each lane adding up V columns in fp32, and the warps'
-// sums meet in shared memory in warp order. V = 8 (16-byte groups) or 1. Four
+// sums meet in shared memory in warp order. V = 8 where the columns are whole
+// groups, read value by value if the rows are not ALIGNED, so that neither gz nor
+// the sums depend on where they lie; else 1. Four
 // blocks an SM with two rows of a warp in flight: with five or six the registers
 // spill (229 and 267 us with silu), with three or two too little is in flight (205
 // and 245), one row at a time waits (236).
-template <class T, int V>
-__global__ void __launch_bounds__(256, V == 8 ? 4 : 1) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
+template <bool ALIGNED, class T>
+__device__ __forceinline__ uint4 load_group(const T* p) {
+  if (ALIGNED) return *reinterpret_cast<const uint4*>(p);
+  const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool ALIGNED, class T>
+__device__ __forceinline__ void store_group(T* p, uint4 v) {
+  if (ALIGNED) {
+    *reinterpret_cast<uint4*>(p) = v;
+    return;
+  }
+  unsigned short* h = reinterpret_cast<unsigned short*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[2 * i] = (unsigned short)w[i];
+    h[2 * i + 1] = (unsigned short)(w[i] >> 16);
+  }
+}
+template <class T, int V, bool ALIGNED>
+__global__ void __launch_bounds__(256, V == 8 && ALIGNED ? 4 : 1) act_grad_kernel(const T* __restrict__ gy, int64_t ld_gy,
                                                        const T* __restrict__ z, int64_t ld_z, T* __restrict__ gz,
                                                        int64_t ld_gz, int rows, int cols, int kind, int rows_per,
                                                        float* __restrict__ partial, T* __restrict__ db) {
@@ -590,8 +615,8 @@ __global__ void __launch_bounds__(256, V == 8 ? 4 : 1) act_grad_kernel(const T* 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (r + 8 * i >= r1) break;
-          ga[i] = *reinterpret_cast<const uint4*>(gy + (r + 8 * i) * ld_gy + col);
-          if (gz) za[i] = *reinterpret_cast<const uint4*>(z + (r + 8 * i) * ld_z + col);
+          ga[i] = load_group<ALIGNED>(gy + (r + 8 * i) * ld_gy + col);
+          if (gz) za[i] = load_group<ALIGNED>(z + (r + 8 * i) * ld_z + col);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -601,7 +626,7 @@ __global__ void __launch_bounds__(256, V == 8 ? 4 : 1) act_grad_kernel(const T* 
           if (gz) {
             unpack8<T>(za[i], x);
             act_grad_all(g, x, kind);
-            *reinterpret_cast<uint4*>(gz + (r + 8 * i) * ld_gz + col) = pack8<T>(g);
+            store_group<ALIGNED>(gz + (r + 8 * i) * ld_gz + col, pack8<T>(g));
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum[e] += g[e];
@@ -958,15 +983,17 @@ static int chunk_rows(int64_t rows, int64_t cols, int v) {
 
 template <class T>
 static int act_grad_typed(const cg_act_grad_args& g, cudaStream_t s) {
-  const bool vec = g.cols % 8 == 0 && aligned16(g.gy) && g.ld_gy % 8 == 0 &&
-                   (g.gz == nullptr || (aligned16(g.z) && aligned16(g.gz) && g.ld_z % 8 == 0 && g.ld_gz % 8 == 0));
+  const bool vec = g.cols % 8 == 0;
+  const bool aligned = aligned16(g.gy) && g.ld_gy % 8 == 0 &&
+                       (g.gz == nullptr || (aligned16(g.z) && aligned16(g.gz) && g.ld_z % 8 == 0 && g.ld_gz % 8 == 0));
   const int per = chunk_rows(g.rows, g.cols, vec ? 8 : 1);
   const int chunks = (int)ceil_div<int64_t>(g.rows, per);
   const dim3 grid((unsigned)ceil_div<int64_t>(g.cols, vec ? 256 : 32), (unsigned)chunks);
   const bool direct = chunks == 1;
   float* partial = g.db && !direct ? g.scratch : nullptr;
   T* db = g.db && direct ? (T*)g.db : nullptr;
-  auto kernel = vec ? act_grad_kernel<T, 8> : act_grad_kernel<T, 1>;
+  auto kernel = !vec ? act_grad_kernel<T, 1, false>
+                : aligned ? act_grad_kernel<T, 8, true> : act_grad_kernel<T, 8, false>;
   if (int rc = half::launch_chained("act_grad_half", kernel, grid, 256, 0, dim3(1, 1), s, (const T*)g.gy, g.ld_gy,
                                     (const T*)g.z, g.ld_z, (T*)g.gz, g.ld_gz, (int)g.rows, (int)g.cols, g.act, per,
                                     partial, db))
