@@ -112,11 +112,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// Beyond +-43 silu, gelu and their derivatives are at their limits.
+constexpr float kFar = 43.0f;
 // z held to [-most, most]; NaN stays NaN.
 __device__ __forceinline__ float hold_nan(float z, float most) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(max_nan(z, -most)), "f"(most));
   return r;
+}
+
+// Eight values held to [-43, 43].
+__device__ __forceinline__ uint32_t hold_two(uint32_t u, __half) {
+  const __half2 far = __float2half2_rn(kFar);
+  const __half2 r = __hmin2_nan(__hmax2_nan(*reinterpret_cast<const __half2*>(&u), __hneg2(far)), far);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hold_two(uint32_t u, __nv_bfloat16) {
+  const __nv_bfloat162 far = __float2bfloat162_rn(kFar);
+  const __nv_bfloat162 r = __hmin2_nan(__hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&u), __hneg2(far)), far);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <class T>
+__device__ __forceinline__ uint4 hold_group(uint4 v) {
+  return make_uint4(hold_two(v.x, T()), hold_two(v.y, T()), hold_two(v.z, T()), hold_two(v.w, T()));
 }
 
 // Two fp32 values per instruction.
@@ -150,9 +168,8 @@ __device__ __forceinline__ float2 rcp2(float2 d) {
 // 2^-x stays below 2^62 for the pair's reciprocal; below it, down to -infinity,
 // silu is smaller still and 0 in the limit. A NaN stays in z and does not enter
 // the reciprocal, which is the other value's too.
-constexpr float kSiluFar = 43.0f;
 __device__ __forceinline__ float2 silu2(float2 z) {
-  z = make_float2(max_nan(z.x, -kSiluFar), max_nan(z.y, -kSiluFar));
+  z = make_float2(max_nan(z.x, -kFar), max_nan(z.y, -kFar));
   const float2 x = mul2(z, both(-kLog2e));
   const float2 e = make_float2(exp2_approx(fminf(x.x, 62.0f)), exp2_approx(fminf(x.y, 62.0f)));
   return mul2(z, rcp2(make_float2(1.0f + e.x, 1.0f + e.y)));
@@ -182,15 +199,15 @@ __device__ __forceinline__ float2 gelu2(float2 z) {
   return fma2(mul2(a, r), r, make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)));
 }
 
-// f' of two values. At the bounds that z is held to, f' is 0 to 1e-17 or 1, its
-// limits at the infinities: a pre-activation that left the range of its type and
-// was kept as -infinity (fp16 below -65504) has the gradient 0 that goes with its
-// output 0. silu's 1 - s is off by an ulp, times z: 5e-6 at the most once z is held.
+// f' of two values within [-43, 43] (hold_nan, hold_group): at the bounds f' is 0
+// to 1e-17 or 1, its limits at the infinities, so a pre-activation that left the
+// range of its type and was kept as -infinity (fp16 below -65504) has the gradient
+// 0 that goes with its output 0. silu's 1 - s is off by an ulp, times z: 5e-6 at
+// the most.
 __device__ __forceinline__ float2 silu_grad2(float2 z) {
-  z = make_float2(hold_nan(z.x, kSiluFar), hold_nan(z.y, kSiluFar));
   const float2 x = mul2(z, both(-kLog2e));
   const float2 e = make_float2(exp2_approx(fminf(x.x, 62.0f)), exp2_approx(fminf(x.y, 62.0f)));
-  const float2 s = rcp2(make_float2(1.0f + e.x, 1.0f + e.y));
+  const float2 s = rcp2(fma2(e, both(1.0f), both(1.0f)));
   // s (1 + z (1 - s)) = s + (z s - z s s)
   const float2 zs = mul2(z, s);
   return fma2(fma2(zs, make_float2(-s.x, -s.y), zs), both(1.0f), s);
@@ -207,30 +224,30 @@ __device__ __forceinline__ float2 gelu_grad2(float2 z) {
   const float2 tail = mul2(mul2(p, t), e);
   // Phi(z) = 1/2 + sign(z) (1/2 - tail)
   const float2 phi = make_float2(0.5f + copysignf(0.5f - tail.x, z.x), 0.5f + copysignf(0.5f - tail.y, z.y));
-  z = make_float2(hold_nan(z.x, 64.0f), hold_nan(z.y, 64.0f));
   return fma2(mul2(z, both(kInvSqrt2Pi)), e, phi);
 }
-// f' of one value, as act_grad_all's.
+// f' of one value.
 __device__ __forceinline__ float act_grad(float z, int kind) {
-  if (kind == CG_ACT_SILU) return silu_grad2(both(z)).x;
-  if (kind == CG_ACT_GELU) return gelu_grad2(both(z)).x;
   if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  z = hold_nan(z, kFar);
+  if (kind == CG_ACT_SILU) {
+    const float s = sigmoid(z);
+    return s * (1.0f + z * (1.0f - s));
+  }
+  if (kind == CG_ACT_GELU) return gelu_grad2(both(z)).x;
   return 1.0f;
 }
 // f'' of one value, with z held as in f': its square would leave fp32.
 __device__ __forceinline__ float act_grad2(float z, int kind) {
+  z = hold_nan(z, kFar);
   if (kind == CG_ACT_SILU) {
-    z = hold_nan(z, kSiluFar);
     const float s = sigmoid(z);
     return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
   }
-  if (kind == CG_ACT_GELU) {
-    z = hold_nan(z, 64.0f);
-    return kInvSqrt2Pi * exp2_approx(z * z * (-0.5f * kLog2e)) * (2.0f - z * z);
-  }
+  if (kind == CG_ACT_GELU) return kInvSqrt2Pi * exp2_approx(z * z * (-0.5f * kLog2e)) * (2.0f - z * z);
   return 0.0f;
 }
-// g <- g f'(z); the branch on the kind is outside the loop.
+// g <- g f'(z), z within [-43, 43]; the branch on the kind is outside the loop.
 template <int N>
 __device__ __forceinline__ void act_grad_all(float (&g)[N], const float (&z)[N], int kind) {
   if (kind == CG_ACT_RELU) {
@@ -624,7 +641,7 @@ __global__ void __launch_bounds__(256, V == 8 && ALIGNED ? 4 : 1) act_grad_kerne
           float g[8], x[8];
           unpack8<T>(ga[i], g);
           if (gz) {
-            unpack8<T>(za[i], x);
+            unpack8<T>(hold_group<T>(za[i]), x);
             act_grad_all(g, x, kind);
             store_group<ALIGNED>(gz + (r + 8 * i) * ld_gz + col, pack8<T>(g));
           }
