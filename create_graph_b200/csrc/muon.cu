@@ -35,6 +35,8 @@ using namespace cg::sm100;
 
 // device error word of this translation unit's kernels
 __device__ int g_muon_error = 0;
+// a diagonal of nothing (see SplitEpi)
+__device__ __align__(16) float g_zeros[32];
 
 constexpr int kGroups = 8;         // shapes per launch
 constexpr int kEntries = 24;       // runs of matrices per prepare launch
@@ -111,6 +113,33 @@ struct Momentum {
   __device__ float next(float m, float g) const { return m + (1.0f - mu) * (g - m); }
   __device__ float update(float m, float g) const { return nesterov ? m + (1.0f - mu) * (g - m) : m; }
 };
+
+// Two fp32 values per instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Sum over a block of WARPS warps in a fixed order.
 template <int WARPS>
@@ -272,6 +301,10 @@ struct EpiArgs {
   int has_aux;
   float alpha, beta;  // alpha aux + beta accumulator
   float diagonal;     // added on the diagonal (of a symmetric result)
+  // diagonals of (batch, up(m, 32)): where the result's goes, its planes getting
+  // zeros; the one that operands and aux lack (see SplitEpi)
+  float* take;
+  const float* apart;
   int lower;          // symmetric result
   // final epilogue: out <- keep out + rate value (keep = 0: out is not read)
   const OutRef* table;
@@ -367,9 +400,13 @@ struct EpiBase {
   __device__ __forceinline__ static uint4* group(unsigned char* at, int p, int r, int c) {
     return reinterpret_cast<uint4*>(at + p * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
   }
-  // v <- alpha aux + beta v
-  __device__ __forceinline__ bool values(float (&v)[32], int q, int* error) {
-    const float alpha = a->alpha, beta = a->beta;
+  // 32 consecutive values of the diagonal kept apart, zeros where there is none
+  __device__ __forceinline__ const float* kept(int first) const {
+    return a->apart != nullptr ? a->apart + (int64_t)batch * ((m + 31) & ~31) + first : g_zeros;
+  }
+  // v <- (alpha + beta (d_row + d_column)) aux + beta v, d the diagonal kept apart
+  __device__ __forceinline__ bool values(float (&v)[32], int col0, int q, int* error) {
+    const float beta = a->beta;
     if (!a->has_aux) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] *= beta;
@@ -379,18 +416,24 @@ struct EpiBase {
       pending = true;
       later = false;
     }
+    const float* d = kept(col0);
+    const float alpha = a->alpha + beta * kept(row0)[lane];
     const bool ok = arrived(error);
     unsigned char* at = block(q);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
+      const float4 d0 = reinterpret_cast<const float4*>(d)[2 * c], d1 = reinterpret_cast<const float4*>(d)[2 * c + 1];
+      const float2 dw[4] = {{d0.x, d0.y}, {d0.z, d0.w}, {d1.x, d1.y}, {d1.z, d1.w}};
       const uint4 h = *group(at, 0, lane, c), l = *group(at, 1, lane, c);
       const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw[i]));
         const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lw[i]));
-        v[8 * c + 2 * i] = alpha * (x.x + y.x) + beta * v[8 * c + 2 * i];
-        v[8 * c + 2 * i + 1] = alpha * (x.y + y.y) + beta * v[8 * c + 2 * i + 1];
+        float* to = v + 8 * c + 2 * i;
+        const float2 r = fma2(fma2(both(beta), dw[i], both(alpha)), add2(x, y), mul2(both(beta), make_float2(to[0], to[1])));
+        to[0] = r.x;
+        to[1] = r.y;
       }
     }
     return ok;
@@ -412,6 +455,17 @@ __device__ __forceinline__ void store_matrices(void* row, const uint32_t (&v)[4]
 }
 
 // The result as planes, for the next product.
+// The tensor core truncates as it adds. Of A A that would bite on the diagonal,
+// one large square and many small terms, all positive, each cut at the square's
+// last bit. So the gram's diagonal d is kept apart in fp32: its planes hold N = A -
+// diag(d), and with beta the factor of A A
+//   (A A)_ij = (N N)_ij + N_ij (d_i + d_j) + [i = j] d_i^2:
+// alpha A + beta A A takes alpha + beta (d_i + d_j) for alpha, and d_i (alpha +
+// beta d_i) more on the diagonal. Relative errors (torch's fp32 products): 55 x
+// 2364 Gaussian 1.0e-6 (1.4e-6), 55 x 600 1.0e-6 (1.9e-6), 55 orthogonal rows of
+// 2364 0.5e-6 (0.7e-6), with d in the product and a fitted factor on it 1.6e-6,
+// 2.7e-6 and 3.3e-6. It costs the polynomial's epilogue two reads of d a block:
+// 12 x 768 x 768 499 -> 507 us, 3 x 257 x 1031 172 -> 175, the 85M step nothing.
 struct SplitEpi : EpiBase {
   using EpiBase::EpiBase;
   __device__ __forceinline__ void put(unsigned char* at, int col, int row) {
@@ -424,11 +478,7 @@ struct SplitEpi : EpiBase {
   }
   __device__ __forceinline__ bool store(float (&v)[32], int col0, int q, int* error) {
     if (outside(col0)) return true;
-    const bool ok = values(v, q, error);
-    if (a->diagonal != 0.0f && row0 == col0) {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] += e == lane ? a->diagonal : 0.0f;
-    }
+    const bool ok = values(v, col0, q, error);
     // hi = fp16(v), lo = fp16(v - hi)
     uint32_t hi[16], lo[16];
 #pragma unroll
@@ -444,6 +494,20 @@ struct SplitEpi : EpiBase {
     for (int c = 0; c < 4; ++c) {
       *group(at, 0, lane, c) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
       *group(at, 1, lane, c) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+    }
+    if (a->lower && row0 == col0) {  // this row's place on the diagonal
+      __half* h = reinterpret_cast<__half*>(group(at, 0, lane, lane >> 3)) + (lane & 7);
+      __half* l = h + 1024;
+      float x = __half2float(*h) + __half2float(*l);
+      if (a->take != nullptr) {
+        a->take[(int64_t)batch * ((m + 31) & ~31) + row0 + lane] = x;  // 0 beyond m
+        x -= x;                                                        // 0, or NaN where it is not finite
+      } else {
+        const float d = kept(row0)[lane];
+        x += d * (a->alpha + a->beta * d) + a->diagonal;
+      }
+      *h = __float2half_rn(x);
+      *l = __float2half_rn(x - __half2float(*h));
     }
     put(at, col0, row0);
     if (a->lower && row0 != col0) {  // the mirror block, transposed 8 x 8 values at a time
@@ -506,7 +570,7 @@ struct FinalEpi : EpiBase {
   // rows of the caller's matrices: fp32 blocks through shared memory
   __device__ __forceinline__ bool store(float (&v)[32], int col0, int q, int* error) {
     if (outside(col0)) return true;
-    const bool ok = values(v, q, error);
+    const bool ok = values(v, col0, q, error);
     float* stage = reinterpret_cast<float*>(block(q));
     __syncwarp();  // every row of the planes has been read
 #pragma unroll
@@ -566,6 +630,7 @@ struct Shape {
   int64_t rows, cols, count;
   int64_t s, pitch, spitch;
   __half *x0, *x1, *gram, *poly;
+  float* diagonal;  // of the gram, (count, up(s, 32))
   int64_t first_matrix;
 };
 
@@ -707,6 +772,7 @@ static int64_t layout(Shape* shapes, int n, char* base, Buffers* b) {
     h.x1 = reinterpret_cast<__half*>(take(x));
     h.gram = reinterpret_cast<__half*>(take(s));
     h.poly = reinterpret_cast<__half*>(take(s));
+    h.diagonal = reinterpret_cast<float*>(take(h.count * up(h.s, 32) * (int64_t)sizeof(float)));
   }
   b->squares = reinterpret_cast<double*>(take(chunks * (int64_t)sizeof(double)));
   b->table = reinterpret_cast<OutRef*>(take(matrices * (int64_t)sizeof(OutRef)));
@@ -847,6 +913,7 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       G.m = G.n = (int)h.s;
       G.k = (int)(wide ? h.cols : h.rows);
       e.beta = 1.0f / kScale;
+      e.take = h.diagonal;
     } else if (step == kPoly) {
       map_s(&G.map_a, h.gram, a_box);
       map_s(&G.map_b, h.gram, b_box);
@@ -854,13 +921,8 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       blocks_s(&e.map_out, h.poly);
       G.m = G.n = G.k = (int)h.s;
       e.alpha = g.b;
-      // The tensor core aligns an instruction's products to the largest and
-      // truncates. The diagonal of A A is one large square and many small ones, all
-      // positive, and came out about 6e-9 low per term of an accumulator (fitted to
-      // 55 x 2364, whose directions all follow one path: 1.6e-6 low together without
-      // this); the other products' small terms have either sign.
-      const int64_t terms = h.s < half::kBK * L.sum_slices ? h.s : half::kBK * L.sum_slices;
-      e.beta = g.c / kScale * (1.0f + 6e-9f * (float)terms);
+      e.beta = g.c / kScale;
+      e.apart = h.diagonal;
       e.diagonal = coarse ? g.a * kScale : 0.0f;
     } else {
       if (wide) {

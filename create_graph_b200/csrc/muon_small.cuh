@@ -7,15 +7,16 @@
 //   G  = Z Z^T (tall: Z^T Z), summed over the cluster through distributed
 //        shared memory: each CTA adds up its share of the partial sums in rank
 //        order and writes the planes of its share to every CTA;
-//   P  = b A + c A A, formed by every CTA for itself, over A's planes;
+//   P  = b A + c A A, formed by every CTA for itself, over A's planes (which lack
+//        the diagonal, as the tiled products' do: see SplitEpi in muon.cu);
 //   Z <- a Z + P Z (tall: a Z + Z P), in place.
 // Each product is 24 UMMAs of 128 x 128 x 16 (lo hi, hi lo and hi hi over k =
 // 128), issued by one thread from operands that all lie in shared memory: a
 // tile of 128-byte swizzled rows is a K-major operand along its columns and an
 // MN-major one along its rows, so Z serves both products as it is stored.
 // What bounds it is the chain of 3 products and 3 passes over the tile per
-// step, not bandwidth or tensor throughput: 35 us for one to 148 matrices of 128 x
-// 128 (2.2 us a product), 59 us with clusters of four (the exchange takes 5 us a
+// step, not bandwidth or tensor throughput: 37 us for one to 148 matrices of 128 x
+// 128 (2.3 us a product), 61 us with clusters of four (the exchange takes 5 us a
 // step); as 17 launches over the batch the same steps took 127 and 150 us.
 #pragma once
 
@@ -53,7 +54,8 @@ struct Smem {
   static constexpr int kZ = 0;                       // two planes
   static constexpr int kA = 2 * kPlane;              // two planes (A, then P)
   static constexpr int kPart = 4 * kPlane;           // 128 x 128 fp32
-  static constexpr int kBar = kPart + kSide * kSide * 4;
+  static constexpr int kDiagonal = kPart + kSide * kSide * 4;  // of A, fp32; its planes hold zeros there
+  static constexpr int kBar = kDiagonal + kSide * 4;
   static constexpr int kBytes = kBar + 256 + 1024 /*alignment*/;
 };
 static_assert(Smem::kBytes <= 227 * 1024, "shared memory budget");
@@ -117,14 +119,23 @@ __device__ inline void issue_product(uint32_t acc, uint32_t a, bool a_mn, uint32
     half::umma_f16<1>(acc, desc(a, a_mn, kk), desc(b, b_mn, kk), idesc, true);
 }
 
+// The factor of two of a row's 32 plane values: the same for all, or one each.
+struct One {
+  float alpha;
+  __device__ __forceinline__ float2 pair(int) const { return both(alpha); }
+};
+struct Each {
+  float2 f[16];
+  __device__ __forceinline__ float2 pair(int i) const { return f[i]; }
+};
+
 // alpha planes(row, 32 columns) + beta v over the planes' own place; returns v.
-template <bool AUX, bool STORE>
-__device__ __forceinline__ void blend_row(unsigned char* planes, int row, int col0, float alpha, float beta,
+template <bool AUX, bool STORE, class Factor>
+__device__ __forceinline__ void blend_row(unsigned char* planes, int row, int col0, const Factor& alpha, float beta,
                                           float (&v)[32]) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     unsigned char* at = planes + plane_at(row, col0 + 8 * g);
-    float x[8];
     if (AUX) {
       const uint4 h = *reinterpret_cast<const uint4*>(at), l = *reinterpret_cast<const uint4*>(at + kPlane);
       const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
@@ -132,12 +143,15 @@ __device__ __forceinline__ void blend_row(unsigned char* planes, int row, int co
       for (int i = 0; i < 4; ++i) {
         const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&hw[i]));
         const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&lw[i]));
-        x[2 * i] = p.x + q.x;
-        x[2 * i + 1] = p.y + q.y;
+        float* to = v + 8 * g + 2 * i;
+        const float2 r = fma2(alpha.pair(4 * g + i), add2(p, q), mul2(both(beta), make_float2(to[0], to[1])));
+        to[0] = r.x;
+        to[1] = r.y;
       }
-    }
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[8 * g + e] = AUX ? alpha * x[e] + beta * v[8 * g + e] : beta * v[8 * g + e];
+      for (int e = 0; e < 8; ++e) v[8 * g + e] *= beta;
+    }
     if (STORE) {
       uint2 h0, l0, h1, l1;
       const float u0[4] = {v[8 * g], v[8 * g + 1], v[8 * g + 2], v[8 * g + 3]};
@@ -148,6 +162,18 @@ __device__ __forceinline__ void blend_row(unsigned char* planes, int row, int co
       *reinterpret_cast<uint4*>(at + kPlane) = make_uint4(l0.x, l0.y, l1.x, l1.y);
     }
   }
+}
+
+// The value at (r, r) of the planes.
+__device__ __forceinline__ float plane_value(const unsigned char* planes, int r) {
+  const unsigned char* at = planes + plane_at(r, r);
+  return __half2float(*reinterpret_cast<const __half*>(at)) + __half2float(*reinterpret_cast<const __half*>(at + kPlane));
+}
+__device__ __forceinline__ void put_plane_value(unsigned char* planes, int r, float x) {
+  unsigned char* at = planes + plane_at(r, r);
+  const __half h = __float2half_rn(x);
+  *reinterpret_cast<__half*>(at) = h;
+  *reinterpret_cast<__half*>(at + kPlane) = __float2half_rn(x - __half2float(h));
 }
 
 // 32 values of a row into the fp32 block.
@@ -165,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
                                                          ~uintptr_t(1023));
   unsigned char *Z = smem + Smem::kZ, *A = smem + Smem::kA;
   float4* part = reinterpret_cast<float4*>(smem + Smem::kPart);
+  float* diagonal = reinterpret_cast<float*>(smem + Smem::kDiagonal);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Smem::kBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
   double* sums = reinterpret_cast<double*>(bar + 2);  // one per CTA of the cluster
@@ -259,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   uint32_t phase = 0;
   // one product: what the threads wrote is visible to the tensor core, and the
   // accumulator to the threads after it
-  auto product = [&](const unsigned char* a, bool a_mn, const unsigned char* b, bool b_mn) {
+  // (meanwhile: what the threads do beside the tensor core)
+  auto product = [&](const unsigned char* a, bool a_mn, const unsigned char* b, bool b_mn, auto meanwhile) {
     fence_proxy_async_all();
     tc_fence_before();
     __syncthreads();
@@ -271,16 +299,19 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
       }
       __syncwarp();
     }
+    meanwhile();
     half::wait(bar, phase & 1, &g_muon_error);
     ++phase;
     tc_fence_after();
   };
+  const auto nothing = [] {};
+  const bool on_diagonal = 32 * quarter == col0;  // this warp's block
   for (int t = 0; t < p.steps; ++t) {
-    product(Z, !wide, Z, !wide);
+    product(Z, !wide, Z, !wide, nothing);
     float v[32];
     tmem_load_32(acc, v);
     if (ranks == 1) {
-      blend_row<false, true>(A, row, col0, 0.0f, 1.0f / kScale, v);
+      blend_row<false, true>(A, row, col0, One{0.0f}, 1.0f / kScale, v);
     } else {
       put_row(part, row, col0, v);
       half::cluster_sync_all();
@@ -313,16 +344,33 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
       }
       half::cluster_sync_all();
     }
-    product(A, false, A, false);
+    if (on_diagonal) {  // the diagonal apart
+      const float d = plane_value(A, row);
+      diagonal[row] = d;
+      put_plane_value(A, row, d - d);  // 0, or NaN where it is not finite
+    }
+    Each factor;
+    float more;
+    product(A, false, A, false, [&] {  // b + c (d_row + d_column), and the diagonal's own term
+      const float beta = p.c / kScale, mine = diagonal[row], alpha = p.b + beta * mine;
+      more = mine * alpha;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const float4 d = *reinterpret_cast<const float4*>(diagonal + col0 + 4 * g);
+        factor.f[2 * g] = fma2(both(beta), make_float2(d.x, d.y), both(alpha));
+        factor.f[2 * g + 1] = fma2(both(beta), make_float2(d.z, d.w), both(alpha));
+      }
+    });
     tmem_load_32(acc, v);
-    blend_row<true, true>(A, row, col0, p.b, p.c / kScale, v);
-    if (wide) product(A, false, Z, true);
-    else product(Z, false, A, false);
+    blend_row<true, true>(A, row, col0, factor, p.c / kScale, v);
+    if (on_diagonal) put_plane_value(A, row, more + plane_value(A, row));
+    if (wide) product(A, false, Z, true, nothing);
+    else product(Z, false, A, false, nothing);
     tmem_load_32(acc, v);
     if (t + 1 < p.steps) {
-      blend_row<true, true>(Z, row, col0, p.a, 1.0f / kScale, v);
+      blend_row<true, true>(Z, row, col0, One{p.a}, 1.0f / kScale, v);
     } else {
-      blend_row<true, false>(Z, row, col0, p.a / kScale, 1.0f / (kScale * kScale), v);
+      blend_row<true, false>(Z, row, col0, One{p.a / kScale}, 1.0f / (kScale * kScale), v);
       put_row(part, row, col0, v);
     }
   }
