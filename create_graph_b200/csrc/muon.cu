@@ -12,7 +12,7 @@
 // the weak directions of a low-rank gradient: five steps of fp16 products
 // measured 6e-3 and of bf16 products 5e-2 relative error on a 32-direction
 // gradient with noise. Every matrix is therefore kept as a pair of fp16 planes
-// hi + lo, scaled by 2^12 (entries of X, A and B stay below 16; lo keeps 22
+// hi + lo, scaled by 2^12 (entries of X, A and B below 16; lo keeps 22
 // significant bits down to entries of 2^-14), and each product is made of the
 // three plane products lo hi + hi lo + hi hi in fp32 accumulators: fp32-level
 // accuracy (1e-6) at a third of the half-precision rate, twice the rate of three
@@ -41,7 +41,11 @@ __device__ __align__(16) float g_zeros[32];
 constexpr int kGroups = 8;         // shapes per launch
 constexpr int kEntries = 24;       // runs of matrices per prepare launch
 constexpr int kMostChunk = 8192;   // elements per block of the prepare passes
-constexpr float kScale = 4096.0f;  // of the stored planes
+
+// What the planes of X, A and B are scaled by (see scales_of).
+struct Scales {
+  float x, a, b;
+};
 
 struct OutRef {
   void* ptr;
@@ -66,7 +70,7 @@ struct Run {
 struct Prepare {
   Run run[kEntries];
   int runs;
-  float eps, mu;
+  float eps, mu, scale;
   int nesterov;
   int chunk;                // elements per block
   double* partial;
@@ -155,17 +159,17 @@ __device__ inline double block_sum(double s) {
   return s;
 }
 
-// kScale / max(norm, eps), what the planes of an update are scaled by, as a power
+// scale / max(norm, eps), what the planes of an update are scaled by, as a power
 // of two and the rest: below a norm of 1.2e-35 the quotient alone leaves fp32's
 // range (and a matrix of zeros would become NaN), above 2^138 its normal numbers.
 struct PlaneScale {
   float power, rest;
   __device__ __forceinline__ float operator()(float v) const { return v * power * rest; }
 };
-__device__ inline PlaneScale plane_scale(double squares, float eps) {
+__device__ inline PlaneScale plane_scale(double squares, float eps, float scale) {
   const double norm = sqrt(squares), d = norm > (double)eps ? norm : (double)eps;
   const double power = d < 0x1p-60 ? 0x1p64 : d > 0x1p60 ? 0x1p-64 : 1.0;
-  const float rest = isnan(squares) ? __int_as_float(0x7fc00000) : (float)((double)kScale / (d * power));
+  const float rest = isnan(squares) ? __int_as_float(0x7fc00000) : (float)((double)scale / (d * power));
   return {(float)power, rest};
 }
 
@@ -181,7 +185,7 @@ namespace muon {
 // 6.6 TB/s, in the first pass, 85 us in the second).
 // NORM: advance the momentum and leave each chunk's sum of squares (in 64
 // bits: squares of gradients may leave the range of 32). Otherwise: read the
-// update again, scale it by 2^12 / max(norm, eps) and write its planes.
+// update again, scale it (plane_scale) and write its planes.
 // Block = one chunk of kChunk elements of one matrix.
 template <class T, bool MOMENTUM, bool NORM>
 __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Prepare p) {
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
     const double* part = p.partial + run.first_chunk + (int64_t)matrix * run.chunks;
     for (int c = threadIdx.x; c < run.chunks; c += 256) s += part[c];
     s = block_sum<8>(s);
-    scaled = plane_scale(s, p.eps);
+    scaled = plane_scale(s, p.eps, p.scale);
     hi = run.planes + (int64_t)matrix * 2 * run.rows * run.pitch;
     lo = hi + (int64_t)run.rows * run.pitch;
   }
@@ -738,6 +742,41 @@ static Plan plan_of(const Shape* shapes, int n, Step step, bool coarse) {
   return best;
 }
 
+// The planes hold entries below 16 at a scale of 2^12, the published coefficients'
+// by far; others may let X, A or B grow, and get the largest power of two that
+// keeps them in fp16's range, up to entries of 10^9. The singular values of X start
+// at 1 at most and follow s -> |a s + b s^3 + c s^5|, an entry is no larger than
+// the largest of them, and the last step's result is fp32.
+static Scales scales_of(const cg_ns_args& g, bool coarse) {
+  const double a = g.a, b = g.b, c = g.c;
+  double x = 1.0, most_x = 1.0, most_a = 1.0, most_b = 0.0;
+  auto larger = [](double m, double v) { return !(fabs(v) < m) ? fmin(fabs(v), 1e9) : m; };
+  for (int t = 0; t < g.steps; ++t) {
+    const double s1 = x * x;
+    most_x = larger(most_x, x);
+    most_a = larger(most_a, s1);
+    // b s + c s^2 (and a) over [0, s1]: its ends and its vertex
+    const double free = coarse ? a : 0.0, vertex = c != 0.0 ? -b / (2.0 * c) : 0.0;
+    for (double s : {0.0, vertex > 0.0 && vertex < s1 ? vertex : 0.0, s1})
+      most_b = larger(most_b, free + s * (b + c * s));
+    // a s + b s^3 + c s^5 over [0, x]: its end and where a + 3 b s^2 + 5 c s^4 = 0
+    double next = larger(0.0, x * (a + s1 * (b + c * s1)));
+    const double root = 9.0 * b * b - 20.0 * a * c;
+    if (root >= 0.0) {
+      const double q = -0.5 * (3.0 * b + copysign(sqrt(root), b));
+      for (double s : {5.0 * c != 0.0 ? q / (5.0 * c) : 0.0, q != 0.0 ? a / q : 0.0})
+        if (s > 0.0 && s < s1) next = larger(next, sqrt(s) * (a + s * (b + c * s)));
+    }
+    x = next;
+  }
+  auto scale = [](double most) {
+    float s = 4096.0f;
+    while (most * s > 61440.0) s *= 0.5f;  // most is 1e9 at the most
+    return s;
+  };
+  return {scale(most_x), scale(most_a), scale(most_b)};
+}
+
 struct Buffers {
   double* squares;
   OutRef* table;
@@ -802,7 +841,7 @@ static int64_t workspace_bytes(const cg_ns_args& g) {
 }
 
 template <class T, bool MOMENTUM>
-static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, int n, const Buffers& b,
+static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, int n, const Buffers& b, float scale,
                    cudaStream_t s) {
   // both passes need every run's place: the first walks all launches, then the second
   for (int pass = 0; pass < 2; ++pass) {
@@ -811,6 +850,7 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
     Prepare p;
     memset(&p, 0, sizeof(p));
     p.eps = g.eps;
+    p.scale = scale;
     p.mu = g.momentum;
     p.nesterov = g.nesterov;
     p.table = b.table;
@@ -870,7 +910,8 @@ static int prepare(const cg_ns_args& g, int from, int to, const Shape* shapes, i
 // X' = a X + B X (a X + X B).
 template <int CG, int BN, class E>
 static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Plan& plan, const Buffers& b,
-                   bool coarse, bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
+                   const Scales& scales, bool coarse, bool odd, bool last, float keep, const float* rate,
+                   cudaStream_t s) {
   half::LaunchOf<E> L;
   memset(&L, 0, sizeof(L));
   L.partial = b.partial;
@@ -912,7 +953,7 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       blocks_s(&e.map_out, h.gram);
       G.m = G.n = (int)h.s;
       G.k = (int)(wide ? h.cols : h.rows);
-      e.beta = 1.0f / kScale;
+      e.beta = scales.a / (scales.x * scales.x);
       e.take = h.diagonal;
     } else if (step == kPoly) {
       map_s(&G.map_a, h.gram, a_box);
@@ -920,10 +961,10 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       blocks_s(&e.map_aux, h.gram);
       blocks_s(&e.map_out, h.poly);
       G.m = G.n = G.k = (int)h.s;
-      e.alpha = g.b;
-      e.beta = g.c / kScale;
+      e.alpha = g.b * (scales.b / scales.a);
+      e.beta = g.c * (scales.b / (scales.a * scales.a));
       e.apart = h.diagonal;
-      e.diagonal = coarse ? g.a * kScale : 0.0f;
+      e.diagonal = coarse ? g.a * scales.b : 0.0f;
     } else {
       if (wide) {
         map_s(&G.map_a, h.poly, a_box);
@@ -939,15 +980,15 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
       G.n = (int)h.cols;
       G.k = (int)h.s;
       e.alpha = g.a;
-      e.beta = 1.0f / kScale;
+      e.beta = 1.0f / scales.b;
     }
     if (rc) return rc;
     e.has_aux = step == kPoly || (step == kUpdate && !coarse);
     e.lower = G.lower = step != kUpdate;
     if (last) {  // leaves the planes' scale
       e.table = b.table + h.first_matrix;
-      e.alpha /= kScale;
-      e.beta /= kScale;
+      e.alpha /= scales.x;
+      e.beta /= scales.x;
       e.keep = keep;
       e.rate = rate[i];
     }
@@ -970,12 +1011,13 @@ static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, c
 
 template <class E>
 static int product(const cg_ns_args& g, const Shape* shapes, int n, Step step, const Plan* plans, const Buffers& b,
-                   bool coarse, bool odd, bool last, float keep, const float* rate, cudaStream_t s) {
+                   const Scales& scales, bool coarse, bool odd, bool last, float keep, const float* rate,
+                   cudaStream_t s) {
   const Plan& p = plans[step];
-  if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
-  if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
-  if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
-  return product<1, 64, E>(g, shapes, n, step, p, b, coarse, odd, last, keep, rate, s);
+  if (p.cg == 2 && p.bn == 256) return product<2, 256, E>(g, shapes, n, step, p, b, scales, coarse, odd, last, keep, rate, s);
+  if (p.cg == 2) return product<2, 128, E>(g, shapes, n, step, p, b, scales, coarse, odd, last, keep, rate, s);
+  if (p.bn == 128) return product<1, 128, E>(g, shapes, n, step, p, b, scales, coarse, odd, last, keep, rate, s);
+  return product<1, 64, E>(g, shapes, n, step, p, b, scales, coarse, odd, last, keep, rate, s);
 }
 
 static float rate_of(const cg_ns_args& g, bool momentum, int64_t rows, int64_t cols) {
@@ -1004,10 +1046,14 @@ static int run_small(const cg_ns_args& g, cudaStream_t s) {
     small::Args p;
     memset(&p, 0, sizeof(p));
     p.steps = g.steps;
+    const Scales scales = scales_of(g, false);
     p.a = g.a;
-    p.b = g.b;
-    p.c = g.c;
+    p.b = g.b * (scales.b / scales.a);
+    p.c = g.c * (scales.b / (scales.a * scales.a));
     p.eps = g.eps;
+    p.scale = scales.x;
+    p.to_a = scales.a / (scales.x * scales.x);
+    p.from_b = 1.0f / scales.b;
     p.rule = {g.momentum, g.nesterov};
     int64_t in_launch = 0;
     auto flush = [&]() -> int {
@@ -1064,17 +1110,6 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
   for (int from = 0, to; from < g.n; from = to) {
     const int n = gather_shapes(g, from, shapes, &to);
     if (n == 0) continue;
-    Buffers b;
-    layout(shapes, n, static_cast<char*>(g.workspace), &b);
-    if (b.counter_bytes) CG_CUDA(cudaMemsetAsync(b.counters, 0, b.counter_bytes, s));
-    if (momentum) rc = prepare<float, true>(g, from, to, shapes, n, b, s);
-    else if (g.dtype == CG_F32) rc = prepare<float, false>(g, from, to, shapes, n, b, s);
-    else if (g.dtype == CG_F16) rc = prepare<__half, false>(g, from, to, shapes, n, b, s);
-    else rc = prepare<__nv_bfloat16, false>(g, from, to, shapes, n, b, s);
-    if (rc) return rc;
-    float rate[kGroups];
-    for (int i = 0; i < n; ++i) rate[i] = rate_of(g, momentum, shapes[i].rows, shapes[i].cols);
-    const float keep = momentum ? 1.0f - g.lr * g.weight_decay : 0.0f;
     // Results that are rounded to half precision, or added to weights a
     // hundredth to a thousandth part at a time, are formed a little less exactly
     // (about 1e-5 relative on strongly decaying spectra instead of 5e-6): B
@@ -1083,16 +1118,28 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     // products run further ahead of the epilogue: an update product of the 85M step takes
     // 273 us against 350.
     const bool coarse = momentum || g.dtype != CG_F32;
+    const Scales scales = scales_of(g, coarse);
+    Buffers b;
+    layout(shapes, n, static_cast<char*>(g.workspace), &b);
+    if (b.counter_bytes) CG_CUDA(cudaMemsetAsync(b.counters, 0, b.counter_bytes, s));
+    if (momentum) rc = prepare<float, true>(g, from, to, shapes, n, b, scales.x, s);
+    else if (g.dtype == CG_F32) rc = prepare<float, false>(g, from, to, shapes, n, b, scales.x, s);
+    else if (g.dtype == CG_F16) rc = prepare<__half, false>(g, from, to, shapes, n, b, scales.x, s);
+    else rc = prepare<__nv_bfloat16, false>(g, from, to, shapes, n, b, scales.x, s);
+    if (rc) return rc;
+    float rate[kGroups];
+    for (int i = 0; i < n; ++i) rate[i] = rate_of(g, momentum, shapes[i].rows, shapes[i].cols);
+    const float keep = momentum ? 1.0f - g.lr * g.weight_decay : 0.0f;
     Plan plans[3];
     for (int i = 0; i < 3; ++i) plans[i] = plan_of(shapes, n, (Step)i, coarse);
     for (int t = 0; t < g.steps; ++t) {
       const bool odd = t & 1, last = t == g.steps - 1;
-      if ((rc = product<SplitEpi>(g, shapes, n, kGram, plans, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
-      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, plans, b, coarse, odd, false, 0.0f, nullptr, s))) return rc;
-      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, plans, b, coarse, odd, false, 0.0f, nullptr, s);
-      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
-      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
-      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, plans, b, coarse, odd, true, keep, rate, s);
+      if ((rc = product<SplitEpi>(g, shapes, n, kGram, plans, b, scales, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if ((rc = product<SplitEpi>(g, shapes, n, kPoly, plans, b, scales, coarse, odd, false, 0.0f, nullptr, s))) return rc;
+      if (!last) rc = product<SplitEpi>(g, shapes, n, kUpdate, plans, b, scales, coarse, odd, false, 0.0f, nullptr, s);
+      else if (g.dtype == CG_F32) rc = product<FinalEpi<float>>(g, shapes, n, kUpdate, plans, b, scales, coarse, odd, true, keep, rate, s);
+      else if (g.dtype == CG_F16) rc = product<FinalEpi<__half>>(g, shapes, n, kUpdate, plans, b, scales, coarse, odd, true, keep, rate, s);
+      else rc = product<FinalEpi<__nv_bfloat16>>(g, shapes, n, kUpdate, plans, b, scales, coarse, odd, true, keep, rate, s);
       if (rc) return rc;
     }
   }

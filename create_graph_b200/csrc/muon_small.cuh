@@ -46,7 +46,9 @@ struct Run {
 struct Args {
   Run run[kRuns];
   int runs, steps;
-  float a, b, c, eps;
+  float a, b, c, eps;  // b and c as factors of A's planes and of their square in B's
+  float scale;         // of X's planes
+  float to_a, from_b;  // X's planes' square to A's planes, B's planes to B
   Momentum rule;
 };
 
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
   half::cluster_sync_all();
   double total = 0.0;
   for (int r = 0; r < ranks; ++r) total += sums[r];
-  const PlaneScale scaled = plane_scale(total, p.eps);
+  const PlaneScale scaled = plane_scale(total, p.eps, p.scale);
 #pragma unroll
   for (int g = 0; g < kGroupsOf4; ++g) {
     const int at = g * kThreads + tid;
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
     float v[32];
     tmem_load_32(acc, v);
     if (ranks == 1) {
-      blend_row<false, true>(A, row, col0, One{0.0f}, 1.0f / kScale, v);
+      blend_row<false, true>(A, row, col0, One{0.0f}, p.to_a, v);
     } else {
       put_row(part, row, col0, v);
       half::cluster_sync_all();
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
           x[3] += f.w;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= 1.0f / kScale;
+        for (int e = 0; e < 4; ++e) x[e] *= p.to_a;
         uint2 h, l;
         split4(x, h, l);
         const uint32_t to = smem_u32(A + plane_at(r, 4 * g));
@@ -352,25 +354,25 @@ __global__ void __launch_bounds__(kThreads, 1) newton_schulz_small_kernel(const 
     Each factor;
     float more;
     product(A, false, A, false, [&] {  // b + c (d_row + d_column), and the diagonal's own term
-      const float beta = p.c / kScale, mine = diagonal[row], alpha = p.b + beta * mine;
+      const float c = p.c, mine = diagonal[row], alpha = p.b + c * mine;
       more = mine * alpha;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         const float4 d = *reinterpret_cast<const float4*>(diagonal + col0 + 4 * g);
-        factor.f[2 * g] = fma2(both(beta), make_float2(d.x, d.y), both(alpha));
-        factor.f[2 * g + 1] = fma2(both(beta), make_float2(d.z, d.w), both(alpha));
+        factor.f[2 * g] = fma2(both(c), make_float2(d.x, d.y), both(alpha));
+        factor.f[2 * g + 1] = fma2(both(c), make_float2(d.z, d.w), both(alpha));
       }
     });
     tmem_load_32(acc, v);
-    blend_row<true, true>(A, row, col0, factor, p.c / kScale, v);
+    blend_row<true, true>(A, row, col0, factor, p.c, v);
     if (on_diagonal) put_plane_value(A, row, more + plane_value(A, row));
     if (wide) product(A, false, Z, true, nothing);
     else product(Z, false, A, false, nothing);
     tmem_load_32(acc, v);
     if (t + 1 < p.steps) {
-      blend_row<true, true>(Z, row, col0, One{p.a}, 1.0f / kScale, v);
+      blend_row<true, true>(Z, row, col0, One{p.a}, p.from_b, v);
     } else {
-      blend_row<true, false>(Z, row, col0, One{p.a / kScale}, 1.0f / (kScale * kScale), v);
+      blend_row<true, false>(Z, row, col0, One{p.a / p.scale}, p.from_b / p.scale, v);
       put_row(part, row, col0, v);
     }
   }

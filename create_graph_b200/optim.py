@@ -114,7 +114,8 @@ def newton_schulz(x: Tensor, steps: int = 5, coefficients: tuple[float, float, f
     (from the right when m > n). float32, float16 or bfloat16 in and out; the
     iteration itself runs at fp32-level accuracy whatever the type, because it
     multiplies the error of the weak directions by a in every step. A matrix of
-    zeros stays zero. Not differentiable."""
+    zeros stays zero. Coefficients that let X, A or the polynomial grow beyond 10^9
+    on the way overflow to NaN. Not differentiable."""
     native.refuse_tangents("newton_schulz", x)
     native.require_cuda(x)
     if x.dim() < 2:

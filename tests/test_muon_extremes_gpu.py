@@ -70,3 +70,26 @@ def test_muon_step_on_zero_gradients(shape):
     opt = FusedMuon(FlatGradients([p], None), lr=0.5, weight_decay=0.5, eps=1e-38)
     opt.step()
     assert torch.equal(p.detach(), w * 0.75)
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-5), (torch.bfloat16, 2.0**-8 + 1e-5)])
+@pytest.mark.parametrize("coefficients,steps", [((18.0, 0.0, 0.0), 2), ((18.0, 0.0, 0.0), 3), ((17.0, -20.0, 4.0), 2),
+                                                ((4.5, -4.0, 3.0), 2), ((-20.0, 3.0, 0.0), 2)])
+@pytest.mark.parametrize("shape", [(1, 1), *SHAPES])
+def test_coefficients_that_let_the_iteration_grow(shape, coefficients, steps, dtype, tol):
+    """X, A or B beyond 16: a matrix of one direction, whose singular value is 1, and a
+    random one. To first order, along that direction's path from s = 1: the polynomial
+    p multiplies a relative error by |s p'(s) / p(s)|, and a step adds 2^-22 for every
+    factor of its terms a X, b X X' X and c X X' X X' X, relative to p(s)."""
+    a, b, c = coefficients
+    s, error = 1.0, 2.0**-22
+    for _ in range(steps):
+        p = a * s + b * s**3 + c * s**5
+        factors = abs(a * s) + 3 * abs(b * s**3) + 5 * abs(c * s**5)
+        error = abs(s * (a + 3 * b * s**2 + 5 * c * s**4) / p) * error + factors / abs(p) * 2.0**-22
+        s = p
+    one = random(shape[0], 1, seed=4) @ random(1, shape[1], seed=5)
+    for x, e in ((one, error), (random(*shape, seed=6), error if min(shape) == 1 else 0.0)):
+        x = x.to(dtype)
+        got = newton_schulz(x, steps=steps, coefficients=coefficients)
+        assert rel(got, orthogonalised(x, steps, coefficients)) < tol + e
