@@ -735,6 +735,10 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(Padded a, Padded b) {
 // ---- host side ---------------------------------------------------------------------
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+static bool known_act(int act) {
+  return act == CG_ACT_NONE || act == CG_ACT_SILU || act == CG_ACT_RELU || act == CG_ACT_GELU;
+}
+
 struct Plan {
   int cg, bn;
   int splits[2], kt_per[2];
@@ -957,8 +961,7 @@ static int run_typed(const cg_linear_args* g, int count, void* workspace, int64_
 
 static int checked(const cg_linear_args& g) {
   CG_REQUIRE(g.dtype == CG_F16 || g.dtype == CG_BF16, "linear_half: dtype %d is neither CG_F16 nor CG_BF16", g.dtype);
-  CG_REQUIRE(g.act == CG_ACT_NONE || g.act == CG_ACT_SILU || g.act == CG_ACT_RELU || g.act == CG_ACT_GELU,
-             "linear_half: bad act %d", g.act);
+  CG_REQUIRE(known_act(g.act), "linear_half: bad act %d", g.act);
   CG_REQUIRE(g.m >= 1 && g.n >= 1 && g.k >= 1, "linear_half: sizes must be at least 1");
   const int64_t most = (1ll << 31) - 512;  // tile coordinates are 32-bit
   CG_REQUIRE(g.m < most && g.n < most && g.k < most, "linear_half: size too large");
@@ -1036,6 +1039,7 @@ static int act_grad_run(const cg_act_grad_args* args, void* stream) {
   const cg_act_grad_args& g = *args;
   CG_REQUIRE(g.dtype == CG_F16 || g.dtype == CG_BF16, "act_grad_half: dtype %d is neither CG_F16 nor CG_BF16",
              g.dtype);
+  CG_REQUIRE(known_act(g.act), "act_grad_half: bad act %d", g.act);
   CG_REQUIRE(g.rows >= 0 && g.cols >= 0 && g.rows < (1ll << 31) - 512 && g.cols < (1ll << 31) - 512,
              "act_grad_half: bad size");
   if (g.rows == 0 || g.cols == 0) {
@@ -1103,6 +1107,7 @@ static int64_t backward_workspace(const cg_linear_backward_args& g) {
 static int backward_run(const cg_linear_backward_args* args, void* stream) {
   CG_REQUIRE(args != nullptr, "linear_half_backward: args is NULL");
   const cg_linear_backward_args& g = *args;
+  CG_REQUIRE(known_act(g.act), "linear_half_backward: bad act %d", g.act);
   CG_REQUIRE(g.m >= 1 && g.n >= 1 && g.k >= 1, "linear_half_backward: sizes must be at least 1");
   CG_REQUIRE(g.workspace_bytes >= backward_workspace(g) &&
                  (backward_workspace(g) == 0 || (g.workspace != nullptr && aligned16(g.workspace))),
@@ -1205,6 +1210,7 @@ int cg_act_grad2_half(const void* h, const void* hb, const void* gy, const void*
                       int64_t cols, int act, int dtype, void* stream) {
   using namespace cg;
   CG_REQUIRE(dtype == CG_F16 || dtype == CG_BF16, "act_grad2_half: dtype %d is neither CG_F16 nor CG_BF16", dtype);
+  CG_REQUIRE(dense::known_act(act), "act_grad2_half: bad act %d", act);
   CG_REQUIRE(rows >= 0 && cols >= 0 && cols < (1ll << 31), "act_grad2_half: bad size");
   if (rows == 0 || cols == 0) return kOk;
   CG_REQUIRE((h || hb) && gy && z && dgy && dz, "act_grad2_half: null buffer");
