@@ -385,7 +385,8 @@ def dense_linear(x: Tensor, w: Tensor, b: Tensor | None, r: Tensor | None, activ
     act = dense._checked(x, w, b, r, activation)
     if x.dim() != 2:
         raise NativeError(f"dense_linear: x must be a matrix, got {tuple(x.shape)}")
-    return dense.product(x, w, b, act, r, keep_z=True)
+    with torch.cuda.device(x.get_device()):
+        return dense.product(x, w, b, act, r, keep_z=True)
 
 
 @dense_linear.register_fake
@@ -397,7 +398,8 @@ def _dense_linear_fake(x, w, b, r, activation):
 def act_grad(gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """(gy f'(z), the sums of its columns) of (M, N) half-precision tensors."""
     act = dense._checked_matrix("act_grad", gy, activation, z)
-    gz, db = dense._act_grad(gy, z, act, True)
+    with torch.cuda.device(gy.get_device()):
+        gz, db = dense._act_grad(gy, z, act, True)
     return (gy.clone() if gz.data_ptr() == gy.data_ptr() else gz.contiguous()), db
 
 
@@ -409,7 +411,9 @@ def _act_grad_fake(gy, z, activation):
 @torch.library.custom_op("cg_b200::act_grad2", mutates_args=())
 def act_grad2(h: Tensor, hb: Tensor, gy: Tensor, z: Tensor, activation: str) -> tuple[Tensor, Tensor]:
     """((h + hb) f'(z), (h + hb) gy f''(z)) for cotangents h, hb of act_grad's outputs."""
-    return dense._act_grad2(h, hb, gy, z, dense._checked_matrix("act_grad2", gy, activation, h, hb, z))
+    act = dense._checked_matrix("act_grad2", gy, activation, h, hb, z)
+    with torch.cuda.device(gy.get_device()):
+        return dense._act_grad2(h, hb, gy, z, act)
 
 
 @act_grad2.register_fake

@@ -109,6 +109,34 @@ def test_any_layout_of_the_pre_activation_is_read_by_rows(calls):
     assert calls[1][1].z == wide.data_ptr() and calls[1][1].ld_z == 20
 
 
+def test_launches_on_the_tensors_own_device(monkeypatch):
+    """Every launch happens with the device of the tensors current: the default
+    stream has the same handle on all of them."""
+    current, launched = [], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(native, "invoke", lambda name, *a, **k: launched.append((name, tuple(current))))
+    monkeypatch.setattr(native, "lib", lambda: Scratch)
+    monkeypatch.setattr(native, "require_cuda", lambda *ts: None)
+    monkeypatch.setattr(dense, "_stream", lambda t: 0)
+    monkeypatch.setattr(dense, "_workspace_bytes", lambda *a: 0)
+    ops.act_grad(GY, GY.clone(), "silu")
+    ops.act_grad2(GY, GY[0].clone(), GY.clone(), GY.clone(), "silu")
+    ops.dense_linear(GY, GY.clone(), None, None, "silu")
+    index = GY.get_device()  # -1: the host's, which stands for the GPU's here
+    assert launched == [(name, (index,)) for name in ("cg_act_grad_half", "cg_act_grad2_half", "cg_linear_half")]
+
+
 @pytest.mark.gpu
 def test_layouts_on_the_gpu():
     gen = torch.Generator().manual_seed(3)
