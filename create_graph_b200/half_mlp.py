@@ -66,15 +66,17 @@ class HalfMLPModel(nn.Module):
 
 class Trainer:
     """The training step: gradients, then one Muon update of the hidden matrices
-    and one AdamW update of the rest, each over its own flat buffers."""
+    (a network of one layer has none) and one AdamW update of the rest, each over
+    its own flat buffers."""
 
     def __init__(self, model: HalfMLPModel, world: int | None = None, lr: float = 1e-2):
         matrices = [layer.weight for layer in model.network.rest]
         kept = {id(p) for p in matrices}
         others = [p for p in model.parameters() if id(p) not in kept]
         self.model = model
-        self.grads = [FlatGradients(matrices, world), FlatGradients(others, world)]
-        self.optimizers = [FusedMuon(self.grads[0], lr=lr), FusedAdamW(self.grads[1], lr=lr)]
+        groups = [(make, params) for make, params in ((FusedMuon, matrices), (FusedAdamW, others)) if params]
+        self.grads = [FlatGradients(params, world) for _, params in groups]
+        self.optimizers = [make(grads, lr=lr) for (make, _), grads in zip(groups, self.grads)]
 
     def step(self, batch: dict, e_target: Tensor, f_target: Tensor) -> Tensor:
         for g in self.grads:
