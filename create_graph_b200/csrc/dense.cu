@@ -203,43 +203,40 @@ __device__ __forceinline__ float2 gelu2(float2 z) {
 // to 1e-17 or 1, its limits at the infinities, so a pre-activation that left the
 // range of its type and was kept as -infinity (fp16 below -65504) has the gradient
 // 0 that goes with its output 0. silu's 1 - s is off by an ulp, times z: 5e-6 at
-// the most.
+// the most. One reciprocal each: these passes wait for memory, not for the special
+// function unit, and neither value depends on the other.
+__device__ __forceinline__ float2 rcp_each(float2 d) { return make_float2(rcp_approx(d.x), rcp_approx(d.y)); }
 __device__ __forceinline__ float2 silu_grad2(float2 z) {
   const float2 x = mul2(z, both(-kLog2e));
-  const float2 e = make_float2(exp2_approx(fminf(x.x, 62.0f)), exp2_approx(fminf(x.y, 62.0f)));
-  const float2 s = rcp2(fma2(e, both(1.0f), both(1.0f)));
+  const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+  const float2 s = rcp_each(fma2(e, both(1.0f), both(1.0f)));
   // s (1 + z (1 - s)) = s + (z s - z s s)
   const float2 zs = mul2(z, s);
   return fma2(fma2(zs, make_float2(-s.x, -s.y), zs), both(1.0f), s);
 }
 __device__ __forceinline__ float2 gelu_grad2(float2 z) {
-  const float2 a = make_float2(fminf(fabsf(z.x), 64.0f), fminf(fabsf(z.y), 64.0f));
-  const float2 t = rcp2(fma2(a, both(0.3275911f * 0.70710678f), both(1.0f)));
-  const float2 u = mul2(mul2(a, a), both(-0.5f * kLog2e));
+  constexpr float kP = 0.3275911f * 0.70710678f;
+  const float2 t = rcp_each(make_float2(fmaf(fabsf(z.x), kP, 1.0f), fmaf(fabsf(z.y), kP, 1.0f)));
+  const float2 u = mul2(mul2(z, z), both(-0.5f * kLog2e));
   const float2 e = make_float2(exp2_approx(u.x), exp2_approx(u.y));
   float2 p = fma2(t, both(0.5307027145f), both(-0.7265760135f));
   p = fma2(t, p, both(0.7107068705f));
   p = fma2(t, p, both(-0.142248368f));
   p = fma2(t, p, both(0.127414796f));
-  const float2 tail = mul2(mul2(p, t), e);
   // Phi(z) = 1/2 + sign(z) (1/2 - tail)
-  const float2 phi = make_float2(0.5f + copysignf(0.5f - tail.x, z.x), 0.5f + copysignf(0.5f - tail.y, z.y));
-  return fma2(mul2(z, both(kInvSqrt2Pi)), e, phi);
+  const float2 h = fma2(mul2(p, t), make_float2(-e.x, -e.y), both(0.5f));
+  const float2 signed_h = make_float2(copysignf(h.x, z.x), copysignf(h.y, z.y));
+  return fma2(fma2(mul2(z, both(kInvSqrt2Pi)), e, both(0.5f)), both(1.0f), signed_h);
 }
-// f' of one value.
+// f' of one value within the same bounds.
 __device__ __forceinline__ float act_grad(float z, int kind) {
-  if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  z = hold_nan(z, kFar);
-  if (kind == CG_ACT_SILU) {
-    const float s = sigmoid(z);
-    return s * (1.0f + z * (1.0f - s));
-  }
+  if (kind == CG_ACT_SILU) return silu_grad2(both(z)).x;
   if (kind == CG_ACT_GELU) return gelu_grad2(both(z)).x;
+  if (kind == CG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
 }
-// f'' of one value, with z held as in f': its square would leave fp32.
+// f'' of one value within the same bounds, where its square stays in fp32.
 __device__ __forceinline__ float act_grad2(float z, int kind) {
-  z = hold_nan(z, kFar);
   if (kind == CG_ACT_SILU) {
     const float s = sigmoid(z);
     return s * (1.0f - s) * (2.0f + z * (1.0f - 2.0f * s));
@@ -577,8 +574,8 @@ __global__ void join_splits_kernel(const __grid_constant__ EpiArgs a, int splits
 
 // ---- elementwise passes of the derivatives -----------------------------------------
 // Bound by HBM: three streams of rows x cols values (65536 x 3072 bf16: 1.2 GB with
-// silu in 195 us, 6.2 TB/s, 94% of the measured copy rate, with gelu in 209 us;
-// 8280 x 3072 31 and 34 us).
+// silu in 199 us, 6.1 TB/s, 93% of the measured copy rate, with gelu in 212 us;
+// 8280 x 3072 32 and 34 us).
 // gz = gy f'(z) and the column sums of gz (the bias gradient) in one pass over
 // gy and z: block (x, y) owns 32 x V columns and the rows of chunk y; its eight
 // warps walk the rows, each lane adding up V columns in fp32, and the warps'
@@ -655,7 +652,7 @@ __global__ void __launch_bounds__(256, V == 8 && ALIGNED ? 4 : 1) act_grad_kerne
     for (int64_t r = r0 + warp; r < r1; r += 8) {
       float g[1] = {to_float(gy[r * ld_gy + col])};
       if (gz) {
-        const float x[1] = {to_float(z[r * ld_z + col])};
+        const float x[1] = {hold_nan(to_float(z[r * ld_z + col]), kFar)};
         act_grad_all(g, x, kind);
         gz[r * ld_gz + col] = from_float<T>(g[0]);
       }
@@ -699,7 +696,7 @@ __global__ void act_grad2_kernel(const T* __restrict__ h, const T* __restrict__ 
   const int64_t n = rows * cols, stride = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += stride) {
     const float t = (h ? to_float(h[i]) : 0.0f) + (hb ? to_float(hb[i % cols]) : 0.0f);
-    const float x = to_float(z[i]);
+    const float x = hold_nan(to_float(z[i]), kFar);
     dgy[i] = from_float<T>(t * act_grad(x, kind));
     dz[i] = from_float<T>(t * to_float(gy[i]) * act_grad2(x, kind));
   }
