@@ -54,6 +54,11 @@ def _fits_tma(t: Tensor, row: int, col: int) -> bool:
         and t.data_ptr() % 16 == 0
 
 
+def _matrix_like(t: Tensor, like: Tensor) -> Tensor:
+    """An uninitialised contiguous matrix of t's shape."""
+    return torch.empty_like(t) if t.is_contiguous() else like.new_empty(t.shape)
+
+
 def _stream(t: Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
@@ -99,21 +104,23 @@ def _operands(*ts: Tensor) -> tuple[list, Tensor | None]:
     return ops, flat
 
 
-def _saved_operands(ops, flat: Tensor | None, *ts: Tensor) -> tuple[list, Tensor | None]:
+def _saved_operands(ops, strides, flat: Tensor | None, x: Tensor, w: Tensor) -> tuple[list, Tensor | None]:
     """The forward's operands as a backward may read them from the saved tensors:
     a copy where the forward left it in the buffer; a tensor that was read in
-    place asked for its layout again, since a saved-tensor hook (save_on_cpu, or
-    any pack that clones) may give it back in another one."""
-    if flat is None or (flat.is_contiguous() and flat.data_ptr() % 16 == 0):
-        ops = [_in_place(t) if op[0] is None else op for op, t in zip(ops, ts)]
-        if None not in ops:
-            return ops, flat
-    return _operands(*ts)
+    place as then, or asked for its layout again where a saved-tensor hook
+    (save_on_cpu, or any pack that clones) gave it back in another one."""
+    if flat is not None:
+        if not flat.is_contiguous() or flat.data_ptr() % 16 != 0:
+            return _operands(x, w)
+    elif x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0 and (x.stride(), w.stride()) == strides:
+        return ops, None  # the usual case
+    ops = [_in_place(t) if op[0] is None else op for op, t in zip(ops, (x, w))]
+    return _operands(x, w) if None in ops else (ops, flat)
 
 
 def _require(what: str, t: Tensor, shape: tuple[int, ...], like: Tensor) -> None:
     """Refuse a tensor that the kernels would misread (its strides may be any)."""
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != shape or t.dtype is not like.dtype or t.device != like.device:
         raise NativeError(f"{what} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(shape)} {like.dtype} "
                           f"on {like.device}")
 
@@ -187,31 +194,33 @@ def product(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: int = 
 def _backward(gy, z, x, w, ops, flat, shape, activation, want_dx, want_dw, want_db):
     """(dx, dw, db) in one call; None for what is not wanted."""
     m, n, k = shape
+    pitch = -(-n // 8) * 8
     args = native.LinearBackwardArgs()
     args.m, args.n, args.k, args.act, args.dtype = m, n, k, activation, native.HALF_DTYPES[gy.dtype]
     gz = None
     if activation == native.ACT_NONE:
         if _fits_tma(gy, 0, 1):
-            args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else -(-n // 8) * 8
+            args.gy, args.ld_gy = gy.data_ptr(), gy.stride(0) if m > 1 else pitch
         else:
             # rows on 16-byte boundaries, whatever other layout would do
             gy = gy.contiguous()
-            args.ld_gy = -(-n // 8) * 8
-            kept = gy.new_empty(m * args.ld_gy)
-            args.gy = kept.data_ptr()
-            native.invoke("cg_pad_rows_half", gy.data_ptr(), n, m, n, args.gy, args.ld_gy, None, 0, 0, 0, None, 0,
+            kept = gy.new_empty(m * pitch)
+            args.gy, args.ld_gy = kept.data_ptr(), pitch
+            native.invoke("cg_pad_rows_half", gy.data_ptr(), n, m, n, args.gy, pitch, None, 0, 0, 0, None, 0,
                           _stream(gy))
     else:
-        gy = _rows(gy)
-        gz = _pitched(m, n, gy)
-        z = _rows(z)
-        args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride(0), n)
-        args.z, args.ld_z = z.data_ptr(), max(z.stride(0), n)
-        args.gz, args.ld_gz = gz.data_ptr(), -(-n // 8) * 8
+        if not gy.is_contiguous():
+            gy = _rows(gy)
+        if not z.is_contiguous():
+            z = _rows(z)
+        gz = torch.empty_like(z) if pitch == n and z.is_contiguous() else gy.new_empty((m, pitch))
+        args.gy, args.ld_gy = gy.data_ptr(), max(gy.stride()[0], n)
+        args.z, args.ld_z = z.data_ptr(), max(z.stride()[0], n)
+        args.gz, args.ld_gz = gz.data_ptr(), pitch
     (_, args.ld_x, args.x_mn_major), (_, args.ld_w, args.w_mn_major) = ops
     args.x, args.w = _address(x, ops[0], flat), _address(w, ops[1], flat)
-    dx = gy.new_empty((m, k)) if want_dx else None
-    dw = gy.new_empty((n, k)) if want_dw else None
+    dx = _matrix_like(x, gy) if want_dx else None
+    dw = _matrix_like(w, gy) if want_dw else None
     db = gy.new_empty(n) if want_db else None
     args.dx, args.dw, args.db = native.ptr(dx), native.ptr(dw), native.ptr(db)
     nbytes = _backward_workspace_bytes(m, n, k, activation, want_dx, want_dw, want_db)
@@ -337,17 +346,17 @@ class _Linear(_Fused):
             y, z = product(x, w, b, activation, r, keep_z)
         else:
             ctx.operands, flat = _operands(x, w)
+            ctx.strides = x.stride(), w.stride()
             y, z = _forward(x, w, ctx.operands, flat, ctx.shape, b, activation, r, keep_z)
         ctx.save_for_backward(x, w, z, flat)
         ctx.inputs = (True, True, b is not None)
         return y, z
 
     @staticmethod
-    def _wanted(ctx):
+    def _wanted(ctx, need, recording):
         """Which of x, w, b the backward pass running now needs."""
-        need = ctx.needs_input_grad[:3]
         m, n, k = ctx.shape
-        if 2.0 * m * n * k < _SMALL_FLOPS and not torch.is_grad_enabled():
+        if 2.0 * m * n * k < _SMALL_FLOPS and not recording:
             return need
         nodes = iter(ctx.next_functions)
         nodes = [next(nodes)[0] if given else None for given in ctx.inputs]
@@ -357,19 +366,23 @@ class _Linear(_Fused):
     def backward(ctx, gy, gz_direct):
         x, w, z, flat = ctx.saved_tensors
         native.refuse_tangents("dense.linear", gy, gz_direct, x, w, z)
-        want = _Linear._wanted(ctx)
-        dr = gy if ctx.needs_input_grad[3] else None
-        if not torch.is_grad_enabled() and gz_direct is None and gy is not None and ctx.operands is not None:
+        *need, need_dr, _ = ctx.needs_input_grad
+        recording = torch.is_grad_enabled()
+        want = _Linear._wanted(ctx, need, recording)
+        dr = gy if need_dr else None
+        if not recording and gz_direct is None and gy is not None and ctx.operands is not None:
             if not any(want):
                 return None, None, None, dr, None
             m, n, k = ctx.shape
-            _require("dense.linear: saved tensor x", x, (m, k), gy)
-            _require("dense.linear: saved tensor weight", w, (n, k), gy)
+            like = gy.dtype, gy.get_device()
+            if x.shape != (m, k) or w.shape != (n, k) or (x.dtype, x.get_device()) != like or \
+                    (w.dtype, w.get_device()) != like:
+                _require("dense.linear: saved tensor x", x, (m, k), gy)
+                _require("dense.linear: saved tensor weight", w, (n, k), gy)
             if z is not None:
                 _require("dense.linear: saved tensor z", z, (m, n), gy)
-            ops, flat = _saved_operands(ctx.operands, flat, x, w)
-            grads = _backward(gy, z, x, w, ops, flat, ctx.shape, ctx.activation, *want)
-            return *grads, dr, None
+            ops, flat = _saved_operands(ctx.operands, ctx.strides, flat, x, w)
+            return *_backward(gy, z, x, w, ops, flat, ctx.shape, ctx.activation, *want), dr, None
         # the differentiable path: products and passes that record their own backward
         gz, db = gz_direct, None
         if gy is not None and any(want):
