@@ -449,8 +449,8 @@ struct BlockEpi : EpiBase {
 // the block is transposed through shared memory and stored one column per lane
 // (z the same way before the activation); the residual of a 32 x 32 block is read
 // before the accumulator is waited for. 4099 x 1031 x 515 fp16 with gelu, residual
-// and z: 41 us (47 with the activation applied value by value behind the
-// transpose), its gradients dx + dW 39 us (47), against 8 us of bytes: the
+// and z: 42 us (47 with the activation applied value by value behind the
+// transpose), its gradients dx + dW 40 us (47), against 8 us of bytes: the
 // two-byte stores, 64 bytes a warp and across sectors, are what is left.
 template <class T>
 struct PlainEpi : EpiBase {
@@ -688,7 +688,8 @@ __global__ void join_columns_kernel(const float* __restrict__ partial, int chunk
   db[c] = from_float<T>(s);
 }
 
-// Second order: t = h + hb; dgy = t f'(z), dz = t gy f''(z).
+// Second order: t = h + hb; dgy = t f'(z), dz = t gy f''(z). Value by value: 8280 x
+// 3072 in 136 us, 1.9 TB/s, bound by its two-byte accesses and their indices.
 template <class T>
 __global__ void act_grad2_kernel(const T* __restrict__ h, const T* __restrict__ hb, const T* __restrict__ gy,
                                  const T* __restrict__ z, T* __restrict__ dgy, T* __restrict__ dz, int64_t rows,

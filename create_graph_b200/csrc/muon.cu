@@ -20,11 +20,12 @@
 // A and B are symmetric: only tiles that reach the lower triangle are formed,
 // and their epilogue stores each value at both places.
 // Matrices of one shape are one batch; all shapes of a call share each launch.
-// What bounds it: many large matrices (the 85M model's 48: 3.6 ms a step) the
-// three products, an update launch running at 1.35 PFLOP/s of plane products and
-// a gram launch at 1.2 (its tiles cross the diagonal); one matrix (3072 x 768:
-// 207 us) the chain of 15 launches, each 10 to 15 us of which 3 to 4 are the
-// way from one launch's end to the next one's first product.
+// What bounds it: many large matrices (the 85M model's 48: 3.2 ms a step alone, 3.7
+// back to back under the power limit) the three products, an update launch
+// running at 1.35 PFLOP/s of plane products and a gram launch at 1.2 (its tiles
+// cross the diagonal); one matrix (3072 x 768: 209 us) the chain of 15 launches,
+// each 10 to 15 us of which 3 to 4 are the way from one launch's end to the next
+// one's first product.
 #include "half_gemm.cuh"
 #include "../../include/cg_b200.h"
 
@@ -1112,7 +1113,8 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     if (n == 0) continue;
     // Results that are rounded to half precision, or added to weights a
     // hundredth to a thousandth part at a time, are formed a little less exactly
-    // (about 1e-5 relative on strongly decaying spectra instead of 5e-6): B
+    // (1e-6 to 6e-6 relative, 1e-5 on strongly decaying spectra, instead of 1e-6
+    // and 3e-6; torch's fp32 products 3e-6 and 5e-6): B
     // carries a on its diagonal, so that X <- B X reads no X beside its operand,
     // and accumulators run for four k-slices instead of one or two, so that the
     // products run further ahead of the epilogue: an update product of the 85M step takes

@@ -18,7 +18,9 @@ with gz and db formed in one pass over gy and the kept pre-activation z, the
 gradients as products of the same kernel, and the second order (f'') as an
 explicit kernel. gz is rounded to the layer's dtype before the two products,
 as every operand of the tensor cores is. Without a gradient to prepare, z is
-not written. The fp32 layers of the energy network are in
+not written. NaN stays NaN; at infinite pre-activations, also ones beyond the
+type's range, f, f' and f'' take their limits. Third and forward-mode
+derivatives are refused. The fp32 layers of the energy network are in
 ``create_graph_b200.nn``.
 """
 

@@ -495,7 +495,8 @@ int cg_neighbor_list(const float* pos, const int32_t* sys_ptr, int64_t n_systems
  * Newton-Schulz orthogonalisation of matrices, and the optimizer step on it:
  *   X = G / max(|G|_F, eps); `steps` times
  *   A = X X^T, B = b A + c A A, X = a X + B X   (X^T X and X B when rows > cols)
- * at fp32-level accuracy (pairs of fp16 planes, three products each).
+ * at fp32-level accuracy (pairs of fp16 planes, three products each). X, A or B
+ * growing beyond 10^9 on the way overflow to NaN.
  * cg_newton_schulz: out = X for every matrix; x and out have the type `dtype`
  * (CG_F32, CG_F16 or CG_BF16) and may be the same memory.
  * cg_muon_step (fp32): with g = x and m = momentum,
