@@ -1114,11 +1114,10 @@ static int run(const cg_ns_args& g, bool momentum, void* stream) {
     // Results that are rounded to half precision, or added to weights a
     // hundredth to a thousandth part at a time, are formed a little less exactly
     // (1e-6 to 6e-6 relative, 1e-5 on strongly decaying spectra, instead of 1e-6
-    // and 3e-6; torch's fp32 products 3e-6 and 5e-6): B
-    // carries a on its diagonal, so that X <- B X reads no X beside its operand,
-    // and accumulators run for four k-slices instead of one or two, so that the
-    // products run further ahead of the epilogue: an update product of the 85M step takes
-    // 273 us against 350.
+    // and 3e-6; torch's fp32 products 3e-6 and 5e-6): B carries a on its diagonal,
+    // so that X <- B X reads no X beside its operand, and accumulators run for four
+    // k-slices instead of one or two, so that the products run further ahead of the
+    // epilogue: an update product of the 85M step takes 273 us against 350.
     const bool coarse = momentum || g.dtype != CG_F32;
     const Scales scales = scales_of(g, coarse);
     Buffers b;
